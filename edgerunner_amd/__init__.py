@@ -13,10 +13,13 @@ from .runtime import (AllocationFailed, Buffer, Capture, Context, Graph, Dequant
                       UnsupportedDataType, MmapFailed, MissingMetadata, TensorNotFound)
 from .gemv import (DequantQ4KMKernel, DequantQ6KKernel, DequantQ8_0Kernel,  # noqa: F401
                    FusedQ8Kernel, GEMVKernel, QuantGEMMKernel, QuantizeQ8RowsKernel, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_0)
+from .kv8 import (HeadRows, KV8AppendKernel, KV8AttentionKernel, KV8Batch, KV8Cache, QKNormRopeKernel,  # noqa: F401
+                  Rope)
 
 __all__ = [
     "Context", "Buffer", "Stream", "Event", "Graph", "Capture", "default_context",
     "GEMVKernel", "FusedQ8Kernel", "QuantGEMMKernel", "QuantizeQ8RowsKernel", "DequantQ8_0Kernel", "DequantQ4KMKernel", "DequantQ6KKernel",
     "GEMVError", "DequantKernelError", "EdgeRunnerHIPError", "WeightLoaderError",
+    "QKNormRopeKernel", "KV8AppendKernel", "KV8AttentionKernel", "KV8Cache", "KV8Batch", "HeadRows", "Rope",
     "TYPE_Q8_0", "TYPE_Q4_K", "TYPE_Q6_K",
 ]

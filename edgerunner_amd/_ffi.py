@@ -52,6 +52,25 @@ class er_tensor_storage(C.Structure):
     ]
 
 
+class er_head_rows(C.Structure):
+    _fields_ = [("data", er_buffer), ("heads", C.c_uint32), ("row_stride", C.c_uint32)]
+
+
+class er_rope(C.Structure):
+    _fields_ = [("inv_freq", er_buffer), ("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32)]
+
+
+class er_kv8_cache(C.Structure):
+    _fields_ = [("k", er_buffer), ("v", er_buffer), ("k_scale", er_buffer), ("v_scale", er_buffer),
+                ("pages", C.c_uint32), ("kv_heads", C.c_uint32), ("page_tokens", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class er_kv8_batch(C.Structure):
+    _fields_ = [("page_table", er_buffer), ("kv_len", er_buffer), ("row_start", er_buffer),
+                ("sequences", C.c_uint32), ("table_stride", C.c_uint32), ("rows", C.c_uint32),
+                ("max_rows", C.c_uint32), ("max_kv_len", C.c_uint32)]
+
+
 class er_gguf_value(C.Structure):
     _fields_ = [
         ("type", C.c_uint32),
@@ -99,6 +118,7 @@ _event = C.c_void_p
 _graph = C.c_void_p
 _u32 = C.c_uint32
 _u64 = C.c_uint64
+_p = C.POINTER
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -186,6 +206,17 @@ SIGNATURES = {
         C.c_int, [_ctx_p, _stream, er_buffer, er_buffer, er_buffer, _u32, _u32, _u32]),
     "er_hip_gemm_q4_k": (C.c_int, [_ctx_p, _stream, er_buffer, er_buffer, er_buffer, _u32, _u32, _u32]),
     "er_hip_gemm_q8_0": (C.c_int, [_ctx_p, _stream, er_buffer, er_buffer, er_buffer, _u32, _u32, _u32]),
+    "er_hip_qk_norm_rope": (
+        C.c_int, [_ctx_p, _stream, _p(er_head_rows), _p(er_head_rows), _p(er_head_rows), _p(er_head_rows), er_buffer,
+                  er_buffer, er_buffer, _p(er_rope), _u32, _u32, C.c_float]),
+    "er_hip_kv8_append": (
+        C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_head_rows), _p(er_head_rows), _u32,
+                  _p(er_head_rows), _p(er_head_rows), er_buffer, er_buffer, _p(er_rope), C.c_float]),
+    "er_hip_kv8_attention": (
+        C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_head_rows), _p(er_head_rows), _u32,
+                  C.c_float, _u32, er_buffer]),
+    "er_hip_kv8_attention_workspace": (
+        C.c_int, [_ctx_p, _p(er_kv8_cache), _p(er_kv8_batch), _u32, C.POINTER(_u64)]),
     "er_gguf_parse_memory": (C.c_int, [C.c_void_p, C.c_uint64, _u32, C.POINTER(C.c_void_p)]),
     "er_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "er_gguf_close": (None, [C.c_void_p]),

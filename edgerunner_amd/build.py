@@ -2,7 +2,7 @@
 
 Produces (next to this file, so they travel with the source tree):
   libedgerunner_hip.so   -- the C-ABI library (include/er_hip.h, er_gguf.h) with
-                            the gfx950 code object embedded
+                            the gfx950 code objects embedded
   libedgerunner_probe.so -- the measurement library: the same sources built with
                             -DER_WITH_PROBES (every er_hip.h entry point plus
                             csrc/er_hip_probe.h); bench.py's ceilings and GEMM
@@ -42,6 +42,8 @@ PROBE_LIB = PKG / "libedgerunner_probe.so"
 SYNTH = PKG / "liber_synth.so"
 CODE_OBJECT = BUILD / "er_kernels.hsaco"
 PROBE_CODE_OBJECT = BUILD / "er_kernels_probe.hsaco"
+KV8_CODE_OBJECT = BUILD / "er_kv8.hsaco"  # the 8-bit cache's kernels, the same in both libraries
+HOST_SOURCES = ("er_hip.cpp", "er_kv8.cpp", "er_gguf.cpp")
 PROBE_DEFINES = ["-DER_WITH_PROBES=1"]
 
 
@@ -50,9 +52,9 @@ def _run(cmd: list[str]) -> None:
     subprocess.run(cmd, check=True)
 
 
-def _code_object_cmd(out: Path, extra: list[str] | None = None) -> list[str]:
+def _code_object_cmd(out: Path, extra: list[str] | None = None, source: str = "er_kernels.hip") -> list[str]:
     return [HIPCC, *DEVICE_FLAGS, *(extra or []), "--genco", "-I", str(CSRC),
-            str(CSRC / "er_kernels.hip"), "-o", str(out)]
+            str(CSRC / source), "-o", str(out)]
 
 
 def build_code_object(extra: list[str] | None = None, out: Path = CODE_OBJECT) -> Path:
@@ -61,11 +63,18 @@ def build_code_object(extra: list[str] | None = None, out: Path = CODE_OBJECT) -
     return out
 
 
-def build_code_objects() -> None:
-    """The product and the measurement code objects, compiled concurrently
-    (one hipcc process each)."""
+def build_kv8_code_object() -> Path:
     BUILD.mkdir(exist_ok=True)
-    cmds = [_code_object_cmd(CODE_OBJECT), _code_object_cmd(PROBE_CODE_OBJECT, PROBE_DEFINES)]
+    _run(_code_object_cmd(KV8_CODE_OBJECT, source="er_kv8.hip"))
+    return KV8_CODE_OBJECT
+
+
+def build_code_objects() -> None:
+    """The product and the measurement code objects and the 8-bit cache's,
+    compiled concurrently (one hipcc process each)."""
+    BUILD.mkdir(exist_ok=True)
+    cmds = [_code_object_cmd(CODE_OBJECT), _code_object_cmd(PROBE_CODE_OBJECT, PROBE_DEFINES),
+            _code_object_cmd(KV8_CODE_OBJECT, source="er_kv8.hip")]
     procs = []
     for c in cmds:
         print("+", " ".join(c), flush=True)
@@ -76,7 +85,8 @@ def build_code_objects() -> None:
 
 
 def _blob_source(code_object: Path) -> str:
-    """Assembly that embeds the code object as er_kernels_blob[_end]."""
+    """Assembly that embeds the code object as er_kernels_blob[_end] and the
+    8-bit cache's as er_kv8_blob."""
     return ("    .section .rodata\n"
             "    .balign 4096\n"
             "    .globl er_kernels_blob\n"
@@ -84,6 +94,11 @@ def _blob_source(code_object: Path) -> str:
             f"    .incbin \"{code_object}\"\n"
             "    .globl er_kernels_blob_end\n"
             "er_kernels_blob_end:\n"
+            "    .byte 0\n"
+            "    .balign 4096\n"
+            "    .globl er_kv8_blob\n"
+            "er_kv8_blob:\n"
+            f"    .incbin \"{KV8_CODE_OBJECT}\"\n"
             "    .byte 0\n"
             "    .section .note.GNU-stack,\"\",@progbits\n")
 
@@ -94,15 +109,16 @@ def build_host_library(code_object: Path = CODE_OBJECT, out: Path = LIB, defines
     blob = BUILD / f"{tag}_blob.S"
     blob.write_text(_blob_source(code_object))
     blob_o = BUILD / f"{tag}_blob.o"
-    host_o = BUILD / f"{tag}_er_hip.o"
     _run(["gcc", "-c", str(blob), "-o", str(blob_o)])
-    gguf_o = BUILD / f"{tag}_er_gguf.o"
-    for src, obj in ((CSRC / "er_hip.cpp", host_o), (CSRC / "er_gguf.cpp", gguf_o)):
+    objs = []
+    for src in (CSRC / name for name in HOST_SOURCES):
+        obj = BUILD / f"{tag}_{src.stem}.o"
+        objs.append(str(obj))
         _run(["g++", "-O2", "-fPIC", "-std=c++17", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__", *(defines or []),
               "-I", str(ROCM / "include"), "-I", str(ROOT / "include"), "-I", str(CSRC),
               "-c", str(src), "-o", str(obj)])
     tmp = out.with_suffix(".so.tmp")
-    _run(["g++", "-shared", "-o", str(tmp), str(host_o), str(gguf_o), str(blob_o), "-pthread",
+    _run(["g++", "-shared", "-o", str(tmp), *objs, str(blob_o), "-pthread",
           "-L", str(ROCM / "lib"), "-lamdhip64", f"-Wl,-rpath,{ROCM / 'lib'}",
           "-Wl,--version-script=" + str(CSRC / "er_hip.map")])
     os.replace(tmp, out)
@@ -116,19 +132,21 @@ SAN_FLAGS = ["-fsanitize=address,undefined", "-fno-sanitize-recover=undefined", 
 
 def build_sanitized(out_dir: Path) -> tuple[Path, Path]:
     """AddressSanitizer + UndefinedBehaviorSanitizer builds of the host code:
-    the C-ABI library (er_hip.cpp, er_gguf.cpp, with the gfx950 code object
-    embedded unchanged) and the CPU oracle.  For CPU runs of the host-side
+    the C-ABI library (er_hip.cpp, er_kv8.cpp, er_gguf.cpp, with the gfx950
+    code objects embedded unchanged) and the CPU oracle.  For CPU runs of the host-side
     tests (argument validation, GGUF parsing); the GPU kernels are never
     built with a sanitizer.  Returns (library, oracle library)."""
     out_dir.mkdir(parents=True, exist_ok=True)
     if not CODE_OBJECT.exists():
         build_code_object()
+    if not KV8_CODE_OBJECT.exists():
+        build_kv8_code_object()
     blob = out_dir / "er_blob.S"
     blob.write_text(_blob_source(CODE_OBJECT))
     blob_o = out_dir / "er_blob.o"
     _run(["gcc", "-c", str(blob), "-o", str(blob_o)])
     objs = []
-    for src in (CSRC / "er_hip.cpp", CSRC / "er_gguf.cpp"):
+    for src in (CSRC / name for name in HOST_SOURCES):
         obj = out_dir / (src.stem + ".o")
         _run(["g++", *SAN_FLAGS, "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", str(ROCM / "include"),
               "-I", str(ROOT / "include"), "-I", str(CSRC), "-c", str(src), "-o", str(obj)])

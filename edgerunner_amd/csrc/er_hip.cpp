@@ -17,6 +17,7 @@
 #endif
 #include "er_error.h"
 #include "er_gemv_cfg.h"
+#include "er_kv8_host.h"
 #include "er_scratch.h"
 
 #include <hip/hip_runtime_api.h>
@@ -274,6 +275,7 @@ struct er_hip_ctx {
     // array (er_scratch.hip), found once at creation; the allocation-free
     // entry points pass it to kernels in place of caller scratch buffers
     void *scratch = nullptr;
+    er_detail::Kv8Kernels kv8;  // the 8-bit cache's kernels (er_kv8.cpp)
     er_device_info info{};
 };
 
@@ -296,6 +298,19 @@ er_status bind_device(const er_hip_ctx *ctx) {
     }
     return ER_OK;
 }
+
+}  // namespace
+
+// what er_kv8.cpp needs of a context
+namespace er_detail {
+
+const Kv8Kernels &kv8_of(const er_hip_ctx *ctx) { return ctx->kv8; }
+int cu_count_of(const er_hip_ctx *ctx) { return ctx->cu_count; }
+er_status bind_device_of(const er_hip_ctx *ctx) { return bind_device(ctx); }
+
+}  // namespace er_detail
+
+namespace {
 
 er_status launch(const er_hip_ctx *ctx, KernelId k, dim3 grid, dim3 block, uint32_t lds,
                  er_stream stream, void **args) {
@@ -1889,6 +1904,12 @@ er_status er_hip_create(int device, er_hip_ctx **out_ctx) {
                     return fail(ER_ERR_FUNCTION_NOT_FOUND, "functionNotFound(%s): %s", name, hipGetErrorString(e));
                 }
             }
+    const er_status kv8 = er_detail::kv8_load(ctx->kv8);
+    if (kv8 != ER_OK) {
+        (void)hipModuleUnload(ctx->module);
+        delete ctx;
+        return kv8;
+    }
     set_tok_mode(ctx, std::getenv("ER_HIP_GEMV_TOK"));
     if (const char *gv = std::getenv("ER_HIP_GEMM_VARIANT")) ctx->gemm_variant = std::atoi(gv);
     if (const char *fv = std::getenv("ER_HIP_GEMV_FP32")) ctx->gemv_fp32 = std::atoi(fv);
@@ -1933,7 +1954,10 @@ er_status er_hip_create(int device, er_hip_ctx **out_ctx) {
 
 void er_hip_destroy(er_hip_ctx *ctx) {
     if (!ctx) return;
-    if (bind_device(ctx) == ER_OK && ctx->module) (void)hipModuleUnload(ctx->module);
+    if (bind_device(ctx) == ER_OK) {
+        if (ctx->module) (void)hipModuleUnload(ctx->module);
+        er_detail::kv8_unload(ctx->kv8);
+    }
     delete ctx;
 }
 

@@ -405,6 +405,118 @@ er_status er_hip_encode_projection(er_hip_ctx *ctx, er_stream stream,
                                    const er_tensor_storage *tensor, er_buffer input,
                                    er_buffer output, uint32_t tokens);
 
+/* ---- between the projections: head norms and rotation, an 8-bit paged
+ * key/value cache and attention over it ----
+ * No counterpart on the reference's quantised path; they stand between the
+ * q/k/v projections (fp32 q and k, fp32 or fp16 v) and the output projection
+ * (fp32 x for the GEMV, bf16 x for the prefill GEMM) of this header. */
+
+/* Rows of heads: element e of head h in row r is data[r * row_stride + h *
+ * head_dim + e] (row_stride in elements, >= heads * head_dim, so the heads may
+ * be columns of a wider projection output).  Element aligned. */
+typedef struct er_head_rows {
+    er_buffer data;
+    uint32_t heads;
+    uint32_t row_stride;
+} er_head_rows;
+
+/* Position rotation.  Pair i < rotary_dim / 2 of a head turns by the angle
+ * position * inv_freq[i], formed in 64 bits: (a, b) -> (a cos - b sin, b cos +
+ * a sin).  The pair is elements (i, i + rotary_dim / 2), or (2i, 2i + 1) where
+ * interleaved is not 0; elements from rotary_dim on pass.  rotary_dim: a
+ * multiple of 8 up to head_dim; 0: no rotation, inv_freq unused. */
+typedef struct er_rope {
+    er_buffer inv_freq; /* fp32 [rotary_dim / 2] */
+    uint32_t rotary_dim;
+    uint32_t interleaved;
+} er_rope;
+
+/* RMS norm of each query and key head and the rotation, in one pass:
+ * n = x / sqrt(mean(x^2) + eps) * norm, then the rotation to positions[row].
+ * q_norm / k_norm (fp32 [head_dim]): a null data pointer leaves the norm out.
+ * k and k_out NULL: queries alone.  An output may be its own input (same
+ * data, heads and stride); otherwise they do not overlap.  head_dim 64, 128
+ * or 256 and rotary_dim as above, else INVALID_VECTOR_SHAPE; a buffer shorter
+ * than its rows -> ENCODING_FAILED; rows 0 does nothing. */
+er_status er_hip_qk_norm_rope(er_hip_ctx *ctx, er_stream stream, const er_head_rows *q, const er_head_rows *k,
+                              const er_head_rows *q_out, const er_head_rows *k_out, er_buffer positions,
+                              er_buffer q_norm, er_buffer k_norm, const er_rope *rope, uint32_t rows,
+                              uint32_t head_dim, float eps);
+
+/* Paged key/value cache of one layer in 8 bits: e4m3 codes (1 sign, 4
+ * exponent, 3 mantissa bits, largest 448, no infinities) with one scale for
+ * each page and key/value head, in keys and in values apart.  A code c stands
+ * for c * scale.  Scales are powers of two, so a block's codes stay exact when
+ * a later token raises its scale (but for e4m3 subnormals). */
+typedef struct er_kv8_cache {
+    er_buffer k;        /* uint8 [pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
+    er_buffer v;        /* the same */
+    er_buffer k_scale;  /* fp32 [pages][kv_heads] */
+    er_buffer v_scale;  /* the same */
+    uint32_t pages;
+    uint32_t kv_heads;
+    uint32_t page_tokens; /* 16, 32 or 64 */
+    uint32_t head_dim;    /* 64, 128 or 256 */
+} er_kv8_cache;
+
+/* The sequences of a call, read on the device (a recorded graph follows later
+ * contents).  Rows row_start[s] .. row_start[s + 1] - 1 of the row buffers are
+ * sequence s's newest tokens: of the kv_len[s] tokens that it has in the cache
+ * once they are appended, they are the last, and the i-th of n rows has the
+ * position kv_len[s] - n + i.  Token t lies in page page_table[s][t /
+ * page_tokens].  Rows from row_start[sequences] on belong to no sequence and
+ * are left as they are; a sequence may have no rows, no tokens, or both.
+ * max_rows and max_kv_len bound what any sequence has: more is not looked at
+ * (rows beyond the first max_rows, tokens beyond the first max_kv_len or
+ * beyond the table).  Rows whose position would be negative are not appended
+ * and attend to nothing.  Entries of page_table outside [0, pages) hold no
+ * tokens: nothing is read or written there.  A page that gets tokens in a call
+ * belongs to one sequence; full pages may be shared by many. */
+typedef struct er_kv8_batch {
+    er_buffer page_table; /* int32 [sequences][table_stride] */
+    er_buffer kv_len;     /* int32 [sequences] */
+    er_buffer row_start;  /* int32 [sequences + 1], ascending */
+    uint32_t sequences;
+    uint32_t table_stride;
+    uint32_t rows;       /* rows that the row buffers hold */
+    uint32_t max_rows;   /* 1 .. rows */
+    uint32_t max_kv_len;
+} er_kv8_batch;
+
+/* Appends the rows' keys and values to the cache.  Keys are normed (k_norm;
+ * null data: not) and rotated to their positions on the way, as
+ * er_hip_qk_norm_rope does; values are stored as they are.  Queries may ride
+ * along (q and q_out not NULL): normed with q_norm, rotated and written to
+ * q_out, which may be q itself.  k fp32; v of v_type ER_TYPE_F32 or
+ * ER_TYPE_F16, both with the cache's heads.
+ * A block's scale is 2^j with the smallest j >= -100 that brings its largest
+ * finite magnitude to 448 or less, over all tokens the block has had since its
+ * first; codes round to nearest even.  NaN and infinities become the NaN code
+ * 0xff and do not enter the scale.  Slots behind the last token keep their bytes.
+ * Sizes -> INVALID_VECTOR_SHAPE, a cache buffer too short ->
+ * INVALID_MATRIX_SHAPE, other buffers too short -> ENCODING_FAILED. */
+er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache, const er_kv8_batch *batch,
+                            const er_head_rows *k, const er_head_rows *v, uint32_t v_type, const er_head_rows *q,
+                            const er_head_rows *q_out, er_buffer k_norm, er_buffer q_norm, const er_rope *rope,
+                            float eps);
+
+/* Causal attention of the batch's rows over the cache: the row at position p
+ * of query head h gets sum_t w_t v_t over the tokens t <= p (and t > p -
+ * window where window is not 0) of its sequence and key/value head h /
+ * (q->heads / kv_heads), w = softmax(scale * q . k_t).  q fp32; out of
+ * out_type ER_TYPE_F32 (products of fp32 accuracy) or ER_TYPE_BF16 (queries
+ * and weights rounded to fp16 for the products).  A row that no token is
+ * visible to gets zeros.  out does not overlap q.
+ * workspace: scratch of er_hip_kv8_attention_workspace bytes (which depend on
+ * the batch's and cache's sizes and q_heads alone), 16-byte aligned; calls and
+ * recorded graphs that may overlap in time need one each.  q->heads is a multiple of
+ * kv_heads, at most 1024 a key/value head.  Errors as er_hip_kv8_append's. */
+er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
+                               const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
+                               uint32_t out_type, float scale, uint32_t window, er_buffer workspace);
+er_status er_hip_kv8_attention_workspace(er_hip_ctx *ctx, const er_kv8_cache *cache, const er_kv8_batch *batch,
+                                         uint32_t q_heads, uint64_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif
