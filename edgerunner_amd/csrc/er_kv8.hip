@@ -19,6 +19,13 @@ ER_DEV float uniform(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
+// A value that no kernel of the launch writes, at an address that all lanes
+// share: a scalar load, which waits for no vector load in flight.
+template <typename T>
+ER_DEV T load_shared(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)(uintptr_t)p;
+}
+
 // ---------------------------------------------------------------- rows of a batch
 
 // Sequence s as the kernels see it: whatever the device arrays hold, rows stay
@@ -29,15 +36,15 @@ struct Sequence {
 ER_DEV Sequence sequence_of(const ErKv8Batch &b, uint32_t s) {
     const int rows = (int)b.rows;
     Sequence q;
-    q.row0 = min(max(b.start[s], 0), rows);
-    q.n = min(max(min(b.start[s + 1], rows) - q.row0, 0), (int)b.maxRows);
-    q.len = min(max(b.len[s], 0), (int)b.maxLen);
+    q.row0 = min(max(load_shared(b.start + s), 0), rows);
+    q.n = min(max(min(load_shared(b.start + s + 1), rows) - q.row0, 0), (int)b.maxRows);
+    q.len = min(max(load_shared(b.len + s), 0), (int)b.maxLen);
     return q;
 }
 
 // The page that token t (0 <= t < len) of sequence s lies in, or -1.
 ER_DEV int page_of(const ErKv8Batch &b, const ErKv8Cache &c, uint32_t s, int t) {
-    const int p = b.table[(size_t)s * b.stride + ((uint32_t)t >> c.shift)];
+    const int p = load_shared(b.table + (size_t)s * b.stride + ((uint32_t)t >> c.shift));
     return (uint32_t)p < c.pages ? p : -1;
 }
 

@@ -19,7 +19,7 @@
 // by more than 8 (in powers of two); weights are 2^(s - m + 7), so at most
 // 2^15, and the reference cancels in the quotient.  Most tiles rescale nothing.
 
-#define ER_NO_MAX (-1.0e30f)  // reference of a column that has seen no score
+#define ER_NO_MAX (-3.0e38f)  // reference of a column that has seen no score
 
 ER_DEV f32x4 mfma16(h8 a, h8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 ER_DEV f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -49,25 +49,10 @@ ER_DEV void transpose_codes(const uint32_t x[8], float f0, float f1, h8 out[4]) 
     out[3] = join(codes_to_h2<true>(a1, f0), codes_to_h2<true>(b1, f0), codes_to_h2<true>(c1, f1), codes_to_h2<true>(d1, f1));
 }
 
-// The NaN codes of an operand: is there one, ones in their places, zeros in their places.
-ER_DEV bool is_nan_h(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7fffu) > 0x7c00u; }
-ER_DEV bool any_nan(h8 x) {
-    bool n = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n |= is_nan_h(x[i]);
-    return n;
-}
-ER_DEV h8 nan_places(h8 x) {
-    h8 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = is_nan_h(x[i]) ? (_Float16)1.0f : (_Float16)0.0f;
-    return r;
-}
-ER_DEV h8 without_nan(h8 x) {
-    h8 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = is_nan_h(x[i]) ? (_Float16)0.0f : x[i];
-    return r;
+// A byte of ones for each NaN code of a dword.
+ER_DEV uint32_t nan_codes(uint32_t c) {
+    const uint32_t top = ((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x7f alone carries into bit 7
+    return (top << 1) - (top >> 7);
 }
 
 // A column of a tile: its row, its query head, and the tokens [lo, hi) that it sees.
@@ -86,13 +71,17 @@ ER_DEV Column column_of(const ErAttendArgs &p, const Sequence &q, uint32_t kvHea
     return c;
 }
 
-// A column's query as B operands: eight consecutive values from `from` on for
-// each of N products, `step` values apart, as one or two fp16 terms.  The
-// query is brought to below 1 by a power of two over the whole head (`join`
-// takes the largest magnitude over the lanes that share the column); returns
-// that power.
+// A column's query times the softmax's scale (and log2 e) as B operands: eight
+// consecutive values from `from` on for each of N products, `step` values
+// apart, as one or two fp16 terms.  It is brought to below 1 by a power of two
+// over the whole head (`join_lanes` takes the largest magnitude over the lanes
+// that share the column); returns that power.  With the keys' scales powers of
+// two as well, a score is its product times a power of two, exactly: the fused
+// multiply-add that takes the reference off it and the product that the
+// reference was taken from agree to the last bit, however large the scores.
 template <int N, int TERMS, typename JOIN>
-ER_DEV float load_query(const float *src, bool live, uint32_t from, uint32_t step, h8 (&b)[TERMS][N], JOIN join_lanes) {
+ER_DEV float load_query(const float *src, bool live, float scale, uint32_t from, uint32_t step, h8 (&b)[TERMS][N],
+                        JOIN join_lanes) {
     float x[N][8];
     float peak = 0.0f;
 #pragma unroll
@@ -104,8 +93,8 @@ ER_DEV float load_query(const float *src, bool live, uint32_t from, uint32_t ste
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[k][i] = lo[i];
-            x[k][4 + i] = hi[i];
+            x[k][i] = lo[i] * scale;
+            x[k][4 + i] = hi[i] * scale;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) peak = fmaxf(peak, finite_magnitude(x[k][i]));
@@ -126,6 +115,10 @@ ER_DEV float load_query(const float *src, bool live, uint32_t from, uint32_t ste
     return exp2i(e);
 }
 
+// The factor of a 16-token part's scores.  Not 0, so that -inf stays the score
+// of a hidden token.
+ER_DEV float score_factor(float qf, float ks) { return fmaxf(qf * ks, 1.2e-38f); }
+
 // Weights of eight tokens as one or two fp16 terms.
 template <int TERMS>
 ER_DEV void weight_terms(const float w[8], h8 (&b)[TERMS]) {
@@ -137,15 +130,11 @@ ER_DEV void weight_terms(const float w[8], h8 (&b)[TERMS]) {
     }
 }
 
-ER_DEV uint16_t to_bf16(float v) {  // nearest even; a NaN stays one
-    const uint32_t u = __float_as_uint(v);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+typedef __bf16 b16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 ER_DEV void store4(const ErAttendArgs &p, int row, uint32_t head, uint32_t d, uint32_t D, f32x4 v) {
     const size_t at = (size_t)row * p.outStride + (size_t)head * D + d;
     if (p.half)
-        *(u16x4_a2 *)((uint16_t *)p.out + at) = u16x4_a2{to_bf16(v.x), to_bf16(v.y), to_bf16(v.z), to_bf16(v.w)};
+        *(b16x4_a2 *)((uint16_t *)p.out + at) = b16x4_a2{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
     else
         *(f32x4_a4 *)((float *)p.out + at) = v;
 }
@@ -166,25 +155,36 @@ struct NarrowTile {
     u32x4 k[2][D / 64];      // lane (n, g): token n of each half, bytes [g D/4, (g + 1) D/4)
     uint32_t v[D / 64][8];   // lane (n, g): tokens 4 g + i of the first half, then of the second, bytes [n D/16, (n + 1) D/16)
     float ks[2], vs[2];      // the halves' scales
-    bool ok[2];              // the half's page exists and holds a visible token
+    int page[2];             // the halves' pages; -1: outside the pool, or no visible token
 };
 
-template <int D>
-ER_DEV void load_narrow(NarrowTile<D> &t, const ErAttendArgs &p, uint32_t s, uint32_t h, int T, int lo, int hi,
-                        uint32_t n, uint32_t g) {
+// The pages of a tile's halves, found a tile ahead of its loads.
+struct NarrowPages {
+    int page[2];
+};
+ER_DEV NarrowPages narrow_pages(const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
+    NarrowPages w;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int at = T + 16 * half;
-        int page = -1;
-        if (at < hi && at + 16 > lo) page = uniform(page_of(p.b, p.c, s, at));
-        t.ok[half] = page >= 0;
-        const size_t block = (size_t)(uint32_t)max(page, 0) * p.c.heads + h;
-        t.ks[half] = p.c.ks[block];
-        t.vs[half] = p.c.vs[block];
-        const uint32_t inside = (uint32_t)at & ((1u << p.c.shift) - 1u);
+        w.page[half] = at < hi && at + 16 > lo ? uniform(page_of(p.b, p.c, s, at)) : -1;
+    }
+    return w;
+}
+
+template <int D>
+ER_DEV void load_narrow(NarrowTile<D> &t, const NarrowPages &w, const ErAttendArgs &p, uint32_t h, int T, uint32_t n,
+                        uint32_t g) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        t.page[half] = w.page[half];
+        const size_t block = (size_t)(uint32_t)max(w.page[half], 0) * p.c.heads + h;
+        t.ks[half] = load_shared(p.c.ks + block);
+        t.vs[half] = load_shared(p.c.vs + block);
+        const uint32_t inside = (uint32_t)(T + 16 * half) & ((1u << p.c.shift) - 1u);
         const size_t base = ((block << p.c.shift) + inside) * D;
-        const uint8_t *kp = p.c.k + base + n * D + g * (D / 4);
-        const uint8_t *vp = p.c.v + base + 4 * g * D + n * (D / 16);
+        const uint8_t *kp = p.c.k + base + (n * D + g * (D / 4));
+        const uint8_t *vp = p.c.v + base + (4 * g * D + n * (D / 16));
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) t.k[half][j] = *(const u32x4 *)(kp + 16 * j);
 #pragma unroll
@@ -192,15 +192,15 @@ ER_DEV void load_narrow(NarrowTile<D> &t, const ErAttendArgs &p, uint32_t s, uin
             if constexpr (D == 64) {
                 t.v[0][4 * half + i] = *(const uint32_t *)(vp + i * D);
             } else if constexpr (D == 128) {
-                const u32x2 w = *(const u32x2 *)(vp + i * D);
-                t.v[0][4 * half + i] = w.x;
-                t.v[1][4 * half + i] = w.y;
+                const u32x2 x = *(const u32x2 *)(vp + i * D);
+                t.v[0][4 * half + i] = x.x;
+                t.v[1][4 * half + i] = x.y;
             } else {
-                const u32x4 w = *(const u32x4 *)(vp + i * D);
-                t.v[0][4 * half + i] = w.x;
-                t.v[1][4 * half + i] = w.y;
-                t.v[2][4 * half + i] = w.z;
-                t.v[3][4 * half + i] = w.w;
+                const u32x4 x = *(const u32x4 *)(vp + i * D);
+                t.v[0][4 * half + i] = x.x;
+                t.v[1][4 * half + i] = x.y;
+                t.v[2][4 * half + i] = x.z;
+                t.v[3][4 * half + i] = x.w;
             }
         }
     }
@@ -225,8 +225,9 @@ template <int D>
 struct NarrowState {
     f32x4 o[D / 16];  // o[j][i]: value (4 g + i) D/16 + j of column n
     float m, l;       // reference; this lane's part of the sum of weights
-    float vref;       // the largest value scale so far: o is in units of vref / 128 (wave-uniform)
+    float vref, vinv; // the largest value scale so far: o is in units of vref / 128; 128 / vref (wave-uniform)
     bool seen;        // a token was visible to the column
+    bool nans;        // a masked tile held NaN codes
 };
 
 // Tokens that some column sees, and tokens that every column sees.
@@ -238,104 +239,107 @@ ER_DEV Spans spans_of(const ErAttendArgs &p, const Sequence &q, uint32_t firstCo
     return Spans{a.lo, b.hi, b.lo, a.hi};
 }
 
-// One product of the values with the weights, where a tile that the columns
-// see in part holds NaN codes: a token hidden from a column must leave it
-// alone, and 0 * NaN would not.  The NaN codes count as zeros, and a second
-// product counts the visible ones.
-template <int TERMS>
-ER_DEV void add_values(f32x4 &o, h8 a, const h8 (&b)[TERMS], h8 visible, bool nans) {
-    if (!nans) {
+// Moves a column's reference up to its scores' largest.
+template <int N, typename ACC>
+ER_DEV void raise_reference(float to, float &m, float &l, ACC (&o)[N]) {
+    const float f = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= f;
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) o = mfma16(a, b[term], o);
-        return;
-    }
-    const f32x4 hits = mfma16(nan_places(a), visible, f32x4{});
-    a = without_nan(a);
+    for (int j = 0; j < N; ++j) o[j] *= f;
+}
+// Moves the value scales' reference up to a tile's largest.
+template <int N, typename ACC>
+ER_DEV void raise_scale(float to, float &vref, float &vinv, ACC (&o)[N]) {
+    const float f = vref / to;
+    vref = to;
+    vinv = 128.0f / to;
 #pragma unroll
-    for (int term = 0; term < TERMS; ++term) o = mfma16(a, b[term], o);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = hits[i] > 0.0f ? __builtin_nanf("") : o[i];
+    for (int j = 0; j < N; ++j) o[j] *= f;
 }
 
+// One tile into the state.  Where some column does not see all of it, or a
+// page is missing, hidden tokens get the score -inf, and those that no column
+// sees have their bytes taken as zeros, whatever they hold.  NaN codes count
+// as zeros too there, since a column may not see them and 0 * NaN is NaN:
+// st.nans remembers that there were some, and mark_nans brings them back.
 template <int D, int TERMS>
-ER_DEV void attend_narrow(NarrowState<D> &st, const NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
+ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
                           int lo, int hi, const Spans &w, uint32_t g) {
-    if (!t.ok[0] && !t.ok[1]) return;
-    float x[8];
+    const bool ok0 = t.page[0] >= 0, ok1 = t.page[1] >= 0;
+    const bool whole = ok0 && ok1 && T >= w.allLo && T + 32 <= w.allHi;
+    f32x4 s[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        f32x4 s = {};
+        s[half] = f32x4{};
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
             const u32x4 c = t.k[half][k / 2];
             const h8 a = k % 2 ? codes_to_h8(c.z, c.w) : codes_to_h8(c.x, c.y);
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) s = mfma16(a, qb[term][k], s);
+            for (int term = 0; term < TERMS; ++term) s[half] = mfma16(a, qb[term][k], s[half]);
         }
-        const float f = qf * t.ks[half];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * half + i] = s[i] * f;
     }
-    const bool whole = t.ok[0] && t.ok[1] && T >= w.allLo && T + 32 <= w.allHi;
-    uint32_t shown = 0xff;
-    if (!whole) {
+    if (whole) {
+        st.seen = true;
+    } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + 16 * (i / 4) + 4 * (int)g + (i & 3);
-            if (!(t.ok[i / 4] && tok >= lo && tok < hi)) {
-                x[i] = -__builtin_inff();
-                shown &= ~(1u << i);
+            const bool ok = i < 4 ? ok0 : ok1, shown = ok && tok >= lo && tok < hi;
+            st.seen |= shown;
+            s[i / 4][i & 3] = shown ? s[i / 4][i & 3] : -__builtin_inff();
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d) {
+                const uint32_t c = ok && tok >= w.anyLo && tok < w.anyHi ? t.v[d][i] : 0u, nan = nan_codes(c);
+                st.nans |= nan != 0;
+                t.v[d][i] = c & ~nan;
             }
         }
     }
-    st.seen |= shown != 0;
-    const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(top > st.m + 8.0f)) {
-        const float m = fmaxf(st.m, column_max4(top));
-        const float f = __builtin_amdgcn_exp2f(st.m - m);
-        st.m = m;
-        st.l *= f;
+    const float f0 = score_factor(qf, ok0 ? t.ks[0] : t.ks[1]), f1 = score_factor(qf, ok1 ? t.ks[1] : t.ks[0]);
+    const float top = fmaxf(fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[0].z, s[0].w)) * f0,
+                            fmaxf(fmaxf(s[1].x, s[1].y), fmaxf(s[1].z, s[1].w)) * f1);
+    if (__any(top > st.m + 8.0f)) raise_reference(fmaxf(st.m, column_max4(top)), st.m, st.l, st.o);
+    const float vs0 = ok0 ? t.vs[0] : t.vs[1], vs1 = ok1 ? t.vs[1] : t.vs[0];
+    if (fmaxf(vs0, vs1) > st.vref) raise_scale(fmaxf(vs0, vs1), st.vref, st.vinv, st.o);
+    const float v0 = vs0 * st.vinv, v1 = vs1 * st.vinv, m7 = st.m - 7.0f;
+    float x[8];
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) st.o[j] *= f;
-    }
-    const float vs0 = t.ok[0] ? t.vs[0] : t.vs[1], vs1 = t.ok[1] ? t.vs[1] : t.vs[0];
-    const float vtop = fmaxf(vs0, vs1);
-    if (vtop > st.vref) {
-        const float f = st.vref / vtop;
-        st.vref = vtop;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) st.o[j] *= f;
-    }
-    const float f0 = 128.0f * (vs0 / st.vref), f1 = 128.0f * (vs1 / st.vref);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - (st.m - 7.0f));
-        st.l += x[i];
-    }
-    h8 b[TERMS], visible;
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(s[i / 4][i & 3] * (i < 4 ? f0 : f1) - m7);
+    st.l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    h8 b[TERMS];
     weight_terms<TERMS>(x, b);
-    // whole tiles, and those whose hidden tokens are hidden from all columns, need no care with NaN codes
-    const bool mixed = !whole && (w.anyLo < w.allLo || w.anyHi > w.allHi);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) visible[i] = (shown >> i) & 1u ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
     for (int d = 0; d < D / 64; ++d) {
-        uint32_t c[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = t.v[d][i];
-        if (!whole) {
-            // tokens that no column sees, or without a page, count as zeros whatever their bytes hold
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int tok = T + 16 * (i / 4) + 4 * (int)g + (i & 3);
-                c[i] = t.ok[i / 4] && tok >= w.anyLo && tok < w.anyHi ? c[i] : 0u;
-            }
-        }
         h8 a[4];
-        transpose_codes(c, f0, f1, a);
-        const bool nans = mixed && __any(any_nan(a[0]) || any_nan(a[1]) || any_nan(a[2]) || any_nan(a[3]));
+        transpose_codes(t.v[d], v0, v1, a);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) add_values<TERMS>(st.o[4 * d + j], a[j], b, visible, nans);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) st.o[4 * d + j] = mfma16(a[j], b[term], st.o[4 * d + j]);
+    }
+}
+
+// The sums that a visible NaN code of the masked tiles belongs to become NaN.
+// Reached only where such a tile held one, so it takes the tokens one by one.
+template <int D>
+ER_DEV void mark_nans(NarrowState<D> &st, const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
+                      int hi, uint32_t g) {
+    for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
+        const int page = page_of(p.b, p.c, s, tok);
+        if (page < 0) continue;
+        const size_t slot = (((size_t)page * p.c.heads + h) << p.c.shift) + ((uint32_t)tok & ((1u << p.c.shift) - 1u));
+        const uint8_t *v = p.c.v + slot * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d) {
+                const uint32_t nan = nan_codes(*(const uint32_t *)(v + (4 * g + i) * (D / 16) + 4 * d));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    st.o[4 * d + j][i] = (nan >> (8 * j)) & 1u ? __builtin_nanf("") : st.o[4 * d + j][i];
+            }
     }
 }
 
@@ -359,21 +363,29 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
 
     NarrowTile<D> t0, t1;
     int T = begin + 32 * (int)wave;
-    if (T < end) load_narrow<D>(t0, p, s, h, T, w.anyLo, end, n, g);
+    NarrowPages pages = narrow_pages(p, s, T, w.anyLo, end);
+    if (T < end) load_narrow<D>(t0, pages, p, h, T, n, g);
+    pages = narrow_pages(p, s, T + 128, w.anyLo, end);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
-                                               g * (D / 4), 8, qb, column_max4) * p.scale;
+                                               p.scale, g * (D / 4), 8, qb, column_max4);
     NarrowState<D> st = {};
     st.m = ER_NO_MAX;
+    auto step = [&](NarrowTile<D> &now, NarrowTile<D> &next) {
+        if (T + 128 < end) {
+            load_narrow<D>(next, pages, p, h, T + 128, n, g);
+            pages = narrow_pages(p, s, T + 256, w.anyLo, end);
+        }
+        if (now.page[0] >= 0 || now.page[1] >= 0) attend_narrow<D, TERMS>(st, now, qb, qf, T, c.lo, c.hi, w, g);
+        T += 128;
+    };
     while (T < end) {
-        if (T + 128 < end) load_narrow<D>(t1, p, s, h, T + 128, w.anyLo, end, n, g);
-        attend_narrow<D, TERMS>(st, t0, qb, qf, T, c.lo, c.hi, w, g);
-        T += 128;
+        step(t0, t1);
         if (T >= end) break;
-        if (T + 128 < end) load_narrow<D>(t0, p, s, h, T + 128, w.anyLo, end, n, g);
-        attend_narrow<D, TERMS>(st, t1, qb, qf, T, c.lo, c.hi, w, g);
-        T += 128;
+        step(t1, t0);
     }
+    // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
+    if (__any(st.nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, g);
 
     // the waves' columns, [wave][column][D + 4], and their references and sums (-1: nothing seen)
     constexpr uint32_t PITCH = D + 4;
@@ -452,8 +464,8 @@ ER_DEV void wide_scales(WideParts &w, const ErAttendArgs &p, uint32_t h) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const size_t block = (size_t)(uint32_t)max(w.page[i], 0) * p.c.heads + h;
-        w.ks[i] = p.c.ks[block];
-        w.vs[i] = p.c.vs[block];
+        w.ks[i] = load_shared(p.c.ks + block);
+        w.vs[i] = load_shared(p.c.vs + block);
     }
 }
 // v[i] for an index that differs between lanes, without an address (which would put v into scratch memory)
@@ -501,16 +513,18 @@ ER_DEV void load_wide(WideTile<D> &t, const WideParts &w, const ErAttendArgs &p,
     }
 }
 
-// LDS: keys [64][D + 8], values transposed [D][64 + 8], both fp16; a flag a
-// wave for NaN codes.  The pitches put consecutive rows 4 banks apart.
+// LDS: keys [64][D + 8], values transposed [D][64 + 8], both fp16.  The
+// pitches put consecutive rows 4 banks apart.
 template <int D>
 struct WideLds {
     _Float16 k[ER_WIDE_TOKENS][D + 8];
     _Float16 v[D][ER_WIDE_TOKENS + 8];
 };
 
-template <int D>
-ER_DEV bool store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w, float vref, int T, int lo, int hi,
+// A tile into LDS.  MIXED (some column of the workgroup does not see all of
+// it): as attend_narrow's masked tiles; true where there were NaN codes.
+template <int D, bool MIXED>
+ER_DEV bool store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w, float vinv, int T, int lo, int hi,
                        uint32_t tid) {
     {
         _Float16 *dst = &to.k[tid >> 2][(tid & 3u) * (D / 4)];
@@ -524,17 +538,21 @@ ER_DEV bool store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w,
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));
-        const bool ok = pick4(w.page, it.part) >= 0;
+        const bool ok = !MIXED || pick4(w.page, it.part) >= 0;
         uint32_t c[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            // tokens that no column sees, or without a page, count as zeros whatever their bytes hold
-            const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
-            c[i] = ok && tok >= lo && tok < hi ? t.v[r][i] : 0u;
-            nan |= (((c[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+            c[i] = t.v[r][i];
+            if constexpr (MIXED) {
+                const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
+                c[i] = ok && tok >= lo && tok < hi ? c[i] : 0u;
+                const uint32_t nans = nan_codes(c[i]);
+                nan |= nans != 0;
+                c[i] &= ~nans;
+            }
         }
         h8 a[4];
-        const float f = ok ? 128.0f * (pick4(w.vs, it.part) / vref) : 1.0f;
+        const float f = ok ? pick4(w.vs, it.part) * vinv : 1.0f;
         transpose_codes(c, f, f, a);
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(h8 *)&to.v[4 * it.dword + j][8 * it.slot] = a[j];
@@ -551,19 +569,87 @@ ER_DEV float column_sum2(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-template <int TERMS>
-ER_DEV void add_values32(f32x16 &o, h8 a, const h8 (&b)[TERMS], h8 visible, bool nans) {
-    if (!nans) {
+// Running state of a wave's 32 columns, as NarrowState's.
+template <int D>
+struct WideState {
+    f32x16 o[D / 32];  // o[d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n
+    float m, l;
+    bool seen;
+};
+
+// One tile into the state, as attend_narrow; `whole`: this wave's columns see all of it.
+template <int D, int TERMS>
+ER_DEV void attend_wide(WideState<D> &st, const WideLds<D> &in, const WideParts &parts, const h8 (&qb)[TERMS][D / 16],
+                        float qf, bool whole, int T, int lo, int hi, uint32_t n, uint32_t hh) {
+    f32x16 s[2];
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) o = mfma32(a, b[term], o);
-        return;
+    for (int th = 0; th < 2; ++th) {
+        s[th] = f32x16{};
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) s[th] = mfma32(a, qb[term][k], s[th]);
+        }
     }
-    const f32x16 hits = mfma32(nan_places(a), visible, f32x16{});
-    a = without_nan(a);
+    if (whole) {
+        st.seen = true;
+    } else {
 #pragma unroll
-    for (int term = 0; term < TERMS; ++term) o = mfma32(a, b[term], o);
+        for (int i = 0; i < 32; ++i) {
+            const int tok = T + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * (int)hh + (i & 3);
+            const bool shown = parts.page[i >> 3] >= 0 && tok >= lo && tok < hi;
+            st.seen |= shown;
+            s[i >> 4][i & 15] = shown ? s[i >> 4][i & 15] : -__builtin_inff();
+        }
+    }
+    float f[4], top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = hits[i] > 0.0f ? __builtin_nanf("") : o[i];
+    for (int i = 0; i < 4; ++i) {
+        f[i] = score_factor(qf, parts.page[i] >= 0 ? parts.ks[i] : 1.0f);
+        float most = s[i >> 1][8 * (i & 1)];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) most = fmaxf(most, s[i >> 1][8 * (i & 1) + j]);
+        top = fmaxf(top, most * f[i]);
+    }
+    if (__any(top > st.m + 8.0f)) raise_reference(fmaxf(st.m, column_max2(top)), st.m, st.l, st.o);
+    const float m7 = st.m - 7.0f;
+#pragma unroll
+    for (int sl = 0; sl < 4; ++sl) {
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(s[sl >> 1][8 * (sl & 1) + i] * f[sl] - m7);
+        st.l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        h8 b[TERMS];
+        weight_terms<TERMS>(e, b);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+            const h8 a = *(const h8 *)&in.v[32 * d + n][16 * sl + 8 * hh];
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) st.o[d] = mfma32(a, b[term], st.o[d]);
+        }
+    }
+}
+
+// As the narrow kernel's.
+template <int D>
+ER_DEV void mark_nans(WideState<D> &st, const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
+                      int hi, uint32_t hh) {
+    for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
+        const int page = page_of(p.b, p.c, s, tok);
+        if (page < 0) continue;
+        const size_t slot = (((size_t)page * p.c.heads + h) << p.c.shift) + ((uint32_t)tok & ((1u << p.c.shift) - 1u));
+        const uint8_t *v = p.c.v + slot * D;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t nan = nan_codes(*(const uint32_t *)(v + 32 * d + 8 * i + 4 * hh));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    st.o[d][4 * i + j] = (nan >> (8 * j)) & 1u ? __builtin_nanf("") : st.o[d][4 * i + j];
+            }
+    }
 }
 
 // 128 columns against one piece of their sequence's tokens, 32 columns a wave:
@@ -572,7 +658,7 @@ ER_DEV void add_values32(f32x16 &o, h8 a, const h8 (&b)[TERMS], h8 visible, bool
 // worked on; a lane half's tokens of a slice lie together there, so that one
 // 16-byte read is an operand.
 template <int D, int TERMS>
-ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds, uint32_t (*nanFlags)[4]) {
+ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // units (sequence, head, piece) are dealt over a multiple of 8 workgroups,
     // and workgroups to the 8 XCDs in turn, so that one XCD's L2 serves all
     // row tiles of a unit; later row tiles see more tokens and start first
@@ -592,9 +678,9 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds, uint32_t (*n
     const bool live = wcol0 + n < cols;
     const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
 
-    f32x16 o[D / 32] = {};
-    float m = ER_NO_MAX, l = 0.0f, vref = 0.0f;
-    bool seen = false;
+    WideState<D> st = {};
+    st.m = ER_NO_MAX;
+    float vref = 0.0f, vinv = 0.0f;
     if (begin < end) {
         WideTile<D> t;
         WideParts now, next;
@@ -603,25 +689,37 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds, uint32_t (*n
         load_wide<D>(t, now, p, h, begin, tid);
         wide_scales(now, p, h);
         h8 qb[TERMS][D / 16];
-        const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live, hh * 8, 16,
-                                                   qb, column_max2) * p.scale;
-        float shrink = 0.0f;
-        auto raise = [&](const WideParts &parts) {  // the value scales' reference, and what it does to o
+        const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live,
+                                                   p.scale, hh * 8, 16, qb, column_max2);
+        // the sums are in units of the reference that their tiles were converted
+        // with, one tile behind the conversion's
+        float unit = 0.0f;
+        bool nans = false;
+        auto convert = [&](WideLds<D> &to, int T) {
             float top = vref;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = parts.page[i] >= 0 ? fmaxf(top, parts.vs[i]) : top;
-            shrink = top > vref ? vref / top : 1.0f;
-            vref = top;
+            for (int i = 0; i < 4; ++i) top = now.page[i] >= 0 ? fmaxf(top, now.vs[i]) : top;
+            if (top > vref) {
+                vref = top;
+                vinv = 128.0f / top;
+            }
+            const bool all = now.page[0] >= 0 && now.page[1] >= 0 && now.page[2] >= 0 && now.page[3] >= 0;
+            if (all && T >= w.allLo && T + 64 <= w.allHi)
+                store_wide<D, false>(to, t, now, vinv, T, w.anyLo, end, tid);
+            else
+                nans |= store_wide<D, true>(to, t, now, vinv, T, w.anyLo, end, tid);
         };
-        raise(now);
-        bool nan = store_wide<D>(lds[0], t, now, vref, begin, w.anyLo, end, tid);
-        nan = __any(nan);
-        if (lane == 0) nanFlags[0][wave] = nan;
+        convert(lds[0], begin);
         uint32_t buf = 0;
         for (int T = begin; T < end; T += 64, buf ^= 1u) {
             __syncthreads();
             const WideParts parts = now;
-            const float rescale = shrink;
+            if (vref > unit) {
+                const float f = unit / vref;
+                unit = vref;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) st.o[d] *= f;
+            }
             const bool more = T + 64 < end;
             if (more) {
                 now = next;
@@ -629,100 +727,33 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds, uint32_t (*n
                 wide_scales(now, p, h);
                 wide_pages(next, p, s, T + 128, w.anyLo, end);
             }
-            bool none = true;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) none &= parts.page[i] < 0;
-            if (rescale != 1.0f) {
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) o[d] *= rescale;
-            }
-            if (!idle && !none && T < ww.anyHi && T + 64 > ww.anyLo) {
-                const WideLds<D> &in = lds[buf];
-                float x[2][16];
-#pragma unroll
-                for (int th = 0; th < 2; ++th) {
-                    f32x16 sc = {};
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
-#pragma unroll
-                        for (int term = 0; term < TERMS; ++term) sc = mfma32(a, qb[term][k], sc);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[th][i] = sc[i] * (qf * parts.ks[2 * th + (i >> 3)]);
-                }
-                bool whole = T >= ww.allLo && T + 64 <= ww.allHi;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) whole &= parts.page[i] >= 0;
-                uint32_t shown = ~0u;
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int tok = T + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * (int)hh + (i & 3);
-                        if (!(parts.page[i >> 3] >= 0 && tok >= c.lo && tok < c.hi)) {
-                            x[i >> 4][i & 15] = -__builtin_inff();
-                            shown &= ~(1u << i);
-                        }
-                    }
-                }
-                seen |= shown != 0;
-                float top = x[0][0];
-#pragma unroll
-                for (int i = 1; i < 32; ++i) top = fmaxf(top, x[i >> 4][i & 15]);
-                if (__any(top > m + 8.0f)) {
-                    const float mm = fmaxf(m, column_max2(top));
-                    const float f = __builtin_amdgcn_exp2f(m - mm);
-                    m = mm;
-                    l *= f;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) o[d] *= f;
-                }
-                const bool nans = !whole && (nanFlags[buf][0] | nanFlags[buf][1] | nanFlags[buf][2] | nanFlags[buf][3]);
-#pragma unroll
-                for (int sl = 0; sl < 4; ++sl) {
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        e[i] = __builtin_amdgcn_exp2f(x[sl >> 1][8 * (sl & 1) + i] - (m - 7.0f));
-                        l += e[i];
-                    }
-                    h8 b[TERMS], visible;
-                    weight_terms<TERMS>(e, b);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        visible[i] = (shown >> (8 * sl + i)) & 1u ? (_Float16)1.0f : (_Float16)0.0f;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-                        add_values32<TERMS>(o[d], *(const h8 *)&in.v[32 * d + n][16 * sl + 8 * hh], b, visible, nans);
-                }
-            }
-            if (more) {
-                raise(now);
-                bool nn = store_wide<D>(lds[buf ^ 1u], t, now, vref, T + 64, w.anyLo, end, tid);
-                nn = __any(nn);
-                if (lane == 0) nanFlags[buf ^ 1u][wave] = nn;
-            }
+            const bool all = parts.page[0] >= 0 && parts.page[1] >= 0 && parts.page[2] >= 0 && parts.page[3] >= 0;
+            if (!idle && T < ww.anyHi && T + 64 > ww.anyLo)
+                attend_wide<D, TERMS>(st, lds[buf], parts, qb, qf, all && T >= ww.allLo && T + 64 <= ww.allHi, T, c.lo,
+                                      c.hi, n, hh);
+            if (more) convert(lds[buf ^ 1u], T + 64);
         }
+        if (__syncthreads_or(nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, hh);
     }
-    l = column_sum2(l);
-    seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f;
+    const float l = column_sum2(st.l);
+    const bool seen = column_max2(st.seen ? 1.0f : 0.0f) > 0.0f;
     if (!live) return;
     const float unitOf = vref * 0.0078125f;
-    const float f = p.splits == 1 ? (seen ? unitOf / l : 0.0f) : unitOf;
+    const float f = p.splits == 1 ? unitOf / l : unitOf;
     const size_t to = part_index(p, piece, c.row, c.head);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t at = 32 * d + 8 * i + 4 * hh;
-            f32x4 v = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * f;
+            const f32x4 v = f32x4{st.o[d][4 * i], st.o[d][4 * i + 1], st.o[d][4 * i + 2], st.o[d][4 * i + 3]} * f;
             if (p.splits == 1)
                 store4(p, c.row, c.head, at, D, seen ? v : f32x4{});
             else if (seen)
                 *(f32x4 *)(p.partO + to * D + at) = v;
         }
     if (p.splits > 1 && hh == 0) {
-        p.partML[2 * to] = m;
+        p.partML[2 * to] = st.m;
         p.partML[2 * to + 1] = seen ? l : -1.0f;
     }
 }
@@ -792,8 +823,7 @@ extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
         er_kv8_attend_wide_d##D##_##NAME(ErAttendArgs p) {                                                         \
         __shared__ WideLds<D> tiles[2];                                                                            \
-        __shared__ uint32_t nanFlags[2][4];                                                                        \
-        kv8_attend_wide<D, TERMS>(p, tiles, nanFlags);                                                             \
+        kv8_attend_wide<D, TERMS>(p, tiles);                                                             \
     }
 ER_KV8_ATTEND(64, 1, bf16, 2, 2)
 ER_KV8_ATTEND(64, 2, f32, 2, 2)
