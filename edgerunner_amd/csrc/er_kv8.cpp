@@ -214,36 +214,48 @@ uint32_t row_chunks(uint32_t strips, uint32_t rows, int cu) {
 // How an attention call is cut up.
 struct AttendPlan {
     bool narrow;
-    uint32_t tiles, splits, chunk;
-    uint32_t most;  // pieces at the most, whatever the window
+    uint32_t shares, least;         // narrow kernel
+    uint32_t tiles, splits, chunk;  // wide kernel
+    uint64_t parts;                 // columns that the workspace holds sums of, at the most over all windows
 };
 
 // Columns (rows times query heads of a key/value head) decide the kernel: up
-// to 16 fit the narrow kernel's one matrix tile.  The tokens of a (sequence,
-// head, row tile) are cut into pieces where those alone are too few
-// workgroups, but into no shorter ones than `least`, below which joining costs more than it gives.
+// to 16 fit the narrow kernel's one matrix tile.
 AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group, uint32_t window, int cu) {
     AttendPlan p{};
-    const uint64_t cols = (uint64_t)b->max_rows * group;
+    const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
     p.narrow = cols <= 16;
-    p.tiles = p.narrow ? 1u : (uint32_t)((cols + 127) / 128);
-    const uint64_t rowsOfTile = p.narrow ? b->max_rows : 128 / group + 2;
-    uint64_t span = most_tokens(c, b);
+    p.splits = 1;
+    const uint64_t pairs = (uint64_t)b->sequences * c->kv_heads;
+    if (p.narrow) {
+        // two workgroups a CU are resident (one of head width 256); a
+        // workgroup's start and its part in the join cost as much as some
+        // hundred tokens, so none takes fewer than that, and what a workgroup
+        // a sequence and head reads in that time is not shared at all
+        const uint64_t resident = (uint64_t)cu * (c->head_dim == 256 ? 1 : 2);
+        if (full > 512) {
+            p.shares = (uint32_t)resident;
+            p.least = 4;
+            p.parts = 2 * resident * cols;
+        }
+        return p;
+    }
+    p.tiles = (uint32_t)((cols + 127) / 128);
+    uint64_t span = full;
     // the tile's rows see window + rows - 1 tokens, and pieces begin at a multiple of 64
-    if (window) span = std::min<uint64_t>(span, (uint64_t)window + rowsOfTile + 63);
-    const uint64_t units = (uint64_t)b->sequences * c->kv_heads * p.tiles;
-    const uint64_t want = p.narrow ? (uint64_t)cu * 8 : (uint64_t)cu * 2;
-    const uint64_t least = p.narrow ? 128 : 512;
-    uint64_t splits = std::min<uint64_t>((want + units - 1) / units, (span + least - 1) / least);
-    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, 1024));
-    p.most = (uint32_t)splits;  // grows with the span, and rounding the pieces up to 64 tokens only takes some away
+    if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
+    // the tokens of a (sequence, head, row tile) are cut into pieces where
+    // those alone are too few workgroups
+    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 2, least = 512;
+    auto pieces = [&](uint64_t tokens) {
+        return std::max<uint64_t>(1, std::min<uint64_t>((want + units - 1) / units, (tokens + least - 1) / least));
+    };
+    const uint64_t splits = pieces(span);
     p.chunk = (uint32_t)std::max<uint64_t>(64, ((span + splits - 1) / splits + 63) & ~63ull);
     p.splits = (uint32_t)std::max<uint64_t>(1, (span + p.chunk - 1) / p.chunk);
+    // pieces(span) grows with the span, and rounding pieces up to 64 tokens only takes some away
+    if (pieces(full) > 1) p.parts = pieces(full) * b->rows * group * c->kv_heads;
     return p;
-}
-
-uint64_t part_floats(const er_kv8_batch *b, uint32_t qHeads, uint32_t splits, uint32_t d) {
-    return (uint64_t)splits * b->rows * qHeads * (d + 2u);
 }
 
 er_status check_group(const char *op, const er_kv8_cache *c, uint32_t qHeads) {
@@ -366,9 +378,7 @@ er_status er_hip_kv8_attention_workspace(er_hip_ctx *ctx, const er_kv8_cache *ca
     if (st == ER_OK) st = check_ctx(ctx);
     if (st != ER_OK) return st;
     if (batch->rows == 0 || batch->sequences == 0) return ER_OK;
-    // a window only shortens the span, and with it the pieces at the most
-    const AttendPlan p = plan_attend(cache, batch, q_heads / cache->kv_heads, 0, cu_count_of(ctx));
-    if (p.most > 1) *bytes = part_floats(batch, q_heads, p.most, cache->head_dim) * 4;
+    *bytes = plan_attend(cache, batch, q_heads / cache->kv_heads, 0, cu_count_of(ctx)).parts * (cache->head_dim + 2) * 4;
     return ER_OK;
 }
 
@@ -402,24 +412,25 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     a.half = out_type == ER_TYPE_BF16;
     a.scale = scale * 1.44269504088896340736f;
     const AttendPlan p = plan_attend(cache, batch, a.group, a.window, cu_count_of(ctx));
+    a.shares = p.shares, a.least = p.least;
     a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
-    if (p.splits > 1) {
-        const uint64_t need = part_floats(batch, q->heads, p.splits, d) * 4;
-        st = check_buffer(op, "workspace", workspace, need, 16);
+    const bool joined = p.splits > 1 || p.shares > 0;
+    if (joined) {
+        st = check_buffer(op, "workspace", workspace, p.parts * (d + 2) * 4, 16);
         if (st != ER_OK) return st;
         a.partO = (float *)workspace.data;
-        a.partML = a.partO + (uint64_t)p.splits * batch->rows * q->heads * d;
+        a.partML = a.partO + p.parts * d;
     }
     const Kv8Kernels &kernels = kv8_of(ctx);
     const int di = dim_index(d);
-    const uint64_t units = (uint64_t)batch->sequences * cache->kv_heads * p.splits;
+    const uint64_t pairs = (uint64_t)batch->sequences * cache->kv_heads;
     if (p.narrow)
-        st = launch(kernels.narrow[di][a.half], op, units, 0, stream, &a);
+        st = launch(kernels.narrow[di][a.half], op, p.shares ? p.shares : pairs, 0, stream, &a);
     else
-        st = launch(kernels.wide[di][a.half], op, ((units + 7) & ~7ull) * p.tiles, 0, stream, &a);
-    if (st != ER_OK || p.splits == 1) return st;
-    return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (((p.splits + 3u) & ~3u) + 4 * d) * 4,
-                  stream, &a);
+        st = launch(kernels.wide[di][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
+    if (st != ER_OK || !joined) return st;
+    const uint32_t most = p.shares ? p.shares : p.splits;
+    return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
 }
 
 }  // extern "C"

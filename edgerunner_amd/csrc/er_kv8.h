@@ -60,12 +60,16 @@ struct ErAttendArgs {
     ErKv8Batch b;
     const float *q;
     void *out;
-    float *partO;             // fp32 [splits][rows][heads][head_dim]
-    float *partML;            // fp32 [splits][rows][heads][2]: the reference exponent and the sum of weights
+    float *partO;             // fp32 [parts][head_dim]: sums of columns whose tokens several workgroups share
+    float *partML;            // fp32 [parts][2]: their reference exponents and sums of weights
     uint32_t qStride, outStride;
     uint32_t group;           // query heads of one key/value head
-    uint32_t splits, chunk;   // pieces of a row tile's tokens, and tokens of a piece (a multiple of 64)
-    uint32_t tiles;           // row tiles of a sequence and key/value head (wide kernel)
+    // narrow kernel: workgroups that share the tokens of all sequences evenly,
+    // at least `least` 64-token steps each (0: a workgroup a sequence and head)
+    uint32_t shares, least;
+    // wide kernel: pieces of a row tile's tokens, tokens of a piece (a multiple
+    // of 64), row tiles of a sequence and key/value head
+    uint32_t splits, chunk, tiles;
     uint32_t window;          // 0: none
     uint32_t half;            // bf16 output
     float scale;              // times log2(e)

@@ -72,24 +72,25 @@ ER_DEV Column column_of(const ErAttendArgs &p, const Sequence &q, uint32_t kvHea
 }
 
 // A column's query times the softmax's scale (and log2 e) as B operands: eight
-// consecutive values from `from` on for each of N products, `step` values
-// apart, as one or two fp16 terms.  It is brought to below 1 by a power of two
+// consecutive values for each of N products, those of product k from `from` +
+// k / 2 * pair + k % 2 * next on, as one or two fp16 terms.  It is brought to below 1 by a power of two
 // over the whole head (`join_lanes` takes the largest magnitude over the lanes
 // that share the column); returns that power.  With the keys' scales powers of
 // two as well, a score is its product times a power of two, exactly: the fused
 // multiply-add that takes the reference off it and the product that the
 // reference was taken from agree to the last bit, however large the scores.
 template <int N, int TERMS, typename JOIN>
-ER_DEV float load_query(const float *src, bool live, float scale, uint32_t from, uint32_t step, h8 (&b)[TERMS][N],
-                        JOIN join_lanes) {
+ER_DEV float load_query(const float *src, bool live, float scale, uint32_t from, uint32_t pair, uint32_t next,
+                        h8 (&b)[TERMS][N], JOIN join_lanes) {
     float x[N][8];
     float peak = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         f32x4 lo = {}, hi = {};
         if (live) {
-            lo = *(const f32x4_a4 *)(src + from + k * step);
-            hi = *(const f32x4_a4 *)(src + from + k * step + 4);
+            const float *v = src + from + k / 2 * pair + k % 2 * next;
+            lo = *(const f32x4_a4 *)v;
+            hi = *(const f32x4_a4 *)(v + 4);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -119,14 +120,23 @@ ER_DEV float load_query(const float *src, bool live, float scale, uint32_t from,
 // of a hidden token.
 ER_DEV float score_factor(float qf, float ks) { return fmaxf(qf * ks, 1.2e-38f); }
 
-// Weights of eight tokens as one or two fp16 terms.
+// Weights of eight tokens as one or two fp16 terms.  The conversion is opaque
+// to the compiler, which else converts a first term twice, packed for the
+// product and single for the second term.
+ER_DEV h2 to_h2(float a, float b) {
+    h2 r;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
 template <int TERMS>
 ER_DEV void weight_terms(const float w[8], h8 (&b)[TERMS]) {
+    const h2 p0 = to_h2(w[0], w[1]), p1 = to_h2(w[2], w[3]), p2 = to_h2(w[4], w[5]), p3 = to_h2(w[6], w[7]);
+    b[0] = join(p0, p1, p2, p3);
+    if constexpr (TERMS == 2) {
+        float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const _Float16 h = (_Float16)w[i];
-        b[0][i] = h;
-        if constexpr (TERMS == 2) b[1][i] = (_Float16)(w[i] - (float)h);
+        for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf((float)b[0][i], -1.0f, w[i]);
+        b[1] = join(to_h2(r[0], r[1]), to_h2(r[2], r[3]), to_h2(r[4], r[5]), to_h2(r[6], r[7]));
     }
 }
 
@@ -142,17 +152,16 @@ ER_DEV void store4(const ErAttendArgs &p, int row, uint32_t head, uint32_t d, ui
 ER_DEV size_t part_index(const ErAttendArgs &p, uint32_t piece, int row, uint32_t head) {
     return ((size_t)piece * p.b.rows + (size_t)row) * (p.group * p.c.heads) + head;
 }
-// sum / weight; zeros where no token is visible.  Where some are and the sum
-// of weights is 0 or NaN (scores without a finite maximum), the quotient is
-// NaN, as the softmax's is.
-ER_DEV float quotient(float l, bool visible) { return visible ? 1.0f / l : 0.0f; }
+// A column's output is its sums times 1 / l; zeros where no token is visible.
+// Where some are and l is 0 or NaN (scores without a finite maximum), the
+// quotient is NaN, as the softmax's is.
 
 // ---------------------------------------------------------------- up to 16 columns: decode
 
 // One 32-token tile of keys and values in registers, as loaded.
 template <int D>
 struct NarrowTile {
-    u32x4 k[2][D / 64];      // lane (n, g): token n of each half, bytes [g D/4, (g + 1) D/4)
+    u32x4 k[2][D / 64];      // lane (n, g): token n of each half, bytes 64 j + 16 g .. + 15 (a load reads 64 bytes of a row)
     uint32_t v[D / 64][8];   // lane (n, g): tokens 4 g + i of the first half, then of the second, bytes [n D/16, (n + 1) D/16)
     float ks[2], vs[2];      // the halves' scales
     int page[2];             // the halves' pages; -1: outside the pool, or no visible token
@@ -183,10 +192,10 @@ ER_DEV void load_narrow(NarrowTile<D> &t, const NarrowPages &w, const ErAttendAr
         t.vs[half] = load_shared(p.c.vs + block);
         const uint32_t inside = (uint32_t)(T + 16 * half) & ((1u << p.c.shift) - 1u);
         const size_t base = ((block << p.c.shift) + inside) * D;
-        const uint8_t *kp = p.c.k + base + (n * D + g * (D / 4));
+        const uint8_t *kp = p.c.k + base + (n * D + 16 * g);
         const uint8_t *vp = p.c.v + base + (4 * g * D + n * (D / 16));
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) t.k[half][j] = *(const u32x4 *)(kp + 16 * j);
+        for (int j = 0; j < D / 64; ++j) t.k[half][j] = *(const u32x4 *)(kp + 64 * j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (D == 64) {
@@ -258,16 +267,15 @@ ER_DEV void raise_scale(float to, float &vref, float &vinv, ACC (&o)[N]) {
     for (int j = 0; j < N; ++j) o[j] *= f;
 }
 
-// One tile into the state.  Where some column does not see all of it, or a
-// page is missing, hidden tokens get the score -inf, and those that no column
-// sees have their bytes taken as zeros, whatever they hold.  NaN codes count
-// as zeros too there, since a column may not see them and 0 * NaN is NaN:
+// One tile into the state.  MASKED: some column does not see all of it, or a
+// page is missing.  Hidden tokens get the score -inf there, and those that no
+// column sees have their bytes taken as zeros, whatever they hold.  NaN codes
+// count as zeros too, since a column may not see them and 0 * NaN is NaN:
 // st.nans remembers that there were some, and mark_nans brings them back.
-template <int D, int TERMS>
+template <int D, int TERMS, bool MASKED>
 ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
                           int lo, int hi, const Spans &w, uint32_t g) {
-    const bool ok0 = t.page[0] >= 0, ok1 = t.page[1] >= 0;
-    const bool whole = ok0 && ok1 && T >= w.allLo && T + 32 <= w.allHi;
+    const bool ok0 = !MASKED || t.page[0] >= 0, ok1 = !MASKED || t.page[1] >= 0;
     f32x4 s[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -280,7 +288,7 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
             for (int term = 0; term < TERMS; ++term) s[half] = mfma16(a, qb[term][k], s[half]);
         }
     }
-    if (whole) {
+    if constexpr (!MASKED) {
         st.seen = true;
     } else {
 #pragma unroll
@@ -343,46 +351,126 @@ ER_DEV void mark_nans(NarrowState<D> &st, const ErAttendArgs &p, uint32_t s, uin
     }
 }
 
+// How the tokens of all sequences and heads are shared between workgroups.
+// Units (sequence, head) lie one behind the other, each `length` steps of 64
+// tokens long, and workgroup w takes steps w * quota .. (w + 1) * quota - 1 of
+// that line: whatever the sequences' lengths, all have the same to read.
+// Where there is so little that each takes the least, units begin at multiples
+// of it, so that no workgroup takes two.
+struct Shares {
+    uint32_t quota, total;
+    bool aligned;
+};
+ER_DEV uint32_t steps_of(const ErAttendArgs &p, const Sequence &q) {
+    if (q.n == 0) return 0;
+    const Spans w = spans_of(p, q, 0, (uint32_t)q.n * p.group - 1);
+    // rows that see nothing take a step all the same, which writes their zeros
+    return max(1u, ((uint32_t)max(w.anyHi - (w.anyLo & ~63), 0) + 63u) >> 6);
+}
+ER_DEV uint32_t shared_length(const ErAttendArgs &p, uint32_t steps, bool aligned) {
+    return aligned ? (steps + p.least - 1) / p.least * p.least : steps;
+}
+ER_DEV uint32_t wave_sum(uint32_t v) {
+#pragma unroll
+    for (int x = 32; x; x >>= 1) v += (uint32_t)__shfl_xor((int)v, x);
+    return v;
+}
+ER_DEV Shares shares_of(const ErAttendArgs &p, uint32_t lane) {
+    uint32_t plain = 0, padded = 0;
+    for (uint32_t at = 0; at < p.b.sequences; at += 64) {
+        if (at + lane < p.b.sequences) {
+            const uint32_t t = steps_of(p, sequence_of(p.b, at + lane));
+            plain += t;
+            padded += shared_length(p, t, true);
+        }
+    }
+    plain = uniform(wave_sum(plain)) * p.c.heads;
+    padded = uniform(wave_sum(padded)) * p.c.heads;
+    Shares s;
+    s.aligned = padded <= p.shares * p.least;
+    s.total = s.aligned ? padded : plain;
+    s.quota = s.aligned ? p.least : max(p.least, (plain + p.shares - 1) / p.shares);
+    return s;
+}
+// The sequence that step `at` of the line belongs to, and where it begins.
+ER_DEV uint32_t sequence_at(const ErAttendArgs &p, bool aligned, uint32_t at, uint32_t lane, uint32_t &begins) {
+    uint32_t before = 0;
+    for (uint32_t s0 = 0;; s0 += 64) {
+        const uint32_t mine = s0 + lane < p.b.sequences
+                                  ? shared_length(p, steps_of(p, sequence_of(p.b, s0 + lane)), aligned) * p.c.heads
+                                  : 0u;
+        uint32_t upTo = mine;  // inclusive prefix sum over the wave
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t other = (uint32_t)__shfl_up((int)upTo, x);
+            if ((int)lane >= x) upTo += other;
+        }
+        const uint64_t past = __ballot(before + upTo > at);
+        if (past || s0 + 64 >= p.b.sequences) {
+            const int i = past ? (int)__ffsll((unsigned long long)past) - 1 : 63;
+            begins = before + (uint32_t)__builtin_amdgcn_readlane((int)(upTo - mine), i);
+            return s0 + (uint32_t)i;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
+    }
+}
+
 // Up to 16 columns (rows of one sequence times query heads of one key/value
-// head) against one piece of its tokens: bound by the bytes of the cache.
-// Every wave takes each fourth 32-token tile straight into registers, 8 KB of
-// codes at head width 128, with the next tile in flight while it works; keys
-// and values need no exchange between lanes, so nothing passes through LDS
-// until the waves' sums are joined at the end.
+// head) against steps [from, to) of their tokens: bound by the bytes of the
+// cache.  Every wave takes each fourth 32-token tile straight into registers,
+// 8 KB of codes at head width 128, with the next tile in flight while it
+// works; keys and values need no exchange between lanes, so nothing passes
+// through LDS until the waves' sums are joined at the end.  The sums of all
+// steps are the columns' outputs; else they go to part `part`.
 template <int D, int TERMS>
-ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
-    const uint32_t piece = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-    const uint32_t h = unit % p.c.heads, s = unit / p.c.heads;
+ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, uint32_t h, uint32_t from, uint32_t to, bool complete,
+                        uint32_t part, float *lds) {
     const Sequence q = sequence_of(p.b, s);
-    if (q.n == 0) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t cols = (uint32_t)q.n * p.group;
     const Spans w = spans_of(p, q, 0, cols - 1);
-    const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
+    const int base = w.anyLo & ~63, begin = base + 64 * (int)from, end = min(w.anyHi, base + 64 * (int)to);
     const Column c = column_of(p, q, h, min(n, cols - 1));
 
+    // The tiles that all columns see whole go through a loop of their own, two
+    // in registers at a time; the few others (ends, missing pages) follow one
+    // by one.  A branch between the two around the sums would have them copied.
+    auto whole = [&](const NarrowPages &k, int T) {
+        return k.page[0] >= 0 && k.page[1] >= 0 && T >= w.allLo && T + 32 <= w.allHi;
+    };
+    NarrowPages pages;
+    int rest = end;  // the first tile that is not whole
+    auto next_whole = [&](int T) {  // the wave's next whole tile from T on, its pages in `pages`; `end` if there is none
+        for (; T < end; T += 128) {
+            pages = narrow_pages(p, s, T, w.anyLo, end);
+            if (whole(pages, T)) return T;
+            rest = min(rest, T);
+        }
+        return end;
+    };
     NarrowTile<D> t0, t1;
-    int T = begin + 32 * (int)wave;
-    NarrowPages pages = narrow_pages(p, s, T, w.anyLo, end);
+    int T = next_whole(begin + 32 * (int)wave);
     if (T < end) load_narrow<D>(t0, pages, p, h, T, n, g);
-    pages = narrow_pages(p, s, T + 128, w.anyLo, end);
+    int U = next_whole(T + 128);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
-                                               p.scale, g * (D / 4), 8, qb, column_max4);
+                                               p.scale, 16 * g, 64, 8, qb, column_max4);
     NarrowState<D> st = {};
     st.m = ER_NO_MAX;
-    auto step = [&](NarrowTile<D> &now, NarrowTile<D> &next) {
-        if (T + 128 < end) {
-            load_narrow<D>(next, pages, p, h, T + 128, n, g);
-            pages = narrow_pages(p, s, T + 256, w.anyLo, end);
-        }
-        if (now.page[0] >= 0 || now.page[1] >= 0) attend_narrow<D, TERMS>(st, now, qb, qf, T, c.lo, c.hi, w, g);
-        T += 128;
-    };
     while (T < end) {
-        step(t0, t1);
-        if (T >= end) break;
-        step(t1, t0);
+        if (U < end) load_narrow<D>(t1, pages, p, h, U, n, g);
+        T = next_whole(U + 128);
+        attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
+        if (U >= end) break;
+        if (T < end) load_narrow<D>(t0, pages, p, h, T, n, g);
+        U = next_whole(T + 128);
+        attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
+    }
+    for (T = rest; T < end; T += 128) {
+        pages = narrow_pages(p, s, T, w.anyLo, end);
+        if (whole(pages, T) || (pages.page[0] < 0 && pages.page[1] < 0)) continue;
+        load_narrow<D>(t0, pages, p, h, T, n, g);
+        attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g);
     }
     // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
     if (__any(st.nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, g);
@@ -393,13 +481,13 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     const float l = column_sum4(st.l);
     const bool seen = column_max4(st.seen ? 1.0f : 0.0f) > 0.0f;
     if (n < cols) {
-        float *to = lds + (wave * cols + n) * PITCH;
+        float *at = lds + (wave * cols + n) * PITCH;
         const float f = st.vref * 0.0078125f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < D / 16; j += 4)
-                *(f32x4 *)(to + (4 * g + i) * (D / 16) + j) =
+                *(f32x4 *)(at + (4 * g + i) * (D / 16) + j) =
                     f32x4{st.o[j][i] * f, st.o[j + 1][i] * f, st.o[j + 2][i] * f, st.o[j + 3][i] * f};
         if (g == 0) {
             sm[wave * 16 + n] = st.m;
@@ -416,25 +504,61 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
         f32x4 o = {};
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-            const float part = sl[v * 16 + col];
-            if (part < 0.0f) continue;
+            const float l = sl[v * 16 + col];
+            if (l < 0.0f) continue;
             visible = true;
             const float f = __builtin_amdgcn_exp2f(sm[v * 16 + col] - m);
-            total += part * f;
+            total += l * f;
             o += *(const f32x4 *)(lds + (v * cols + col) * PITCH + d) * f;
         }
-        const Column k = column_of(p, q, h, col);
-        if (p.splits == 1) {
-            const float r = quotient(total, visible);
-            store4(p, k.row, k.head, d, D, visible ? o * r : f32x4{});
+        if (complete) {
+            const Column k = column_of(p, q, h, col);
+            store4(p, k.row, k.head, d, D, visible ? o * (1.0f / total) : f32x4{});
         } else {
-            const size_t to = part_index(p, piece, k.row, k.head);
-            if (visible) *(f32x4 *)(p.partO + to * D + d) = o;
+            const size_t at = (size_t)part * (p.b.maxRows * p.group) + col;
+            if (visible) *(f32x4 *)(p.partO + at * D + d) = o;
             if (d == 0) {
-                p.partML[2 * to] = m;
-                p.partML[2 * to + 1] = visible ? total : -1.0f;
+                p.partML[2 * at] = m;
+                p.partML[2 * at + 1] = visible ? total : -1.0f;
             }
         }
+    }
+}
+
+template <int D, int TERMS>
+ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
+    const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
+    if (p.shares == 0) {
+        const uint32_t s = blockIdx.x / H, h = blockIdx.x % H, steps = steps_of(p, sequence_of(p.b, s));
+        if (steps) narrow_unit<D, TERMS>(p, s, h, 0, steps, true, 0, lds);
+        return;
+    }
+    const Shares sh = shares_of(p, lane);
+    uint32_t at = blockIdx.x * sh.quota;
+    const uint32_t last = min(at + sh.quota, sh.total);
+    if (at >= last) return;
+    uint32_t begins, s = uniform(sequence_at(p, sh.aligned, at, lane, begins));
+    begins = uniform(begins);
+    uint32_t steps = steps_of(p, sequence_of(p.b, s)), length = shared_length(p, steps, sh.aligned);
+    uint32_t h = (at - begins) / length;
+    begins += h * length;
+    while (true) {
+        // a unit that begins here and goes on in later workgroups leaves its
+        // sums in this one's second part, one that began earlier in its first
+        const uint32_t from = at - begins, to = min(last - begins, steps);
+        narrow_unit<D, TERMS>(p, s, h, from, to, from == 0 && to == steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u), lds);
+        begins += length;
+        at = begins;
+        if (at >= last) return;
+        if (++h == H) {
+            h = 0;
+            do {
+                ++s;
+                steps = steps_of(p, sequence_of(p.b, s));
+            } while (steps == 0);
+            length = shared_length(p, steps, sh.aligned);
+        }
+        __syncthreads();  // the sums in LDS have been read
     }
 }
 
@@ -690,7 +814,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
         wide_scales(now, p, h);
         h8 qb[TERMS][D / 16];
         const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live,
-                                                   p.scale, hh * 8, 16, qb, column_max2);
+                                                   p.scale, 8 * hh, 32, 16, qb, column_max2);
         // the sums are in units of the reference that their tiles were converted
         // with, one tile behind the conversion's
         float unit = 0.0f;
@@ -760,56 +884,76 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
 
 // ---------------------------------------------------------------- joining the pieces
 
-// One row and head's pieces: weights 2^(m - max) / sum from the references and
-// sums, then the weighted outputs; a quarter of the pieces to each wave.
-template <int D>
-ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
-    const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
-    const uint32_t s = uniform(sequence_of_row(p.b, row, lane));
-    if (s >= p.b.sequences) return;
-    const Sequence q = sequence_of(p.b, s);
-    if ((int)row < q.row0 || (int)row >= q.row0 + q.n) return;
-    float *weight = lds, *red = lds + ((p.splits + 3u) & ~3u);  // [splits], [4][D]
+// One column's parts: weights 2^(m - max) / sum from the references and sums,
+// then the weighted outputs, D / 4 lanes a part.  index(i): where part i lies.
+template <int D, typename INDEX>
+ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t head, float *lds, INDEX index) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    float *red = lds, *weight = lds + 4 * ER_KV8_THREADS;  // [lanes][4], [parts]
     float top = ER_NO_MAX;
-    for (uint32_t i = lane; i < p.splits; i += 64) top = fmaxf(top, p.partML[2 * part_index(p, i, (int)row, head)]);
+    for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, p.partML[2 * index(i)]);
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     float total = 0.0f;
     bool seen = false;
-    for (uint32_t i = lane; i < p.splits; i += 64) {
-        const size_t at = 2 * part_index(p, i, (int)row, head);
+    for (uint32_t i = lane; i < parts; i += 64) {
+        const size_t at = 2 * index(i);
         const float l = p.partML[at + 1];
-        const float f = l < 0.0f ? -1.0f : __builtin_amdgcn_exp2f(p.partML[at] - top);
-        if (!(l < 0.0f)) {
-            total += l * f;
-            seen = true;
-        }
-        if (wave == 0) weight[i] = f;
+        const bool some = !(l < 0.0f);
+        const float f = some ? __builtin_amdgcn_exp2f(p.partML[at] - top) : -1.0f;
+        if (some) total += l * f;
+        seen |= some;
+        if (tid < 64) weight[i] = f;
     }
     // every wave has the sum, of the same terms in the same order
 #pragma unroll
     for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
     seen = __any(seen);
     __syncthreads();
-    constexpr int PER = D / 64;
-    float o[PER] = {};
-    for (uint32_t i = wave; i < p.splits; i += 4) {
+    constexpr uint32_t LANES = D / 4, AT_ONCE = ER_KV8_THREADS / LANES;
+    const uint32_t mine = tid / LANES, d = (tid % LANES) * 4;
+    f32x4 o = {};
+#pragma unroll 4
+    for (uint32_t i = mine; i < parts; i += AT_ONCE) {
         const float f = weight[i];
-        if (f < 0.0f) continue;
-        const float *src = p.partO + part_index(p, i, (int)row, head) * D + lane * PER;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] += f * src[j];
+        if (f >= 0.0f || f != f) o += *(const f32x4 *)(p.partO + index(i) * D + d) * f;
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) red[wave * D + lane * PER + j] = o[j];
+    *(f32x4 *)(red + 4 * tid) = o;
     __syncthreads();
-    if (tid < D / 4) {
+    if (tid < LANES) {
         f32x4 v = {};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v += *(const f32x4 *)(red + k * D + 4 * tid);
-        store4(p, (int)row, head, 4 * tid, D, seen ? v * quotient(total, true) : f32x4{});
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v += *(const f32x4 *)(red + 4 * (k * LANES + tid));
+        store4(p, row, head, 4 * tid, D, seen ? v * (1.0f / total) : f32x4{});
     }
+}
+
+// One row and query head after the wide kernel (a part a piece) or the narrow
+// one (a part a workgroup that had some of the unit's steps).
+template <int D>
+ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
+    const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t s = uniform(sequence_of_row(p.b, row, lane));
+    if (s >= p.b.sequences) return;
+    const Sequence q = sequence_of(p.b, s);
+    if ((int)row < q.row0 || (int)row >= q.row0 + q.n) return;
+    if (p.shares == 0) {
+        join_parts<D>(p, p.splits, (int)row, head, lds, [&](uint32_t i) { return part_index(p, i, (int)row, head); });
+        return;
+    }
+    const Shares sh = shares_of(p, lane);
+    uint32_t before = 0;
+    for (uint32_t i = lane; i < s; i += 64) before += shared_length(p, steps_of(p, sequence_of(p.b, i)), sh.aligned);
+    before = uniform(wave_sum(before)) * p.c.heads;
+    const uint32_t steps = steps_of(p, q);
+    const uint32_t begins = before + head / p.group * shared_length(p, steps, sh.aligned);
+    const uint32_t w0 = begins / sh.quota, parts = (begins + steps - 1) / sh.quota - w0 + 1;
+    if (parts == 1) return;  // one workgroup had it all and wrote it
+    const uint32_t cols = p.b.maxRows * p.group, col = (row - (uint32_t)q.row0) * p.group + head % p.group;
+    join_parts<D>(p, parts, (int)row, head, lds, [&](uint32_t i) {
+        return (size_t)(2 * (w0 + i) + (i == 0 ? 1u : 0u)) * cols + col;
+    });
 }
 
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];

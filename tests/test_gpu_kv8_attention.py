@@ -115,6 +115,30 @@ def test_split_along_the_cache(ctx, d, P, hq, hkv, lens, rows, window, half):
     c.check(c.run(half, window), half, window)
 
 
+@pytest.mark.parametrize("d,P,hq,hkv,lens,rows,window", [
+    (64, 16, 8, 8, [9000, 30, 0, 7000, 4500, 1, 700], [1, 1, 0, 1, 1, 1, 1], 0),
+    (64, 32, 16, 8, [12000, 64, 128, 6000, 2000], [2, 1, 8, 3, 5], 0),
+    (128, 64, 16, 8, [20000, 500], [1, 2], 0), (256, 64, 4, 4, [11000, 7000, 100], [1, 1, 4], 0),
+    (64, 64, 8, 8, [30000, 20000, 3000], [1, 3, 2], 9000)])
+def test_shared_evenly(ctx, d, P, hq, hkv, lens, rows, window):
+    """Enough tokens that workgroups' shares begin and end inside sequences and span several heads and sequences."""
+    c = Case(ctx, d + len(lens), lens, rows, P, d, hq, hkv, behind=1)
+    c.check(c.run(window=window), window=window)
+
+
+@pytest.mark.parametrize("many", [150, 64, 65])
+def test_shared_between_many_sequences(ctx, many):
+    """More sequences than a wave has lanes, some of them empty, in aligned and in even shares."""
+    rng = np.random.default_rng(many)
+    for most in (600, 4000):
+        lens = [int(x) for x in rng.integers(0, most, many)]
+        lens[many // 2] = 0
+        lens[-1] = most
+        rows = [min(n, 1) for n in lens]
+        c = Case(ctx, many, lens, rows, 64, 64, 2, 2)
+        c.check(c.run())
+
+
 # A lone token's weight is 2^(7 + e), e the rounding of its reference less 7; the sum holds it in fp32, the product with the
 # value rounded to two fp16 terms (2^-22 of it), and the quotient rounds three times (each 2^-24): the value comes back to
 LONE = 2.0 ** -22 + 3 * 2.0 ** -24
@@ -327,7 +351,8 @@ def test_captured_and_replayed_with_later_lengths(ctx):
             got = ob.download(np.float32).reshape(c.q.shape)
             c.raw = got
             c.check(got.astype(np.float64))
-            assert np.array_equal(c.run().astype(np.float32), got)
+            eager = c.run(batch=c.b.upload(ctx, max_len=900))  # the recorded call's bounds, so its cuts and bits
+            assert np.array_equal(eager.astype(np.float32), got)
         cap.graph.destroy()
         del held
         st.destroy()
