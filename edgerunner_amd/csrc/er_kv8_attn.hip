@@ -351,6 +351,11 @@ ER_DEV void mark_nans(NarrowState<D> &st, const ErAttendArgs &p, uint32_t s, uin
     }
 }
 
+template <int N>
+struct Const {
+    static constexpr int value = N;
+};
+
 // How the tokens of all sequences and heads are shared between workgroups.
 // Units (sequence, head) lie one behind the other, each `length` steps of 64
 // tokens long, and workgroup w takes steps w * quota .. (w + 1) * quota - 1 of
@@ -370,22 +375,55 @@ ER_DEV uint32_t steps_of(const ErAttendArgs &p, const Sequence &q) {
 ER_DEV uint32_t shared_length(const ErAttendArgs &p, uint32_t steps, bool aligned) {
     return aligned ? (steps + p.least - 1) / p.least * p.least : steps;
 }
-ER_DEV uint32_t wave_sum(uint32_t v) {
-#pragma unroll
-    for (int x = 32; x; x >>= 1) v += (uint32_t)__shfl_xor((int)v, x);
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then row ends
+// into the rows behind.
+ER_DEV uint32_t wave_prefix(uint32_t v) {
+    auto from = [](uint32_t x, auto ctrl, auto rows) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    v += from(v, Const<0x111>{}, Const<0xf>{});  // lanes 1, 2, 4 and 8 before
+    v += from(v, Const<0x112>{}, Const<0xf>{});
+    v += from(v, Const<0x114>{}, Const<0xf>{});
+    v += from(v, Const<0x118>{}, Const<0xf>{});
+    v += from(v, Const<ER_DPP_ROW_BCAST15>{}, Const<0xa>{});
+    v += from(v, Const<ER_DPP_ROW_BCAST31>{}, Const<0xc>{});
     return v;
 }
-ER_DEV Shares shares_of(const ErAttendArgs &p, uint32_t lane) {
-    uint32_t plain = 0, padded = 0;
-    for (uint32_t at = 0; at < p.b.sequences; at += 64) {
-        if (at + lane < p.b.sequences) {
-            const uint32_t t = steps_of(p, sequence_of(p.b, at + lane));
-            plain += t;
-            padded += shared_length(p, t, true);
-        }
+ER_DEV uint32_t lane_of(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
+ER_DEV uint32_t wave_sum(uint32_t v) { return lane_of(wave_prefix(v), 63); }
+
+// Lane i's sequence of the first 64, loaded once: most batches have no more,
+// and what a workgroup needs to know of others then passes between lanes.
+struct LaneSequence {
+    Sequence q;
+    uint32_t steps;
+};
+ER_DEV LaneSequence lane_sequence(const ErAttendArgs &p, uint32_t s) {
+    LaneSequence l = {};
+    if (s < p.b.sequences) {
+        l.q = sequence_of(p.b, s);
+        l.steps = steps_of(p, l.q);
     }
-    plain = uniform(wave_sum(plain)) * p.c.heads;
-    padded = uniform(wave_sum(padded)) * p.c.heads;
+    return l;
+}
+ER_DEV LaneSequence lane_sequence_at(const ErAttendArgs &p, const LaneSequence &first, uint32_t s) {
+    if (s >= 64) return lane_sequence(p, s);
+    LaneSequence l;
+    l.q.row0 = (int)lane_of((uint32_t)first.q.row0, s);
+    l.q.n = (int)lane_of((uint32_t)first.q.n, s);
+    l.q.len = (int)lane_of((uint32_t)first.q.len, s);
+    l.steps = lane_of(first.steps, s);
+    return l;
+}
+ER_DEV Shares shares_of(const ErAttendArgs &p, const LaneSequence &first, uint32_t lane) {
+    uint32_t plain = first.steps, padded = shared_length(p, first.steps, true);
+    for (uint32_t at = 64; at < p.b.sequences; at += 64) {
+        const uint32_t t = lane_sequence(p, at + lane).steps;
+        plain += t;
+        padded += shared_length(p, t, true);
+    }
+    plain = wave_sum(plain) * p.c.heads;
+    padded = wave_sum(padded) * p.c.heads;
     Shares s;
     s.aligned = padded <= p.shares * p.least;
     s.total = s.aligned ? padded : plain;
@@ -393,25 +431,19 @@ ER_DEV Shares shares_of(const ErAttendArgs &p, uint32_t lane) {
     return s;
 }
 // The sequence that step `at` of the line belongs to, and where it begins.
-ER_DEV uint32_t sequence_at(const ErAttendArgs &p, bool aligned, uint32_t at, uint32_t lane, uint32_t &begins) {
+ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bool aligned, uint32_t at, uint32_t lane,
+                            uint32_t &begins) {
     uint32_t before = 0;
     for (uint32_t s0 = 0;; s0 += 64) {
-        const uint32_t mine = s0 + lane < p.b.sequences
-                                  ? shared_length(p, steps_of(p, sequence_of(p.b, s0 + lane)), aligned) * p.c.heads
-                                  : 0u;
-        uint32_t upTo = mine;  // inclusive prefix sum over the wave
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-            const uint32_t other = (uint32_t)__shfl_up((int)upTo, x);
-            if ((int)lane >= x) upTo += other;
-        }
+        const uint32_t steps = s0 ? lane_sequence(p, s0 + lane).steps : first.steps;
+        const uint32_t mine = shared_length(p, steps, aligned) * p.c.heads, upTo = wave_prefix(mine);
         const uint64_t past = __ballot(before + upTo > at);
         if (past || s0 + 64 >= p.b.sequences) {
-            const int i = past ? (int)__ffsll((unsigned long long)past) - 1 : 63;
-            begins = before + (uint32_t)__builtin_amdgcn_readlane((int)(upTo - mine), i);
-            return s0 + (uint32_t)i;
+            const uint32_t i = past ? (uint32_t)__ffsll((unsigned long long)past) - 1u : 63u;
+            begins = before + lane_of(upTo - mine, i);
+            return s0 + i;
         }
-        before += (uint32_t)__builtin_amdgcn_readlane((int)upTo, 63);
+        before += lane_of(upTo, 63);
     }
 }
 
@@ -423,9 +455,8 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, bool aligned, uint32_t at, ui
 // through LDS until the waves' sums are joined at the end.  The sums of all
 // steps are the columns' outputs; else they go to part `part`.
 template <int D, int TERMS>
-ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, uint32_t h, uint32_t from, uint32_t to, bool complete,
-                        uint32_t part, float *lds) {
-    const Sequence q = sequence_of(p.b, s);
+ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t from, uint32_t to,
+                        bool complete, uint32_t part, float *lds) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t cols = (uint32_t)q.n * p.group;
     const Spans w = spans_of(p, q, 0, cols - 1);
@@ -529,34 +560,34 @@ template <int D, int TERMS>
 ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
     if (p.shares == 0) {
-        const uint32_t s = blockIdx.x / H, h = blockIdx.x % H, steps = steps_of(p, sequence_of(p.b, s));
-        if (steps) narrow_unit<D, TERMS>(p, s, h, 0, steps, true, 0, lds);
+        const uint32_t s = blockIdx.x / H, h = blockIdx.x % H;
+        const LaneSequence l = lane_sequence(p, s);
+        if (l.steps) narrow_unit<D, TERMS>(p, s, l.q, h, 0, l.steps, true, 0, lds);
         return;
     }
-    const Shares sh = shares_of(p, lane);
+    const LaneSequence first = lane_sequence(p, lane);
+    const Shares sh = shares_of(p, first, lane);
     uint32_t at = blockIdx.x * sh.quota;
     const uint32_t last = min(at + sh.quota, sh.total);
     if (at >= last) return;
-    uint32_t begins, s = uniform(sequence_at(p, sh.aligned, at, lane, begins));
-    begins = uniform(begins);
-    uint32_t steps = steps_of(p, sequence_of(p.b, s)), length = shared_length(p, steps, sh.aligned);
-    uint32_t h = (at - begins) / length;
+    uint32_t begins, s = sequence_at(p, first, sh.aligned, at, lane, begins);
+    LaneSequence l = lane_sequence_at(p, first, s);
+    uint32_t length = shared_length(p, l.steps, sh.aligned), h = (at - begins) / length;
     begins += h * length;
     while (true) {
         // a unit that begins here and goes on in later workgroups leaves its
         // sums in this one's second part, one that began earlier in its first
-        const uint32_t from = at - begins, to = min(last - begins, steps);
-        narrow_unit<D, TERMS>(p, s, h, from, to, from == 0 && to == steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u), lds);
+        const uint32_t from = at - begins, to = min(last - begins, l.steps);
+        narrow_unit<D, TERMS>(p, s, l.q, h, from, to, from == 0 && to == l.steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u),
+                              lds);
         begins += length;
         at = begins;
         if (at >= last) return;
         if (++h == H) {
             h = 0;
-            do {
-                ++s;
-                steps = steps_of(p, sequence_of(p.b, s));
-            } while (steps == 0);
-            length = shared_length(p, steps, sh.aligned);
+            do l = lane_sequence_at(p, first, ++s);
+            while (l.steps == 0);
+            length = shared_length(p, l.steps, sh.aligned);
         }
         __syncthreads();  // the sums in LDS have been read
     }
@@ -884,6 +915,17 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
 
 // ---------------------------------------------------------------- joining the pieces
 
+ER_DEV float wave_top(float v) {
+    v = dpp_max<ER_DPP_QUAD_XOR1>(v);
+    v = dpp_max<ER_DPP_QUAD_XOR2>(v);
+    v = dpp_max<ER_DPP_ROW_HALF_MIRROR>(v);
+    v = dpp_max<ER_DPP_ROW_MIRROR>(v);
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16 * i));
+    return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+}
+
 // One column's parts: weights 2^(m - max) / sum from the references and sums,
 // then the weighted outputs, D / 4 lanes a part.  index(i): where part i lies.
 template <int D, typename INDEX>
@@ -892,8 +934,7 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
     float *red = lds, *weight = lds + 4 * ER_KV8_THREADS;  // [lanes][4], [parts]
     float top = ER_NO_MAX;
     for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, p.partML[2 * index(i)]);
-#pragma unroll
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    top = wave_top(top);
     float total = 0.0f;
     bool seen = false;
     for (uint32_t i = lane; i < parts; i += 64) {
@@ -906,8 +947,7 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
         if (tid < 64) weight[i] = f;
     }
     // every wave has the sum, of the same terms in the same order
-#pragma unroll
-    for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
+    total = group_sum<64>(total);
     seen = __any(seen);
     __syncthreads();
     constexpr uint32_t LANES = D / 4, AT_ONCE = ER_KV8_THREADS / LANES;
@@ -934,21 +974,22 @@ template <int D>
 ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
     const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
     const uint32_t lane = threadIdx.x & 63u;
+    const LaneSequence first = lane_sequence(p, lane);
     const uint32_t s = uniform(sequence_of_row(p.b, row, lane));
     if (s >= p.b.sequences) return;
-    const Sequence q = sequence_of(p.b, s);
+    const LaneSequence l = lane_sequence_at(p, first, s);
+    const Sequence &q = l.q;
     if ((int)row < q.row0 || (int)row >= q.row0 + q.n) return;
     if (p.shares == 0) {
         join_parts<D>(p, p.splits, (int)row, head, lds, [&](uint32_t i) { return part_index(p, i, (int)row, head); });
         return;
     }
-    const Shares sh = shares_of(p, lane);
-    uint32_t before = 0;
-    for (uint32_t i = lane; i < s; i += 64) before += shared_length(p, steps_of(p, sequence_of(p.b, i)), sh.aligned);
-    before = uniform(wave_sum(before)) * p.c.heads;
-    const uint32_t steps = steps_of(p, q);
-    const uint32_t begins = before + head / p.group * shared_length(p, steps, sh.aligned);
-    const uint32_t w0 = begins / sh.quota, parts = (begins + steps - 1) / sh.quota - w0 + 1;
+    const Shares sh = shares_of(p, first, lane);
+    uint32_t before = lane < s ? shared_length(p, first.steps, sh.aligned) : 0;
+    for (uint32_t i = 64 + lane; i < s; i += 64) before += shared_length(p, lane_sequence(p, i).steps, sh.aligned);
+    before = wave_sum(before) * p.c.heads;
+    const uint32_t begins = before + head / p.group * shared_length(p, l.steps, sh.aligned);
+    const uint32_t w0 = begins / sh.quota, parts = (begins + l.steps - 1) / sh.quota - w0 + 1;
     if (parts == 1) return;  // one workgroup had it all and wrote it
     const uint32_t cols = p.b.maxRows * p.group, col = (row - (uint32_t)q.row0) * p.group + head % p.group;
     join_parts<D>(p, parts, (int)row, head, lds, [&](uint32_t i) {
