@@ -120,12 +120,12 @@ ER_DEV float load_query(const float *src, bool live, float scale, uint32_t from,
 // of a hidden token.
 ER_DEV float score_factor(float qf, float ks) { return fmaxf(qf * ks, 1.2e-38f); }
 
-// Weights of eight tokens as one or two fp16 terms.  The conversion is opaque
-// to the compiler, which else converts a first term twice, packed for the
-// product and single for the second term.
+// Weights of eight tokens as one or two fp16 terms.  The pair is hidden from
+// the compiler (by no instruction at all), which else converts a first term
+// twice, packed for the product and single for the second term.
 ER_DEV h2 to_h2(float a, float b) {
-    h2 r;
-    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    h2 r = {(_Float16)a, (_Float16)b};
+    asm("" : "+v"(r));
     return r;
 }
 template <int TERMS>
@@ -676,43 +676,45 @@ struct WideLds {
     _Float16 v[D][ER_WIDE_TOKENS + 8];
 };
 
-// A tile into LDS.  MIXED (some column of the workgroup does not see all of
-// it): as attend_narrow's masked tiles; true where there were NaN codes.
-template <int D, bool MIXED>
-ER_DEV bool store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w, float vinv, int T, int lo, int hi,
-                       uint32_t tid) {
-    {
-        _Float16 *dst = &to.k[tid >> 2][(tid & 3u) * (D / 4)];
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            *(h8 *)(dst + 16 * j) = codes_to_h8(t.k[j].x, t.k[j].y);
-            *(h8 *)(dst + 16 * j + 8) = codes_to_h8(t.k[j].z, t.k[j].w);
-        }
-    }
+// The values of a tile that some column of the workgroup does not see whole,
+// as attend_narrow's masked tiles; true where there were NaN codes.
+template <int D>
+ER_DEV bool mask_wide(WideTile<D> &t, const WideParts &w, int T, int lo, int hi, uint32_t tid) {
     bool nan = false;
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));
-        const bool ok = !MIXED || pick4(w.page, it.part) >= 0;
-        uint32_t c[8];
+        const bool ok = pick4(w.page, it.part) >= 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            c[i] = t.v[r][i];
-            if constexpr (MIXED) {
-                const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
-                c[i] = ok && tok >= lo && tok < hi ? c[i] : 0u;
-                const uint32_t nans = nan_codes(c[i]);
-                nan |= nans != 0;
-                c[i] &= ~nans;
-            }
+            const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
+            const uint32_t c = ok && tok >= lo && tok < hi ? t.v[r][i] : 0u, nans = nan_codes(c);
+            nan |= nans != 0;
+            t.v[r][i] = c & ~nans;
         }
+    }
+    return nan;
+}
+
+// A tile into LDS as fp16, values in units of the reference scale.
+template <int D>
+ER_DEV void store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w, float vinv, uint32_t tid) {
+    _Float16 *dst = &to.k[tid >> 2][(tid & 3u) * (D / 4)];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        *(h8 *)(dst + 16 * j) = codes_to_h8(t.k[j].x, t.k[j].y);
+        *(h8 *)(dst + 16 * j + 8) = codes_to_h8(t.k[j].z, t.k[j].w);
+    }
+#pragma unroll
+    for (int r = 0; r < (D + 127) / 128; ++r) {
+        const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));
+        // a missing page's values are zeros: any finite scale does
+        const float f = pick4(w.page, it.part) >= 0 ? pick4(w.vs, it.part) * vinv : 1.0f;
         h8 a[4];
-        const float f = ok ? pick4(w.vs, it.part) * vinv : 1.0f;
-        transpose_codes(c, f, f, a);
+        transpose_codes(t.v[r], f, f, a);
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(h8 *)&to.v[4 * it.dword + j][8 * it.slot] = a[j];
     }
-    return nan;
 }
 
 ER_DEV float column_max2(float v) {
@@ -724,71 +726,17 @@ ER_DEV float column_sum2(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Running state of a wave's 32 columns, as NarrowState's.
-template <int D>
+// Running state of a wave's NC x 32 columns, as NarrowState's.
+template <int D, int NC>
 struct WideState {
-    f32x16 o[D / 32];  // o[d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n
-    float m, l;
-    bool seen;
+    f32x16 o[NC][D / 32];  // o[c][d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n of 32-column block c
+    float m[NC], l[NC];
+    bool seen[NC];
 };
-
-// One tile into the state, as attend_narrow; `whole`: this wave's columns see all of it.
-template <int D, int TERMS>
-ER_DEV void attend_wide(WideState<D> &st, const WideLds<D> &in, const WideParts &parts, const h8 (&qb)[TERMS][D / 16],
-                        float qf, bool whole, int T, int lo, int hi, uint32_t n, uint32_t hh) {
-    f32x16 s[2];
-#pragma unroll
-    for (int th = 0; th < 2; ++th) {
-        s[th] = f32x16{};
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) s[th] = mfma32(a, qb[term][k], s[th]);
-        }
-    }
-    if (whole) {
-        st.seen = true;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int tok = T + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * (int)hh + (i & 3);
-            const bool shown = parts.page[i >> 3] >= 0 && tok >= lo && tok < hi;
-            st.seen |= shown;
-            s[i >> 4][i & 15] = shown ? s[i >> 4][i & 15] : -__builtin_inff();
-        }
-    }
-    float f[4], top = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = score_factor(qf, parts.page[i] >= 0 ? parts.ks[i] : 1.0f);
-        float most = s[i >> 1][8 * (i & 1)];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) most = fmaxf(most, s[i >> 1][8 * (i & 1) + j]);
-        top = fmaxf(top, most * f[i]);
-    }
-    if (__any(top > st.m + 8.0f)) raise_reference(fmaxf(st.m, column_max2(top)), st.m, st.l, st.o);
-    const float m7 = st.m - 7.0f;
-#pragma unroll
-    for (int sl = 0; sl < 4; ++sl) {
-        float e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(s[sl >> 1][8 * (sl & 1) + i] * f[sl] - m7);
-        st.l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-        h8 b[TERMS];
-        weight_terms<TERMS>(e, b);
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-            const h8 a = *(const h8 *)&in.v[32 * d + n][16 * sl + 8 * hh];
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) st.o[d] = mfma32(a, b[term], st.o[d]);
-        }
-    }
-}
 
 // As the narrow kernel's.
 template <int D>
-ER_DEV void mark_nans(WideState<D> &st, const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
+ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
                       int hi, uint32_t hh) {
     for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
         const int page = page_of(p.b, p.c, s, tok);
@@ -802,17 +750,18 @@ ER_DEV void mark_nans(WideState<D> &st, const ErAttendArgs &p, uint32_t s, uint3
                 const uint32_t nan = nan_codes(*(const uint32_t *)(v + 32 * d + 8 * i + 4 * hh));
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    st.o[d][4 * i + j] = (nan >> (8 * j)) & 1u ? __builtin_nanf("") : st.o[d][4 * i + j];
+                    o[d][4 * i + j] = (nan >> (8 * j)) & 1u ? __builtin_nanf("") : o[d][4 * i + j];
             }
     }
 }
 
-// 128 columns against one piece of their sequence's tokens, 32 columns a wave:
-// bound by the matrix products and the softmax's exponentials.  The four waves
-// convert each 64-token tile to fp16 once, into LDS, while the tile before is
-// worked on; a lane half's tokens of a slice lie together there, so that one
-// 16-byte read is an operand.
-template <int D, int TERMS>
+// 128 NC columns against one piece of their sequence's tokens, 32 NC columns
+// a wave: bound by the matrix products and, nearly as much, by the softmax's
+// exponentials and the LDS reads of the products' operands, which NC columns
+// of blocks share.  The four waves convert each 64-token tile to fp16 once,
+// into LDS, while the tile before is worked on; a lane half's tokens of a
+// slice lie together there, so that one 16-byte read is an operand.
+template <int D, int TERMS, int NC>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // units (sequence, head, piece) are dealt over a multiple of 8 workgroups,
     // and workgroups to the 8 XCDs in turn, so that one XCD's L2 serves all
@@ -822,35 +771,47 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     if (unit >= units) return;
     const uint32_t piece = unit % p.splits, h = (unit / p.splits) % p.c.heads, s = unit / p.splits / p.c.heads;
     const Sequence q = sequence_of(p.b, s);
-    const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * 128;
+    const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * (128 * NC);
     if (col0 >= cols) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 31u, hh = lane >> 5;
-    const Spans w = spans_of(p, q, col0, min(col0 + 127, cols - 1));
-    const uint32_t wcol0 = col0 + 32 * wave;
-    const bool idle = wcol0 >= cols;  // this wave has no columns; it converts all the same
-    const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 31, cols - 1));
-    const Column c = column_of(p, q, h, min(wcol0 + n, cols - 1));
-    const bool live = wcol0 + n < cols;
+    const Spans w = spans_of(p, q, col0, min(col0 + 128 * NC - 1, cols - 1));
+    const uint32_t wcol0 = col0 + 32 * NC * wave;
+    const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 32 * NC - 1, cols - 1));
+    Column c[NC];
+    bool live[NC];
+#pragma unroll
+    for (int b = 0; b < NC; ++b) {
+        c[b] = column_of(p, q, h, min(wcol0 + 32 * b + n, cols - 1));
+        live[b] = wcol0 + 32 * b + n < cols;
+    }
     const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
 
-    WideState<D> st = {};
-    st.m = ER_NO_MAX;
-    float vref = 0.0f, vinv = 0.0f;
+    WideState<D, NC> st = {};
+#pragma unroll
+    for (int b = 0; b < NC; ++b) st.m[b] = ER_NO_MAX;
+    float vref = 0.0f;
     if (begin < end) {
         WideTile<D> t;
-        WideParts now, next;
+        WideParts now, next;  // of the tile in `t`, and of the one behind it
         wide_pages(now, p, s, begin, w.anyLo, end);
         wide_pages(next, p, s, begin + 64, w.anyLo, end);
         load_wide<D>(t, now, p, h, begin, tid);
         wide_scales(now, p, h);
-        h8 qb[TERMS][D / 16];
-        const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live,
-                                                   p.scale, 8 * hh, 32, 16, qb, column_max2);
+        h8 qb[NC][TERMS][D / 16];
+        float qf[NC];
+#pragma unroll
+        for (int b = 0; b < NC; ++b)
+            qf[b] = load_query<D / 16, TERMS>(p.q + (size_t)c[b].row * p.qStride + (size_t)c[b].head * D, live[b],
+                                              p.scale, 8 * hh, 32, 16, qb[b], column_max2);
         // the sums are in units of the reference that their tiles were converted
         // with, one tile behind the conversion's
-        float unit = 0.0f;
+        float vinv = 0.0f, unitOf = 0.0f;
         bool nans = false;
-        auto convert = [&](WideLds<D> &to, int T) {
+        auto whole = [&](const WideParts &k, const Spans &w, int T) {
+            return k.page[0] >= 0 && k.page[1] >= 0 && k.page[2] >= 0 && k.page[3] >= 0 && T >= w.allLo &&
+                   T + 64 <= w.allHi;
+        };
+        auto prepare = [&](int T) {  // what the tile in `t` needs before its conversion
             float top = vref;
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = now.page[i] >= 0 ? fmaxf(top, now.vs[i]) : top;
@@ -858,58 +819,141 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                 vref = top;
                 vinv = 128.0f / top;
             }
-            const bool all = now.page[0] >= 0 && now.page[1] >= 0 && now.page[2] >= 0 && now.page[3] >= 0;
-            if (all && T >= w.allLo && T + 64 <= w.allHi)
-                store_wide<D, false>(to, t, now, vinv, T, w.anyLo, end, tid);
-            else
-                nans |= store_wide<D, true>(to, t, now, vinv, T, w.anyLo, end, tid);
+            if (!whole(now, w, T)) nans |= mask_wide<D>(t, now, T, w.anyLo, end, tid);
         };
-        convert(lds[0], begin);
+        prepare(begin);
+        store_wide<D>(lds[0], t, now, vinv, tid);
+        WideParts parts = now;
+        now = next;
+        if (begin + 64 < end) {
+            load_wide<D>(t, now, p, h, begin + 64, tid);
+            wide_scales(now, p, h);
+            wide_pages(next, p, s, begin + 128, w.anyLo, end);
+        }
         uint32_t buf = 0;
         for (int T = begin; T < end; T += 64, buf ^= 1u) {
             __syncthreads();
-            const WideParts parts = now;
-            if (vref > unit) {
-                const float f = unit / vref;
-                unit = vref;
+            if (vref > unitOf) {
+                const float f = unitOf / vref;
+                unitOf = vref;
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) st.o[d] *= f;
+                for (int b = 0; b < NC; ++b)
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d) st.o[b][d] *= f;
             }
-            const bool more = T + 64 < end;
-            if (more) {
+            if (T + 64 < end) prepare(T + 64);
+            // the scores, and between their products the next tile's
+            // conversion (behind the last tile, of what is there: nobody reads it)
+            const WideLds<D> &in = lds[buf];
+            f32x16 sc[2][NC];
+#pragma unroll
+            for (int th = 0; th < 2; ++th) {
+#pragma unroll
+                for (int b = 0; b < NC; ++b) sc[th][b] = f32x16{};
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
+#pragma unroll
+                    for (int b = 0; b < NC; ++b)
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) sc[th][b] = mfma32(a, qb[b][term][k], sc[th][b]);
+                }
+            }
+            store_wide<D>(lds[buf ^ 1u], t, now, vinv, tid);
+            float f[NC][4];
+#pragma unroll
+            for (int b = 0; b < NC; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[b][i] = score_factor(qf[b], parts.page[i] >= 0 ? parts.ks[i] : 1.0f);
+            const bool clear = whole(parts, ww, T);
+            if (!clear) {
+#pragma unroll
+                for (int b = 0; b < NC; ++b)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int tok = T + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * (int)hh + (i & 3);
+                        const bool shown = parts.page[i >> 3] >= 0 && tok >= c[b].lo && tok < c[b].hi;
+                        st.seen[b] |= shown;
+                        sc[i >> 4][b][i & 15] = shown ? sc[i >> 4][b][i & 15] : -__builtin_inff();
+                    }
+            }
+            parts = now;
+            if (T + 128 < end) {
                 now = next;
-                load_wide<D>(t, now, p, h, T + 64, tid);
+                load_wide<D>(t, now, p, h, T + 128, tid);
                 wide_scales(now, p, h);
-                wide_pages(next, p, s, T + 128, w.anyLo, end);
+                wide_pages(next, p, s, T + 192, w.anyLo, end);
             }
-            const bool all = parts.page[0] >= 0 && parts.page[1] >= 0 && parts.page[2] >= 0 && parts.page[3] >= 0;
-            if (!idle && T < ww.anyHi && T + 64 > ww.anyLo)
-                attend_wide<D, TERMS>(st, lds[buf], parts, qb, qf, all && T >= ww.allLo && T + 64 <= ww.allHi, T, c.lo,
-                                      c.hi, n, hh);
-            if (more) convert(lds[buf ^ 1u], T + 64);
+            float top[NC];
+            bool raise = false;
+#pragma unroll
+            for (int b = 0; b < NC; ++b) {
+                st.seen[b] |= clear;
+                top[b] = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float most = sc[i >> 1][b][8 * (i & 1)];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[i >> 1][b][8 * (i & 1) + j]);
+                    top[b] = fmaxf(top[b], most * f[b][i]);
+                }
+                raise |= top[b] > st.m[b] + 8.0f;
+            }
+            if (__any(raise)) {
+#pragma unroll
+                for (int b = 0; b < NC; ++b) raise_reference(fmaxf(st.m[b], column_max2(top[b])), st.m[b], st.l[b], st.o[b]);
+            }
+#pragma unroll
+            for (int sl = 0; sl < 4; ++sl) {
+                h8 wb[NC][TERMS];
+#pragma unroll
+                for (int b = 0; b < NC; ++b) {
+                    const float m7 = st.m[b] - 7.0f;
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        e[i] = __builtin_amdgcn_exp2f(sc[sl >> 1][b][8 * (sl & 1) + i] * f[b][sl] - m7);
+                    st.l[b] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                    weight_terms<TERMS>(e, wb[b]);
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const h8 a = *(const h8 *)&in.v[32 * d + n][16 * sl + 8 * hh];
+#pragma unroll
+                    for (int b = 0; b < NC; ++b)
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) st.o[b][d] = mfma32(a, wb[b][term], st.o[b][d]);
+                }
+            }
         }
-        if (__syncthreads_or(nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, hh);
+        if (__syncthreads_or(nans)) {
+#pragma unroll
+            for (int b = 0; b < NC; ++b) mark_nans<D>(st.o[b], p, s, h, begin, end, c[b].lo, c[b].hi, hh);
+        }
     }
-    const float l = column_sum2(st.l);
-    const bool seen = column_max2(st.seen ? 1.0f : 0.0f) > 0.0f;
-    if (!live) return;
     const float unitOf = vref * 0.0078125f;
-    const float f = p.splits == 1 ? unitOf / l : unitOf;
-    const size_t to = part_index(p, piece, c.row, c.head);
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int b = 0; b < NC; ++b) {
+        const float l = column_sum2(st.l[b]);
+        const bool seen = column_max2(st.seen[b] ? 1.0f : 0.0f) > 0.0f;
+        if (!live[b]) continue;
+        const float f = p.splits == 1 ? unitOf / l : unitOf;
+        const size_t to = part_index(p, piece, c[b].row, c[b].head);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t at = 32 * d + 8 * i + 4 * hh;
-            const f32x4 v = f32x4{st.o[d][4 * i], st.o[d][4 * i + 1], st.o[d][4 * i + 2], st.o[d][4 * i + 3]} * f;
-            if (p.splits == 1)
-                store4(p, c.row, c.head, at, D, seen ? v : f32x4{});
-            else if (seen)
-                *(f32x4 *)(p.partO + to * D + at) = v;
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t at = 32 * d + 8 * i + 4 * hh;
+                const f32x4 v = f32x4{st.o[b][d][4 * i], st.o[b][d][4 * i + 1], st.o[b][d][4 * i + 2], st.o[b][d][4 * i + 3]} * f;
+                if (p.splits == 1)
+                    store4(p, c[b].row, c[b].head, at, D, seen ? v : f32x4{});
+                else if (seen)
+                    *(f32x4 *)(p.partO + to * D + at) = v;
+            }
+        if (p.splits > 1 && hh == 0) {
+            p.partML[2 * to] = st.m[b];
+            p.partML[2 * to + 1] = seen ? l : -1.0f;
         }
-    if (p.splits > 1 && hh == 0) {
-        p.partML[2 * to] = st.m;
-        p.partML[2 * to + 1] = seen ? l : -1.0f;
     }
 }
 
@@ -999,23 +1043,35 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
 
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
 
-#define ER_KV8_ATTEND(D, TERMS, NAME, NARROW, WAVES)                                                               \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, NARROW)                                           \
+#define ER_KV8_NARROW(D, TERMS, NAME, WAVES)                                                                       \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
         er_kv8_attend_narrow_d##D##_##NAME(ErAttendArgs p) {                                                       \
         __shared__ __attribute__((aligned(16))) float sums[64 * (D + 4) + 128];                                    \
         kv8_attend_narrow<D, TERMS>(p, sums);                                                                      \
-    }                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        er_kv8_attend_wide_d##D##_##NAME(ErAttendArgs p) {                                                         \
-        __shared__ WideLds<D> tiles[2];                                                                            \
-        kv8_attend_wide<D, TERMS>(p, tiles);                                                             \
     }
-ER_KV8_ATTEND(64, 1, bf16, 2, 2)
-ER_KV8_ATTEND(64, 2, f32, 2, 2)
-ER_KV8_ATTEND(128, 1, bf16, 2, 2)
-ER_KV8_ATTEND(128, 2, f32, 2, 1)
-ER_KV8_ATTEND(256, 1, bf16, 1, 1)
-ER_KV8_ATTEND(256, 2, f32, 1, 1)
+ER_KV8_NARROW(64, 1, bf16, 2)
+ER_KV8_NARROW(64, 2, f32, 2)
+ER_KV8_NARROW(128, 1, bf16, 2)
+ER_KV8_NARROW(128, 2, f32, 2)
+ER_KV8_NARROW(256, 1, bf16, 1)
+ER_KV8_NARROW(256, 2, f32, 1)
+
+#define ER_KV8_WIDE(D, TERMS, NAME, NC, WAVES)                                                                     \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
+        er_kv8_attend_wide##NC##_d##D##_##NAME(ErAttendArgs p) {                                                   \
+        __shared__ WideLds<D> tiles[2];                                                                            \
+        kv8_attend_wide<D, TERMS, NC>(p, tiles);                                                                   \
+    }
+ER_KV8_WIDE(64, 1, bf16, 1, 2)
+ER_KV8_WIDE(64, 2, f32, 1, 2)
+ER_KV8_WIDE(64, 1, bf16, 2, 1)
+ER_KV8_WIDE(64, 2, f32, 2, 1)
+ER_KV8_WIDE(128, 1, bf16, 1, 2)
+ER_KV8_WIDE(128, 2, f32, 1, 1)
+ER_KV8_WIDE(128, 1, bf16, 2, 1)
+ER_KV8_WIDE(128, 2, f32, 2, 1)
+ER_KV8_WIDE(256, 1, bf16, 1, 1)
+ER_KV8_WIDE(256, 2, f32, 1, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_d##D(ErAttendArgs p) {                \

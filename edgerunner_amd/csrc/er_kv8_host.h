@@ -13,7 +13,8 @@ constexpr int kKv8Dims = 3;  // head widths 64, 128, 256
 struct Kv8Kernels {
     hipModule_t module = nullptr;
     hipFunction_t rope[kKv8Dims] = {}, append[kKv8Dims] = {}, join[kKv8Dims] = {};
-    hipFunction_t narrow[kKv8Dims][2] = {}, wide[kKv8Dims][2] = {};  // [fp32, bf16 output]
+    hipFunction_t narrow[kKv8Dims][2] = {};   // [fp32, bf16 output]
+    hipFunction_t wide[2][kKv8Dims][2] = {};  // [128, 256 columns a workgroup]; no 256 at head width 256
 };
 
 // Loads the cache's code object on the current device and resolves its kernels.
