@@ -623,7 +623,7 @@ ER_DEV void wide_scales(WideParts &w, const ErAttendArgs &p, uint32_t h) {
         w.vs[i] = load_shared(p.c.vs + block);
     }
 }
-// v[i] for an index that differs between lanes, without an address (which would put v into scratch memory)
+// v[i], without an address (which would put v into scratch memory)
 template <typename T>
 ER_DEV T pick4(const T (&v)[4], uint32_t i) {
     const T a = v[0], b = v[1], c = v[2], d = v[3];
@@ -639,11 +639,12 @@ struct ValueItem {
     int first;
 };
 template <int D>
-ER_DEV ValueItem value_item(uint32_t it) {
+ER_DEV ValueItem value_item(uint32_t tid, uint32_t r) {
+    const uint32_t it = (tid + ER_KV8_THREADS * r) & (2 * D - 1);  // D = 64: half the threads repeat
     ValueItem v;
     v.slot = it / (D / 4);
     v.dword = it % (D / 4);
-    v.part = v.slot >> 1;
+    v.part = D >= 128 ? uniform(v.slot >> 1) : v.slot >> 1;  // from width 128 on the same for the wave
     v.first = (int)(16 * v.part + 4 * (v.slot & 1));
     return v;
 }
@@ -652,19 +653,22 @@ template <int D>
 ER_DEV void load_wide(WideTile<D> &t, const WideParts &w, const ErAttendArgs &p, uint32_t h, int T, uint32_t tid) {
     const uint32_t mask = (1u << p.c.shift) - 1u;
     {
-        const uint32_t tok = tid >> 2;
-        const size_t block = (size_t)(uint32_t)max(pick4(w.page, tok >> 4), 0) * p.c.heads + h;
-        const uint8_t *src = p.c.k + ((block << p.c.shift) + (((uint32_t)T + tok) & mask)) * D + (tid & 3u) * (D / 4);
+        // a wave's 16 tokens are one part; the part's start is the same for the wave
+        const uint32_t part = uniform(tid >> 6);
+        const size_t block = (size_t)(uint32_t)max(pick4(w.page, part), 0) * p.c.heads + h;
+        const uint8_t *src = p.c.k + ((block << p.c.shift) + (((uint32_t)T + 16 * part) & mask)) * D;
+        const uint32_t at = ((tid & 63u) >> 2) * D + (tid & 3u) * (D / 4);
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) t.k[j] = *(const u32x4 *)(src + 16 * j);
+        for (int j = 0; j < D / 64; ++j) t.k[j] = *(const u32x4 *)(src + at + 16 * j);
     }
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
-        const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));  // D = 64: half the threads repeat
+        const ValueItem it = value_item<D>(tid, r);
         const size_t block = (size_t)(uint32_t)max(pick4(w.page, it.part), 0) * p.c.heads + h;
-        const uint8_t *src = p.c.v + ((block << p.c.shift) + (((uint32_t)T + (uint32_t)it.first) & mask)) * D + 4 * it.dword;
+        const uint8_t *src = p.c.v + ((block << p.c.shift) + (((uint32_t)T + 16 * it.part) & mask)) * D;
+        const uint32_t at = 4 * (it.slot & 1) * D + 4 * it.dword;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t.v[r][i] = *(const uint32_t *)(src + ((i & 3) + 8 * (i >> 2)) * D);
+        for (int i = 0; i < 8; ++i) t.v[r][i] = *(const uint32_t *)(src + at + ((i & 3) + 8 * (i >> 2)) * D);
     }
 }
 
@@ -683,7 +687,7 @@ ER_DEV bool mask_wide(WideTile<D> &t, const WideParts &w, int T, int lo, int hi,
     bool nan = false;
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
-        const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));
+        const ValueItem it = value_item<D>(tid, r);
         const bool ok = pick4(w.page, it.part) >= 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -707,7 +711,7 @@ ER_DEV void store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w,
     }
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
-        const ValueItem it = value_item<D>((tid + 256 * r) & (2 * D - 1));
+        const ValueItem it = value_item<D>(tid, r);
         // a missing page's values are zeros: any finite scale does
         const float f = pick4(w.page, it.part) >= 0 ? pick4(w.vs, it.part) * vinv : 1.0f;
         h8 a[4];
@@ -812,12 +816,13 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                    T + 64 <= w.allHi;
         };
         auto prepare = [&](int T) {  // what the tile in `t` needs before its conversion
-            float top = vref;
+            // positive floats order as their bits, which scalar registers compare
+            uint32_t top = __float_as_uint(vref);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = now.page[i] >= 0 ? fmaxf(top, now.vs[i]) : top;
-            if (top > vref) {
-                vref = top;
-                vinv = 128.0f / top;
+            for (int i = 0; i < 4; ++i) top = now.page[i] >= 0 ? max(top, __float_as_uint(now.vs[i])) : top;
+            if (top > __float_as_uint(vref)) {
+                vref = __uint_as_float(top);
+                vinv = 128.0f / vref;
             }
             if (!whole(now, w, T)) nans |= mask_wide<D>(t, now, T, w.anyLo, end, tid);
         };
@@ -833,7 +838,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
         uint32_t buf = 0;
         for (int T = begin; T < end; T += 64, buf ^= 1u) {
             __syncthreads();
-            if (vref > unitOf) {
+            if (__float_as_uint(vref) > __float_as_uint(unitOf)) {
                 const float f = unitOf / vref;
                 unitOf = vref;
 #pragma unroll
@@ -845,20 +850,17 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
             // the scores, and between their products the next tile's
             // conversion (behind the last tile, of what is there: nobody reads it)
             const WideLds<D> &in = lds[buf];
-            f32x16 sc[2][NC];
+            f32x16 sc[2][NC] = {};
 #pragma unroll
-            for (int th = 0; th < 2; ++th) {
+            for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-                for (int b = 0; b < NC; ++b) sc[th][b] = f32x16{};
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
+                for (int th = 0; th < 2; ++th) {
                     const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
 #pragma unroll
                     for (int b = 0; b < NC; ++b)
 #pragma unroll
                         for (int term = 0; term < TERMS; ++term) sc[th][b] = mfma32(a, qb[b][term][k], sc[th][b]);
                 }
-            }
             store_wide<D>(lds[buf ^ 1u], t, now, vinv, tid);
             float f[NC][4];
 #pragma unroll
