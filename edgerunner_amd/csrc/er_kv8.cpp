@@ -30,17 +30,17 @@ er_status kv8_load(Kv8Kernels &k) {
     er_status st = ER_OK;
     for (int d = 0; d < kKv8Dims && st == ER_OK; ++d) {
         char name[64];
-        auto named = [&](const char *form, const char *out) {
-            std::snprintf(name, sizeof(name), form, dims[d], out);
+        auto named = [&](const char *form, int page, const char *out) {
+            std::snprintf(name, sizeof(name), form, dims[d], page, out);
             return name;
         };
-        st = find(k.rope[d], named("er_qk_norm_rope_d%d", ""));
-        if (st == ER_OK) st = find(k.append[d], named("er_kv8_append_d%d", ""));
-        if (st == ER_OK) st = find(k.join[d], named("er_kv8_join_d%d", ""));
-        for (int o = 0; o < 2 && st == ER_OK; ++o) {
-            st = find(k.narrow[d][o], named("er_kv8_attend_narrow_d%d_%s", outs[o]));
-            if (st == ER_OK) st = find(k.wide[0][d][o], named("er_kv8_attend_wide1_d%d_%s", outs[o]));
-            if (st == ER_OK && dims[d] < 256) st = find(k.wide[1][d][o], named("er_kv8_attend_wide2_d%d_%s", outs[o]));
+        st = find(k.rope[d], named("er_qk_norm_rope_d%d", 0, ""));
+        if (st == ER_OK) st = find(k.append[d], named("er_kv8_append_d%d", 0, ""));
+        if (st == ER_OK) st = find(k.join[d], named("er_kv8_join_d%d", 0, ""));
+        for (int i = 0; i < kKv8Pages * 2 && st == ER_OK; ++i) {
+            const int page = i / 2, out = i % 2;
+            st = find(k.narrow[d][page][out], named("er_kv8_attend_narrow_d%d_p%d_%s", 16 << page, outs[out]));
+            if (st == ER_OK) st = find(k.wide[d][page][out], named("er_kv8_attend_wide_d%d_p%d_%s", 16 << page, outs[out]));
         }
     }
     if (st != ER_OK) kv8_unload(k);
@@ -216,8 +216,7 @@ uint32_t row_chunks(uint32_t strips, uint32_t rows, int cu) {
 struct AttendPlan {
     bool narrow;
     uint32_t shares, least;         // narrow kernel
-    uint32_t blocks;                // wide kernel: 32-column blocks a wave
-    uint32_t tiles, splits, chunk;
+    uint32_t tiles, splits, chunk;  // wide kernel
     uint64_t parts;                 // columns that the workspace holds sums of, at the most over all windows
 };
 
@@ -242,15 +241,13 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
         }
         return p;
     }
-    p.blocks = 1;
-    const uint32_t tileCols = 128 * p.blocks;
-    p.tiles = (uint32_t)((cols + tileCols - 1) / tileCols);
+    p.tiles = (uint32_t)((cols + 127) / 128);
     uint64_t span = full;
     // the tile's rows see window + rows - 1 tokens, and pieces begin at a multiple of 64
-    if (window) span = std::min<uint64_t>(span, (uint64_t)window + tileCols / group + 2 + 63);
+    if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
     // the tokens of a (sequence, head, row tile) are cut into pieces where
     // those alone are too few workgroups
-    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * (p.blocks == 2 ? 1 : 2), least = 512;
+    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 2, least = 512;
     auto pieces = [&](uint64_t tokens) {
         return std::max<uint64_t>(1, std::min<uint64_t>((want + units - 1) / units, (tokens + least - 1) / least));
     };
@@ -429,9 +426,9 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     const int di = dim_index(d);
     const uint64_t pairs = (uint64_t)batch->sequences * cache->kv_heads;
     if (p.narrow)
-        st = launch(kernels.narrow[di][a.half], op, p.shares ? p.shares : pairs, 0, stream, &a);
+        st = launch(kernels.narrow[di][a.c.shift - 4][a.half], op, p.shares ? p.shares : pairs, 0, stream, &a);
     else
-        st = launch(kernels.wide[p.blocks - 1][di][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
+        st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
     const uint32_t most = p.shares ? p.shares : p.splits;
     return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (4 * ER_KV8_THREADS + most) * 4, stream, &a);

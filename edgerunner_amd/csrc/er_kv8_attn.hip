@@ -171,27 +171,31 @@ struct NarrowTile {
 struct NarrowPages {
     int page[2];
 };
+template <int P>
 ER_DEV NarrowPages narrow_pages(const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
     NarrowPages w;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int at = T + 16 * half;
-        w.page[half] = at < hi && at + 16 > lo ? uniform(page_of(p.b, p.c, s, at)) : -1;
-    }
+    constexpr int AT = P < 32 ? 16 : 32;  // tokens that one entry covers
+    auto page = [&](int at) { return at < hi && at + AT > lo ? uniform(page_of(p.b, p.c, s, at)) : -1; };
+    w.page[0] = page(T);
+    w.page[1] = P < 32 ? page(T + 16) : w.page[0];
     return w;
 }
 
-template <int D>
+template <int D, int P>
 ER_DEV void load_narrow(NarrowTile<D> &t, const NarrowPages &w, const ErAttendArgs &p, uint32_t h, int T, uint32_t n,
                         uint32_t g) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         t.page[half] = w.page[half];
         const size_t block = (size_t)(uint32_t)max(w.page[half], 0) * p.c.heads + h;
-        t.ks[half] = load_shared(p.c.ks + block);
-        t.vs[half] = load_shared(p.c.vs + block);
-        const uint32_t inside = (uint32_t)(T + 16 * half) & ((1u << p.c.shift) - 1u);
-        const size_t base = ((block << p.c.shift) + inside) * D;
+        if (half == 0 || P < 32) {
+            t.ks[half] = load_shared(p.c.ks + block);
+            t.vs[half] = load_shared(p.c.vs + block);
+        } else {
+            t.ks[1] = t.ks[0];
+            t.vs[1] = t.vs[0];
+        }
+        const size_t base = block * (P * D) + ((uint32_t)(T + 16 * half) % P) * D;
         const uint8_t *kp = p.c.k + base + (n * D + 16 * g);
         const uint8_t *vp = p.c.v + base + (4 * g * D + n * (D / 16));
 #pragma unroll
@@ -454,7 +458,7 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bo
 // works; keys and values need no exchange between lanes, so nothing passes
 // through LDS until the waves' sums are joined at the end.  The sums of all
 // steps are the columns' outputs; else they go to part `part`.
-template <int D, int TERMS>
+template <int D, int P, int TERMS>
 ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t from, uint32_t to,
                         bool complete, uint32_t part, float *lds) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
@@ -473,7 +477,7 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     int rest = end;  // the first tile that is not whole
     auto next_whole = [&](int T) {  // the wave's next whole tile from T on, its pages in `pages`; `end` if there is none
         for (; T < end; T += 128) {
-            pages = narrow_pages(p, s, T, w.anyLo, end);
+            pages = narrow_pages<P>(p, s, T, w.anyLo, end);
             if (whole(pages, T)) return T;
             rest = min(rest, T);
         }
@@ -481,7 +485,7 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     };
     NarrowTile<D> t0, t1;
     int T = next_whole(begin + 32 * (int)wave);
-    if (T < end) load_narrow<D>(t0, pages, p, h, T, n, g);
+    if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
     int U = next_whole(T + 128);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
@@ -489,18 +493,18 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     NarrowState<D> st = {};
     st.m = ER_NO_MAX;
     while (T < end) {
-        if (U < end) load_narrow<D>(t1, pages, p, h, U, n, g);
+        if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
         T = next_whole(U + 128);
         attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
         if (U >= end) break;
-        if (T < end) load_narrow<D>(t0, pages, p, h, T, n, g);
+        if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
         U = next_whole(T + 128);
         attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
     }
     for (T = rest; T < end; T += 128) {
-        pages = narrow_pages(p, s, T, w.anyLo, end);
+        pages = narrow_pages<P>(p, s, T, w.anyLo, end);
         if (whole(pages, T) || (pages.page[0] < 0 && pages.page[1] < 0)) continue;
-        load_narrow<D>(t0, pages, p, h, T, n, g);
+        load_narrow<D, P>(t0, pages, p, h, T, n, g);
         attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g);
     }
     // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
@@ -556,13 +560,13 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     }
 }
 
-template <int D, int TERMS>
+template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
     if (p.shares == 0) {
         const uint32_t s = blockIdx.x / H, h = blockIdx.x % H;
         const LaneSequence l = lane_sequence(p, s);
-        if (l.steps) narrow_unit<D, TERMS>(p, s, l.q, h, 0, l.steps, true, 0, lds);
+        if (l.steps) narrow_unit<D, P, TERMS>(p, s, l.q, h, 0, l.steps, true, 0, lds);
         return;
     }
     const LaneSequence first = lane_sequence(p, lane);
@@ -578,7 +582,7 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
         // a unit that begins here and goes on in later workgroups leaves its
         // sums in this one's second part, one that began earlier in its first
         const uint32_t from = at - begins, to = min(last - begins, l.steps);
-        narrow_unit<D, TERMS>(p, s, l.q, h, from, to, from == 0 && to == l.steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u),
+        narrow_unit<D, P, TERMS>(p, s, l.q, h, from, to, from == 0 && to == l.steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u),
                               lds);
         begins += length;
         at = begins;
@@ -597,38 +601,56 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
 
 #define ER_WIDE_TOKENS 64
 
-// What a tile's four 16-token parts bring: page, scales.
-struct WideParts {
-    int page[4];
-    float ks[4], vs[4];
+// What a tile's pages bring: 64 / P of them.
+template <int P>
+struct WidePages {
+    static constexpr int N = ER_WIDE_TOKENS / P;
+    int page[N];
+    float ks[N], vs[N];
+    // all of the tile is there
+    __device__ __forceinline__ bool all() const {
+        bool r = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r &= page[i] >= 0;
+        return r;
+    }
 };
-template <int D>
+template <int D, int P>
 struct WideTile {
     u32x4 k[D / 64];                       // token tid / 4, bytes [(tid & 3) D/4, + D/4)
     uint32_t v[(D + 127) / 128][8];        // see value_item
 };
 
-ER_DEV void wide_pages(WideParts &w, const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
+template <int P>
+ER_DEV void wide_pages(WidePages<P> &w, const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = T + 16 * i;
-        w.page[i] = at < hi && at + 16 > lo ? uniform(page_of(p.b, p.c, s, at)) : -1;
+    for (int i = 0; i < w.N; ++i) {
+        const int at = T + P * i;
+        w.page[i] = at < hi && at + P > lo ? uniform(page_of(p.b, p.c, s, at)) : -1;
     }
 }
-ER_DEV void wide_scales(WideParts &w, const ErAttendArgs &p, uint32_t h) {
+template <int P>
+ER_DEV void wide_scales(WidePages<P> &w, const ErAttendArgs &p, uint32_t h) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < w.N; ++i) {
         const size_t block = (size_t)(uint32_t)max(w.page[i], 0) * p.c.heads + h;
         w.ks[i] = load_shared(p.c.ks + block);
         w.vs[i] = load_shared(p.c.vs + block);
     }
 }
-// v[i], without an address (which would put v into scratch memory)
-template <typename T>
-ER_DEV T pick4(const T (&v)[4], uint32_t i) {
-    const T a = v[0], b = v[1], c = v[2], d = v[3];
-    const T x = i & 1u ? b : a, y = i & 1u ? d : c;
-    return i & 2u ? y : x;
+// Entry of a tile's 16-token part, without an address (which would put v into scratch memory).
+template <int N>
+ER_DEV int of_part(const int (&v)[N], uint32_t part) {
+    if constexpr (N == 1) {
+        return v[0];
+    } else if constexpr (N == 2) {
+        const int a = v[0], b = v[1];
+        return part & 2u ? b : a;
+    } else {
+        const int a = v[0], b = v[1], c = v[2], d = v[3];
+        const int x = part & 1u ? b : a, y = part & 1u ? d : c;
+        return part & 2u ? y : x;
+    }
 }
 
 // Item `it` of a tile's values: four codes (dword) of the eight tokens (first
@@ -649,14 +671,13 @@ ER_DEV ValueItem value_item(uint32_t tid, uint32_t r) {
     return v;
 }
 
-template <int D>
-ER_DEV void load_wide(WideTile<D> &t, const WideParts &w, const ErAttendArgs &p, uint32_t h, int T, uint32_t tid) {
-    const uint32_t mask = (1u << p.c.shift) - 1u;
+template <int D, int P>
+ER_DEV void load_wide(WideTile<D, P> &t, const WidePages<P> &w, const ErAttendArgs &p, uint32_t h, uint32_t tid) {
     {
         // a wave's 16 tokens are one part; the part's start is the same for the wave
         const uint32_t part = uniform(tid >> 6);
-        const size_t block = (size_t)(uint32_t)max(pick4(w.page, part), 0) * p.c.heads + h;
-        const uint8_t *src = p.c.k + ((block << p.c.shift) + (((uint32_t)T + 16 * part) & mask)) * D;
+        const size_t block = (size_t)(uint32_t)max(of_part(w.page, part), 0) * p.c.heads + h;
+        const uint8_t *src = p.c.k + block * (P * D) + (16 * part % P) * D;
         const uint32_t at = ((tid & 63u) >> 2) * D + (tid & 3u) * (D / 4);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) t.k[j] = *(const u32x4 *)(src + at + 16 * j);
@@ -664,31 +685,33 @@ ER_DEV void load_wide(WideTile<D> &t, const WideParts &w, const ErAttendArgs &p,
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>(tid, r);
-        const size_t block = (size_t)(uint32_t)max(pick4(w.page, it.part), 0) * p.c.heads + h;
-        const uint8_t *src = p.c.v + ((block << p.c.shift) + (((uint32_t)T + 16 * it.part) & mask)) * D;
+        const size_t block = (size_t)(uint32_t)max(of_part(w.page, it.part), 0) * p.c.heads + h;
+        const uint8_t *src = p.c.v + block * (P * D) + (16 * it.part % P) * D;
         const uint32_t at = 4 * (it.slot & 1) * D + 4 * it.dword;
 #pragma unroll
         for (int i = 0; i < 8; ++i) t.v[r][i] = *(const uint32_t *)(src + at + ((i & 3) + 8 * (i >> 2)) * D);
     }
 }
 
-// LDS: keys [64][D + 8], values transposed [D][64 + 8], both fp16.  The
-// pitches put consecutive rows 4 banks apart.
+// A tile's codes in LDS: keys by token, values by element with the tokens of
+// lane half hh's slice sl at bytes 32 hh + 8 sl, so that one 16-byte read holds
+// the codes of two operands.  The pitches put consecutive rows 4 and 20 banks
+// apart, which spreads 16 of them over all 64.
 template <int D>
 struct WideLds {
-    _Float16 k[ER_WIDE_TOKENS][D + 8];
-    _Float16 v[D][ER_WIDE_TOKENS + 8];
+    uint8_t k[ER_WIDE_TOKENS][D + 16];
+    uint8_t v[D][ER_WIDE_TOKENS + 16];
 };
 
 // The values of a tile that some column of the workgroup does not see whole,
 // as attend_narrow's masked tiles; true where there were NaN codes.
-template <int D>
-ER_DEV bool mask_wide(WideTile<D> &t, const WideParts &w, int T, int lo, int hi, uint32_t tid) {
+template <int D, int P>
+ER_DEV bool mask_wide(WideTile<D, P> &t, const WidePages<P> &w, int T, int lo, int hi, uint32_t tid) {
     bool nan = false;
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>(tid, r);
-        const bool ok = pick4(w.page, it.part) >= 0;
+        const bool ok = of_part(w.page, it.part) >= 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
@@ -700,24 +723,24 @@ ER_DEV bool mask_wide(WideTile<D> &t, const WideParts &w, int T, int lo, int hi,
     return nan;
 }
 
-// A tile into LDS as fp16, values in units of the reference scale.
-template <int D>
-ER_DEV void store_wide(WideLds<D> &to, const WideTile<D> &t, const WideParts &w, float vinv, uint32_t tid) {
-    _Float16 *dst = &to.k[tid >> 2][(tid & 3u) * (D / 4)];
+// A tile into LDS.
+template <int D, int P>
+ER_DEV void store_wide(WideLds<D> &to, const WideTile<D, P> &t, uint32_t tid) {
+    uint8_t *dst = &to.k[tid >> 2][(tid & 3u) * (D / 4)];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-        *(h8 *)(dst + 16 * j) = codes_to_h8(t.k[j].x, t.k[j].y);
-        *(h8 *)(dst + 16 * j + 8) = codes_to_h8(t.k[j].z, t.k[j].w);
-    }
+    for (int j = 0; j < D / 64; ++j) *(u32x4 *)(dst + 16 * j) = t.k[j];
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>(tid, r);
-        // a missing page's values are zeros: any finite scale does
-        const float f = pick4(w.page, it.part) >= 0 ? pick4(w.vs, it.part) * vinv : 1.0f;
-        h8 a[4];
-        transpose_codes(t.v[r], f, f, a);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *(h8 *)&to.v[4 * it.dword + j][8 * it.slot] = a[j];
+        const uint32_t *x = t.v[r];
+        const uint32_t a0 = zip_lo(x[0], x[1]), a1 = zip_hi(x[0], x[1]), b0 = zip_lo(x[2], x[3]), b1 = zip_hi(x[2], x[3]);
+        const uint32_t c0 = zip_lo(x[4], x[5]), c1 = zip_hi(x[4], x[5]), d0 = zip_lo(x[6], x[7]), d1 = zip_hi(x[6], x[7]);
+        uint8_t *v = &to.v[4 * it.dword][32 * (it.slot & 1) + 8 * it.part];
+        constexpr uint32_t PITCH = ER_WIDE_TOKENS + 16, LOW = 0x05040100u, HIGH = 0x07060302u;
+        *(u32x2 *)v = u32x2{__builtin_amdgcn_perm(b0, a0, LOW), __builtin_amdgcn_perm(d0, c0, LOW)};
+        *(u32x2 *)(v + PITCH) = u32x2{__builtin_amdgcn_perm(b0, a0, HIGH), __builtin_amdgcn_perm(d0, c0, HIGH)};
+        *(u32x2 *)(v + 2 * PITCH) = u32x2{__builtin_amdgcn_perm(b1, a1, LOW), __builtin_amdgcn_perm(d1, c1, LOW)};
+        *(u32x2 *)(v + 3 * PITCH) = u32x2{__builtin_amdgcn_perm(b1, a1, HIGH), __builtin_amdgcn_perm(d1, c1, HIGH)};
     }
 }
 
@@ -729,14 +752,6 @@ ER_DEV float column_sum2(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-
-// Running state of a wave's NC x 32 columns, as NarrowState's.
-template <int D, int NC>
-struct WideState {
-    f32x16 o[NC][D / 32];  // o[c][d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n of 32-column block c
-    float m[NC], l[NC];
-    bool seen[NC];
-};
 
 // As the narrow kernel's.
 template <int D>
@@ -759,13 +774,13 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
     }
 }
 
-// 128 NC columns against one piece of their sequence's tokens, 32 NC columns
-// a wave: bound by the matrix products and, nearly as much, by the softmax's
-// exponentials and the LDS reads of the products' operands, which NC columns
-// of blocks share.  The four waves convert each 64-token tile to fp16 once,
-// into LDS, while the tile before is worked on; a lane half's tokens of a
-// slice lie together there, so that one 16-byte read is an operand.
-template <int D, int TERMS, int NC>
+// 128 columns against one piece of their sequence's tokens, 32 columns a wave:
+// bound by the matrix products and, nearly as much, by the instructions of the
+// softmax and the conversions.  The four waves copy each 64-token tile's codes
+// into LDS while the tile before is worked on, and convert them as they read
+// operands: codes are half the LDS traffic of fp16, and small enough that
+// three workgroups fit a CU at head width 128.
+template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // units (sequence, head, piece) are dealt over a multiple of 8 workgroups,
     // and workgroups to the 8 XCDs in turn, so that one XCD's L2 serves all
@@ -775,187 +790,146 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     if (unit >= units) return;
     const uint32_t piece = unit % p.splits, h = (unit / p.splits) % p.c.heads, s = unit / p.splits / p.c.heads;
     const Sequence q = sequence_of(p.b, s);
-    const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * (128 * NC);
+    const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * 128;
     if (col0 >= cols) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 31u, hh = lane >> 5;
-    const Spans w = spans_of(p, q, col0, min(col0 + 128 * NC - 1, cols - 1));
-    const uint32_t wcol0 = col0 + 32 * NC * wave;
-    const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 32 * NC - 1, cols - 1));
-    Column c[NC];
-    bool live[NC];
-#pragma unroll
-    for (int b = 0; b < NC; ++b) {
-        c[b] = column_of(p, q, h, min(wcol0 + 32 * b + n, cols - 1));
-        live[b] = wcol0 + 32 * b + n < cols;
-    }
+    const Spans w = spans_of(p, q, col0, min(col0 + 127, cols - 1));
+    const uint32_t wcol0 = col0 + 32 * wave;
+    const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 31, cols - 1));
+    const Column c = column_of(p, q, h, min(wcol0 + n, cols - 1));
+    const bool live = wcol0 + n < cols;
     const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
 
-    WideState<D, NC> st = {};
-#pragma unroll
-    for (int b = 0; b < NC; ++b) st.m[b] = ER_NO_MAX;
-    float vref = 0.0f;
+    f32x16 o[D / 32] = {};  // o[d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n, in units of vref / 128
+    float m = ER_NO_MAX, l = 0.0f, vref = 0.0f, vinv = 0.0f;
+    bool seen = false;
     if (begin < end) {
-        WideTile<D> t;
-        WideParts now, next;  // of the tile in `t`, and of the one behind it
+        WideTile<D, P> t;
+        WidePages<P> now, next;  // of the tile in `t`, and of the one behind it
         wide_pages(now, p, s, begin, w.anyLo, end);
         wide_pages(next, p, s, begin + 64, w.anyLo, end);
-        load_wide<D>(t, now, p, h, begin, tid);
+        load_wide<D, P>(t, now, p, h, tid);
         wide_scales(now, p, h);
-        h8 qb[NC][TERMS][D / 16];
-        float qf[NC];
-#pragma unroll
-        for (int b = 0; b < NC; ++b)
-            qf[b] = load_query<D / 16, TERMS>(p.q + (size_t)c[b].row * p.qStride + (size_t)c[b].head * D, live[b],
-                                              p.scale, 8 * hh, 32, 16, qb[b], column_max2);
-        // the sums are in units of the reference that their tiles were converted
-        // with, one tile behind the conversion's
-        float vinv = 0.0f, unitOf = 0.0f;
+        h8 qb[TERMS][D / 16];
+        const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live, p.scale,
+                                                   16 * hh, 32, 8, qb, column_max2);
         bool nans = false;
-        auto whole = [&](const WideParts &k, const Spans &w, int T) {
-            return k.page[0] >= 0 && k.page[1] >= 0 && k.page[2] >= 0 && k.page[3] >= 0 && T >= w.allLo &&
-                   T + 64 <= w.allHi;
+        auto whole = [&](const WidePages<P> &k, const Spans &w, int T) {
+            return k.all() && T >= w.allLo && T + 64 <= w.allHi;
         };
-        auto prepare = [&](int T) {  // what the tile in `t` needs before its conversion
-            // positive floats order as their bits, which scalar registers compare
-            uint32_t top = __float_as_uint(vref);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = now.page[i] >= 0 ? max(top, __float_as_uint(now.vs[i])) : top;
-            if (top > __float_as_uint(vref)) {
-                vref = __uint_as_float(top);
-                vinv = 128.0f / vref;
-            }
-            if (!whole(now, w, T)) nans |= mask_wide<D>(t, now, T, w.anyLo, end, tid);
-        };
-        prepare(begin);
-        store_wide<D>(lds[0], t, now, vinv, tid);
-        WideParts parts = now;
+        if (!whole(now, w, begin)) nans |= mask_wide<D, P>(t, now, begin, w.anyLo, end, tid);
+        store_wide<D, P>(lds[0], t, tid);
+        WidePages<P> parts = now;
         now = next;
         if (begin + 64 < end) {
-            load_wide<D>(t, now, p, h, begin + 64, tid);
+            load_wide<D, P>(t, now, p, h, tid);
             wide_scales(now, p, h);
             wide_pages(next, p, s, begin + 128, w.anyLo, end);
         }
         uint32_t buf = 0;
         for (int T = begin; T < end; T += 64, buf ^= 1u) {
             __syncthreads();
-            if (__float_as_uint(vref) > __float_as_uint(unitOf)) {
-                const float f = unitOf / vref;
-                unitOf = vref;
-#pragma unroll
-                for (int b = 0; b < NC; ++b)
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) st.o[b][d] *= f;
-            }
-            if (T + 64 < end) prepare(T + 64);
-            // the scores, and between their products the next tile's
-            // conversion (behind the last tile, of what is there: nobody reads it)
             const WideLds<D> &in = lds[buf];
-            f32x16 sc[2][NC] = {};
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                for (int th = 0; th < 2; ++th) {
-                    const h8 a = *(const h8 *)&in.k[32 * th + n][16 * k + 8 * hh];
-#pragma unroll
-                    for (int b = 0; b < NC; ++b)
-#pragma unroll
-                        for (int term = 0; term < TERMS; ++term) sc[th][b] = mfma32(a, qb[b][term][k], sc[th][b]);
-                }
-            store_wide<D>(lds[buf ^ 1u], t, now, vinv, tid);
-            float f[NC][4];
-#pragma unroll
-            for (int b = 0; b < NC; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[b][i] = score_factor(qf[b], parts.page[i] >= 0 ? parts.ks[i] : 1.0f);
             const bool clear = whole(parts, ww, T);
-            if (!clear) {
+            seen |= clear;
+            // the value scales' reference; positive floats order as their bits, which scalar registers compare
+            uint32_t most = __float_as_uint(vref);
 #pragma unroll
-                for (int b = 0; b < NC; ++b)
+            for (int i = 0; i < parts.N; ++i)
+                most = parts.page[i] >= 0 ? max(most, __float_as_uint(parts.vs[i])) : most;
+            if (most > __float_as_uint(vref)) raise_scale(__uint_as_float(most), vref, vinv, o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int tok = T + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * (int)hh + (i & 3);
-                        const bool shown = parts.page[i >> 3] >= 0 && tok >= c[b].lo && tok < c[b].hi;
-                        st.seen[b] |= shown;
-                        sc[i >> 4][b][i & 15] = shown ? sc[i >> 4][b][i & 15] : -__builtin_inff();
+            for (int th = 0; th < 2; ++th) {
+                f32x16 sc = {};
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const u32x4 k = *(const u32x4 *)&in.k[32 * th + n][32 * j + 16 * hh];
+                    const h8 a0 = codes_to_h8(k.x, k.y), a1 = codes_to_h8(k.z, k.w);
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        sc = mfma32(a0, qb[term][2 * j], sc);
+                        sc = mfma32(a1, qb[term][2 * j + 1], sc);
                     }
+                }
+                if (th == 1 && T + 64 < end) {
+                    if (!whole(now, w, T + 64)) nans |= mask_wide<D, P>(t, now, T + 64, w.anyLo, end, tid);
+                    store_wide<D, P>(lds[buf ^ 1u], t, tid);
+                }
+                if (!clear) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int tok = T + 32 * th + 8 * (i >> 2) + 4 * (int)hh + (i & 3);
+                        const bool shown = parts.page[(32 * th + 16 * (i >> 3)) / P] >= 0 && tok >= c.lo && tok < c.hi;
+                        seen |= shown;
+                        sc[i] = shown ? sc[i] : -__builtin_inff();
+                    }
+                }
+                float f[2], v[2], top = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = (32 * th + 16 * i) / P;
+                    const bool there = parts.page[e] >= 0;  // a missing page's values are zeros: any finite scale does
+                    f[i] = score_factor(qf, there ? parts.ks[e] : 1.0f);
+                    v[i] = there ? parts.vs[e] * vinv : 1.0f;
+                    float peak = sc[8 * i];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) peak = fmaxf(peak, sc[8 * i + j]);
+                    top = fmaxf(top, peak * f[i]);
+                }
+                if (__any(top > m + 8.0f)) raise_reference(fmaxf(m, column_max2(top)), m, l, o);
+                const float m7 = m - 7.0f;
+                h8 wb[2][TERMS];
+#pragma unroll
+                for (int sl = 0; sl < 2; ++sl) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(sc[8 * sl + i] * f[sl] - m7);
+                    l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                    weight_terms<TERMS>(e, wb[sl]);
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const u32x4 x = *(const u32x4 *)&in.v[32 * d + n][32 * hh + 16 * th];
+                    const h8 a0 = join(codes_to_h2<false>(x.x, v[0]), codes_to_h2<true>(x.x, v[0]),
+                                       codes_to_h2<false>(x.y, v[0]), codes_to_h2<true>(x.y, v[0]));
+                    const h8 a1 = join(codes_to_h2<false>(x.z, v[1]), codes_to_h2<true>(x.z, v[1]),
+                                       codes_to_h2<false>(x.w, v[1]), codes_to_h2<true>(x.w, v[1]));
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) {
+                        o[d] = mfma32(a0, wb[0][term], o[d]);
+                        o[d] = mfma32(a1, wb[1][term], o[d]);
+                    }
+                }
             }
             parts = now;
             if (T + 128 < end) {
                 now = next;
-                load_wide<D>(t, now, p, h, T + 128, tid);
+                load_wide<D, P>(t, now, p, h, tid);
                 wide_scales(now, p, h);
                 wide_pages(next, p, s, T + 192, w.anyLo, end);
             }
-            float top[NC];
-            bool raise = false;
-#pragma unroll
-            for (int b = 0; b < NC; ++b) {
-                st.seen[b] |= clear;
-                top[b] = -__builtin_inff();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float most = sc[i >> 1][b][8 * (i & 1)];
-#pragma unroll
-                    for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[i >> 1][b][8 * (i & 1) + j]);
-                    top[b] = fmaxf(top[b], most * f[b][i]);
-                }
-                raise |= top[b] > st.m[b] + 8.0f;
-            }
-            if (__any(raise)) {
-#pragma unroll
-                for (int b = 0; b < NC; ++b) raise_reference(fmaxf(st.m[b], column_max2(top[b])), st.m[b], st.l[b], st.o[b]);
-            }
-#pragma unroll
-            for (int sl = 0; sl < 4; ++sl) {
-                h8 wb[NC][TERMS];
-#pragma unroll
-                for (int b = 0; b < NC; ++b) {
-                    const float m7 = st.m[b] - 7.0f;
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        e[i] = __builtin_amdgcn_exp2f(sc[sl >> 1][b][8 * (sl & 1) + i] * f[b][sl] - m7);
-                    st.l[b] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                    weight_terms<TERMS>(e, wb[b]);
-                }
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    const h8 a = *(const h8 *)&in.v[32 * d + n][16 * sl + 8 * hh];
-#pragma unroll
-                    for (int b = 0; b < NC; ++b)
-#pragma unroll
-                        for (int term = 0; term < TERMS; ++term) st.o[b][d] = mfma32(a, wb[b][term], st.o[b][d]);
-                }
-            }
         }
-        if (__syncthreads_or(nans)) {
-#pragma unroll
-            for (int b = 0; b < NC; ++b) mark_nans<D>(st.o[b], p, s, h, begin, end, c[b].lo, c[b].hi, hh);
-        }
+        if (__syncthreads_or(nans)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);
     }
-    const float unitOf = vref * 0.0078125f;
+    l = column_sum2(l);
+    seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f;
+    if (!live) return;
+    const float f = p.splits == 1 ? vref * 0.0078125f / l : vref * 0.0078125f;
+    const size_t to = part_index(p, piece, c.row, c.head);
 #pragma unroll
-    for (int b = 0; b < NC; ++b) {
-        const float l = column_sum2(st.l[b]);
-        const bool seen = column_max2(st.seen[b] ? 1.0f : 0.0f) > 0.0f;
-        if (!live[b]) continue;
-        const float f = p.splits == 1 ? unitOf / l : unitOf;
-        const size_t to = part_index(p, piece, c[b].row, c[b].head);
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t at = 32 * d + 8 * i + 4 * hh;
-                const f32x4 v = f32x4{st.o[b][d][4 * i], st.o[b][d][4 * i + 1], st.o[b][d][4 * i + 2], st.o[b][d][4 * i + 3]} * f;
-                if (p.splits == 1)
-                    store4(p, c[b].row, c[b].head, at, D, seen ? v : f32x4{});
-                else if (seen)
-                    *(f32x4 *)(p.partO + to * D + at) = v;
-            }
-        if (p.splits > 1 && hh == 0) {
-            p.partML[2 * to] = st.m[b];
-            p.partML[2 * to + 1] = seen ? l : -1.0f;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t at = 32 * d + 8 * i + 4 * hh;
+            const f32x4 v = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * f;
+            if (p.splits == 1)
+                store4(p, c.row, c.head, at, D, seen ? v : f32x4{});
+            else if (seen)
+                *(f32x4 *)(p.partO + to * D + at) = v;
         }
+    if (p.splits > 1 && hh == 0) {
+        p.partML[2 * to] = m;
+        p.partML[2 * to + 1] = seen ? l : -1.0f;
     }
 }
 
@@ -1045,35 +1019,30 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
 
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
 
-#define ER_KV8_NARROW(D, TERMS, NAME, WAVES)                                                                       \
+// One kernel for each head width, page size and output type.  WAVES: waves a
+// SIMD that the registers leave room for.
+#define ER_KV8_NARROW(D, P, TERMS, NAME, WAVES)                                                                    \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        er_kv8_attend_narrow_d##D##_##NAME(ErAttendArgs p) {                                                       \
+        er_kv8_attend_narrow_d##D##_p##P##_##NAME(ErAttendArgs p) {                                                \
         __shared__ __attribute__((aligned(16))) float sums[64 * (D + 4) + 128];                                    \
-        kv8_attend_narrow<D, TERMS>(p, sums);                                                                      \
+        kv8_attend_narrow<D, P, TERMS>(p, sums);                                                                   \
     }
-ER_KV8_NARROW(64, 1, bf16, 2)
-ER_KV8_NARROW(64, 2, f32, 2)
-ER_KV8_NARROW(128, 1, bf16, 2)
-ER_KV8_NARROW(128, 2, f32, 2)
-ER_KV8_NARROW(256, 1, bf16, 1)
-ER_KV8_NARROW(256, 2, f32, 1)
-
-#define ER_KV8_WIDE(D, TERMS, NAME, NC, WAVES)                                                                     \
+#define ER_KV8_WIDE(D, P, TERMS, NAME, WAVES)                                                                      \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        er_kv8_attend_wide##NC##_d##D##_##NAME(ErAttendArgs p) {                                                   \
-        __shared__ WideLds<D> tiles[2];                                                                            \
-        kv8_attend_wide<D, TERMS, NC>(p, tiles);                                                                   \
+        er_kv8_attend_wide_d##D##_p##P##_##NAME(ErAttendArgs p) {                                                  \
+        __shared__ __attribute__((aligned(16))) WideLds<D> tiles[2];                                               \
+        kv8_attend_wide<D, P, TERMS>(p, tiles);                                                                    \
     }
-ER_KV8_WIDE(64, 1, bf16, 1, 2)
-ER_KV8_WIDE(64, 2, f32, 1, 2)
-ER_KV8_WIDE(64, 1, bf16, 2, 1)
-ER_KV8_WIDE(64, 2, f32, 2, 1)
-ER_KV8_WIDE(128, 1, bf16, 1, 2)
-ER_KV8_WIDE(128, 2, f32, 1, 1)
-ER_KV8_WIDE(128, 1, bf16, 2, 1)
-ER_KV8_WIDE(128, 2, f32, 2, 1)
-ER_KV8_WIDE(256, 1, bf16, 1, 1)
-ER_KV8_WIDE(256, 2, f32, 1, 1)
+#define ER_KV8_PAGES(D, P, NARROW, WIDE)                                                                           \
+    ER_KV8_NARROW(D, P, 1, bf16, NARROW)                                                                           \
+    ER_KV8_NARROW(D, P, 2, f32, NARROW)                                                                            \
+    ER_KV8_WIDE(D, P, 1, bf16, WIDE)                                                                               \
+    ER_KV8_WIDE(D, P, 2, f32, WIDE)
+#define ER_KV8_ATTEND(D, NARROW, WIDE)                                                                             \
+    ER_KV8_PAGES(D, 16, NARROW, WIDE) ER_KV8_PAGES(D, 32, NARROW, WIDE) ER_KV8_PAGES(D, 64, NARROW, WIDE)
+ER_KV8_ATTEND(64, 2, 3)
+ER_KV8_ATTEND(128, 2, 2)
+ER_KV8_ATTEND(256, 1, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_d##D(ErAttendArgs p) {                \

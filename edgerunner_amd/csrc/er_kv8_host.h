@@ -8,13 +8,13 @@
 
 namespace er_detail {
 
-constexpr int kKv8Dims = 3;  // head widths 64, 128, 256
+constexpr int kKv8Dims = 3;   // head widths 64, 128, 256
+constexpr int kKv8Pages = 3;  // pages of 16, 32, 64 tokens
 
 struct Kv8Kernels {
     hipModule_t module = nullptr;
     hipFunction_t rope[kKv8Dims] = {}, append[kKv8Dims] = {}, join[kKv8Dims] = {};
-    hipFunction_t narrow[kKv8Dims][2] = {};   // [fp32, bf16 output]
-    hipFunction_t wide[2][kKv8Dims][2] = {};  // [128, 256 columns a workgroup]; no 256 at head width 256
+    hipFunction_t narrow[kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};  // [fp32, bf16 output]
 };
 
 // Loads the cache's code object on the current device and resolves its kernels.
