@@ -37,6 +37,7 @@ er_status kv8_load(Kv8Kernels &k) {
         st = find(k.rope[d], named("er_qk_norm_rope_d%d", 0, ""));
         if (st == ER_OK) st = find(k.append[d], named("er_kv8_append_d%d", 0, ""));
         if (st == ER_OK) st = find(k.join[d], named("er_kv8_join_d%d", 0, ""));
+        if (st == ER_OK) st = find(k.joinRow[d], named("er_kv8_join_row_d%d", 0, ""));
         for (int i = 0; i < kKv8Pages * 2 && st == ER_OK; ++i) {
             const int page = i / 2, out = i % 2;
             st = find(k.narrow[d][page][out], named("er_kv8_attend_narrow_d%d_p%d_%s", 16 << page, outs[out]));
@@ -229,11 +230,10 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     p.splits = 1;
     const uint64_t pairs = (uint64_t)b->sequences * c->kv_heads;
     if (p.narrow) {
-        // two workgroups a CU are resident (one of head width 256); a
-        // workgroup's start and its part in the join cost as much as some
+        // two workgroups a CU are resident; a workgroup's start and its part in the join cost as much as some
         // hundred tokens, so none takes fewer than that, and what a workgroup
         // a sequence and head reads in that time is not shared at all
-        const uint64_t resident = (uint64_t)cu * (c->head_dim == 256 ? 1 : 2);
+        const uint64_t resident = (uint64_t)cu * 2;
         if (full > 512) {
             p.shares = (uint32_t)resident;
             p.least = 4;
@@ -247,7 +247,7 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
     // the tokens of a (sequence, head, row tile) are cut into pieces where
     // those alone are too few workgroups
-    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 2, least = 512;
+    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 4, least = 256;
     auto pieces = [&](uint64_t tokens) {
         return std::max<uint64_t>(1, std::min<uint64_t>((want + units - 1) / units, (tokens + least - 1) / least));
     };
@@ -430,6 +430,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     else
         st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
+    if (!p.shares && p.splits <= 16) return launch(kernels.joinRow[di], op, batch->rows, 0, stream, &a);
     const uint32_t most = p.shares ? p.shares : p.splits;
     return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
 }

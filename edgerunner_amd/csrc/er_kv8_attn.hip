@@ -492,14 +492,24 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
                                                p.scale, 16 * g, 64, 8, qb, column_max4);
     NarrowState<D> st = {};
     st.m = ER_NO_MAX;
-    while (T < end) {
-        if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
-        T = next_whole(U + 128);
-        attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
-        if (U >= end) break;
-        if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
-        U = next_whole(T + 128);
-        attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
+    if constexpr (D < 256) {
+        while (T < end) {
+            if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
+            T = next_whole(U + 128);
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
+            if (U >= end) break;
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            U = next_whole(T + 128);
+            attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
+        }
+    } else {
+        // 16 KB a tile: one in registers, and twice the waves
+        while (T < end) {
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
+            T = U;
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            U = next_whole(T + 128);
+        }
     }
     for (T = rest; T < end; T += 128) {
         pages = narrow_pages<P>(p, s, T, w.anyLo, end);
@@ -1017,6 +1027,34 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
     });
 }
 
+// All heads of one row after the wide kernel, where the parts are few: four
+// values a thread, its column's references and sums read by all its lanes.
+template <int D>
+ER_DEV void kv8_join_row(const ErAttendArgs &p) {
+    const uint32_t row = blockIdx.x, heads = p.group * p.c.heads, lane = threadIdx.x & 63u;
+    const uint32_t s = uniform(sequence_of_row(p.b, row, lane));
+    if (s >= p.b.sequences) return;
+    const Sequence q = sequence_of(p.b, s);
+    if ((int)row < q.row0 || (int)row >= q.row0 + q.n) return;
+    for (uint32_t at = threadIdx.x; at < heads * (D / 4); at += ER_KV8_THREADS) {
+        const uint32_t head = at / (D / 4), d = (at % (D / 4)) * 4;
+        float top = ER_NO_MAX, total = 0.0f;
+        bool seen = false;
+        for (uint32_t i = 0; i < p.splits; ++i) top = fmaxf(top, p.partML[2 * part_index(p, i, (int)row, head)]);
+        f32x4 o = {};
+        for (uint32_t i = 0; i < p.splits; ++i) {
+            const size_t part = part_index(p, i, (int)row, head);
+            const float l = p.partML[2 * part + 1];
+            if (l < 0.0f) continue;
+            const float f = __builtin_amdgcn_exp2f(p.partML[2 * part] - top);
+            total += l * f;
+            o += *(const f32x4 *)(p.partO + part * D + d) * f;
+            seen = true;
+        }
+        store4(p, (int)row, head, d, D, seen ? o * (1.0f / total) : f32x4{});
+    }
+}
+
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
 
 // One kernel for each head width, page size and output type.  WAVES: waves a
@@ -1042,11 +1080,14 @@ extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
     ER_KV8_PAGES(D, 16, NARROW, WIDE) ER_KV8_PAGES(D, 32, NARROW, WIDE) ER_KV8_PAGES(D, 64, NARROW, WIDE)
 ER_KV8_ATTEND(64, 2, 3)
 ER_KV8_ATTEND(128, 2, 2)
-ER_KV8_ATTEND(256, 1, 1)
+ER_KV8_ATTEND(256, 2, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_d##D(ErAttendArgs p) {                \
         kv8_join<D>(p, er_kv8_lds);                                                                                \
+    }                                                                                                              \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_row_d##D(ErAttendArgs p) {            \
+        kv8_join_row<D>(p);                                                                                        \
     }
 ER_KV8_JOIN(64)
 ER_KV8_JOIN(128)

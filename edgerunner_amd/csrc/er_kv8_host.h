@@ -13,7 +13,7 @@ constexpr int kKv8Pages = 3;  // pages of 16, 32, 64 tokens
 
 struct Kv8Kernels {
     hipModule_t module = nullptr;
-    hipFunction_t rope[kKv8Dims] = {}, append[kKv8Dims] = {}, join[kKv8Dims] = {};
+    hipFunction_t rope[kKv8Dims] = {}, append[kKv8Dims] = {}, join[kKv8Dims] = {}, joinRow[kKv8Dims] = {};
     hipFunction_t narrow[kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};  // [fp32, bf16 output]
 };
 
