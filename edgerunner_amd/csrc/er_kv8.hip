@@ -98,24 +98,57 @@ ER_DEV Pairs load_pairs(const float *p, const PairPlace &pl) {
     return to_pairs(lo, hi, pl.neighbours);
 }
 
-// cos and sin of the four pairs' angles.  position * frequency is formed and
-// brought to a fraction of a turn in 64 bits (at position 10^6 an fp32 product
-// is off by 0.03 rad); the fraction goes to fp32, off by at most 2^-25 turns.
+// cos and sin of a fraction of a turn, |x| <= 1/2: the nearest quarter turn is
+// taken off exactly, and the Taylor series of the rest, |a| <= pi / 4, end
+// where their next terms are below 2^-25 (a^11 / 11! and a^10 / 10!).  About
+// half the instructions of two library calls, which reduce each on its own.
+ER_DEV void cos_sin_turn(float x, float &c, float &s) {
+    const float q = rintf(4.0f * x);
+    const float a = (x - 0.25f * q) * 6.283185307f, z = a * a;
+    float sn = __builtin_fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
+    sn = __builtin_fmaf(z, sn, 8.3333333e-3f);
+    sn = __builtin_fmaf(z, sn, -1.6666667e-1f);
+    sn = __builtin_fmaf(a * z, sn, a);
+    float cs = __builtin_fmaf(z, 2.4801587e-5f, -1.3888889e-3f);
+    cs = __builtin_fmaf(z, cs, 4.1666667e-2f);
+    cs = __builtin_fmaf(z, cs, -0.5f);
+    cs = __builtin_fmaf(z, cs, 1.0f);
+    const int k = (int)q;
+    const float u = k & 1 ? sn : cs, v = k & 1 ? cs : sn;
+    c = (k + 1) & 2 ? -u : u;
+    s = k & 2 ? -v : v;
+}
+
+// The four pairs' frequencies in turns, and their cos and sin at a position.
+// position * frequency is formed and brought to a fraction of a turn in 64
+// bits (at position 10^6 an fp32 product is off by 0.03 rad); the fraction goes
+// to fp32, off by at most 2^-25 turns.
+struct Frequencies {
+    double f[4];
+    bool on;
+};
 struct Turns {
     float c[4], s[4];
     bool on;
 };
-ER_DEV Turns turns_of(int position, const float *freq, uint32_t sub, bool turns) {
-    Turns t = {};
-    t.on = turns;
+ER_DEV Frequencies frequencies_of(const float *freq, uint32_t sub, bool turns) {
+    Frequencies r = {};
+    r.on = turns;
     if (turns) {
         const f32x4 f = *(const f32x4_a4 *)(freq + 4u * sub);
 #pragma unroll
+        for (int i = 0; i < 4; ++i) r.f[i] = (double)f[i] * 0.15915494309189533577;  // 1 / 2 pi
+    }
+    return r;
+}
+ER_DEV Turns turns_of(int position, const Frequencies &f) {
+    Turns t = {};
+    t.on = f.on;
+    if (f.on) {
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const double turn = (double)position * (double)f[i] * 0.15915494309189533577;  // 1 / 2 pi
-            const float part = (float)(turn - rint(turn));
-            t.s[i] = sinpif(2.0f * part);
-            t.c[i] = cospif(2.0f * part);
+            const double turn = (double)position * f.f[i];
+            cos_sin_turn((float)(turn - rint(turn)), t.c[i], t.s[i]);
         }
     }
     return t;
@@ -186,7 +219,7 @@ ER_DEV void qk_norm_rope(const ErRopeArgs &p) {
     if (row >= p.rows) return;
     const uint32_t lane = threadIdx.x & 63u, sub = lane % (D / 8), group = lane / (D / 8);
     const PairPlace pl = pair_place(sub, p.rot, p.pairs);
-    const Turns t = turns_of(p.positions ? p.positions[row] : 0, p.freq, sub, pl.turns);
+    const Turns t = turns_of(p.positions ? p.positions[row] : 0, frequencies_of(p.freq, sub, pl.turns));
     constexpr uint32_t PER = 512 / D;
     // strips of the query heads, then of the key heads, dealt to the row's waves in turn
     const uint32_t qStrips = (p.q.heads + PER - 1) / PER;
@@ -260,7 +293,7 @@ ER_DEV void turn_query_row(const ErAppendArgs &p) {
     const int at = (int)row - q.row0, position = q.len - q.n + at;
     if (at < 0 || at >= q.n || position < 0) return;
     const PairPlace pl = pair_place(sub, p.rot, p.pairs);
-    const Turns t = turns_of(position, p.freq, sub, pl.turns);
+    const Turns t = turns_of(position, frequencies_of(p.freq, sub, pl.turns));
     turn_heads<D>(p.q, row, chunk, p.chunks, group, pl, t, p.eps);
 }
 
@@ -276,8 +309,9 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
     constexpr int TOKENS = ER_KV8_THREADS / LANES < P ? ER_KV8_THREADS / LANES : P;  // tokens a pass
     constexpr int PASSES = P / TOKENS;
     const uint32_t H = p.c.heads;
-    const bool values = blockIdx.x & 1u;
-    uint32_t at = blockIdx.x >> 1;
+    // keys first, as they take longer, and so that every XCD gets as many
+    const bool values = blockIdx.x >= p.cacheBlocks / 2;
+    uint32_t at = values ? blockIdx.x - p.cacheBlocks / 2 : blockIdx.x;
     const uint32_t head = at % H;
     at /= H;
     const uint32_t span = at % p.spans, s = at / p.spans;
@@ -299,6 +333,7 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
     const bool norm = !values && p.kNorm != nullptr;
     Pairs w = {};
     if (norm) w = load_pairs(p.kNorm, pl);
+    const Frequencies freq = frequencies_of(p.freq, sub, pl.turns);
     Pairs v[PASSES];
     float peak = 0.0f;
 #pragma unroll
@@ -325,7 +360,7 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
         const int t = begin + i * TOKENS + slot;
         if (!values) {
             const bool live = slot < TOKENS && t >= t0 && t < t1;
-            norm_turn<D>(v[i], norm, w, turns_of(t, p.freq, sub, pl.turns && live), p.eps);
+            norm_turn<D>(v[i], norm, w, live ? turns_of(t, freq) : Turns{}, p.eps);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
