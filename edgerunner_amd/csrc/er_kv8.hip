@@ -179,6 +179,105 @@ ER_DEV void norm_turn(Pairs &v, bool norm, const Pairs &w, const Turns &t, float
     }
 }
 
+// The same in 64 bits for keys on their way into codes: rounded to fp32 before,
+// one in some hundred thousand, those next to a border, would get the other
+// code.  64-bit operations run at the rate of 32-bit ones here (the fp32 form
+// took 14 us for three ragged prompts of an 8B layer, this one 16); the
+// results go to fp32 by rounding to odd, which no later rounding to fewer bits
+// notices.
+template <int CTRL>
+ER_DEV double dpp_of(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int W>
+ER_DEV double group_sum64(double v) {  // W = 8, 16 or 32 lanes
+    v += dpp_of<ER_DPP_QUAD_XOR1>(v);
+    v += dpp_of<ER_DPP_QUAD_XOR2>(v);
+    v += dpp_of<ER_DPP_ROW_HALF_MIRROR>(v);
+    if constexpr (W >= 16) v += dpp_of<ER_DPP_ROW_MIRROR>(v);
+    if constexpr (W == 32) v += __shfl_xor(v, 16);
+    return v;
+}
+ER_DEV float round_to_odd(double v) {
+    float f = (float)v;
+    const double back = (double)f;
+    uint32_t u = __float_as_uint(f);
+    if (fabs(back) > fabs(v)) u -= 1;  // to zero
+    if (back != v && v == v) u |= 1;
+    return __uint_as_float(u);
+}
+// cos and sin of a fraction of a turn as cos_sin_turn; the next terms of the
+// series are below 2^-40.
+ER_DEV void cos_sin_turn64(double x, double &c, double &s) {
+    const double q = rint(4.0 * x);
+    const double a = (x - 0.25 * q) * 6.283185307179586477, z = a * a;
+    double sn = __builtin_fma(z, 1.6059043836821613e-10, -2.5052108385441719e-8);
+    sn = __builtin_fma(z, sn, 2.7557319223985893e-6);
+    sn = __builtin_fma(z, sn, -1.9841269841269841e-4);
+    sn = __builtin_fma(z, sn, 8.3333333333333333e-3);
+    sn = __builtin_fma(z, sn, -1.6666666666666667e-1);
+    sn = __builtin_fma(a * z, sn, a);
+    double cs = __builtin_fma(z, 2.0876756987868099e-9, -2.7557319223985891e-7);
+    cs = __builtin_fma(z, cs, 2.4801587301587302e-5);
+    cs = __builtin_fma(z, cs, -1.3888888888888889e-3);
+    cs = __builtin_fma(z, cs, 4.1666666666666667e-2);
+    cs = __builtin_fma(z, cs, -0.5);
+    cs = __builtin_fma(z, cs, 1.0);
+    const int k = (int)q;
+    const double u = k & 1 ? sn : cs, v = k & 1 ? cs : sn;
+    c = (k + 1) & 2 ? -u : u;
+    s = k & 2 ? -v : v;
+}
+struct Turns64 {
+    double c[4], s[4];
+};
+ER_DEV void turns64_of(Turns64 &t, int position, const Frequencies &f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double turn = (double)position * f.f[i];
+        cos_sin_turn64(turn - rint(turn), t.c[i], t.s[i]);
+    }
+}
+// t further on by the angles of `by`.
+ER_DEV void turn_on(Turns64 &t, const Turns64 &by) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double c = t.c[i] * by.c[i] - t.s[i] * by.s[i];
+        t.s[i] = t.s[i] * by.c[i] + t.c[i] * by.s[i];
+        t.c[i] = c;
+    }
+}
+template <int D>
+ER_DEV void norm_turn64(Pairs &p, bool norm, const Pairs &w, bool turns, const Turns64 &t, double eps) {
+    double a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[i] = (double)p.a[i];
+        b[i] = (double)p.b[i];
+    }
+    if (norm) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = __builtin_fma(b[i], b[i], __builtin_fma(a[i], a[i], sum));
+        // one Newton step doubles the correct bits of the instruction's root, over 20
+        const double ms = group_sum64<D / 8>(sum) * (1.0 / D) + eps, r0 = __builtin_amdgcn_rsq(ms);
+        const double r = r0 * __builtin_fma(-0.5 * ms * r0, r0, 1.5);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] *= r * (double)w.a[i];
+            b[i] *= r * (double)w.b[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        p.a[i] = round_to_odd(turns ? a[i] * t.c[i] - b[i] * t.s[i] : a[i]);
+        p.b[i] = round_to_odd(turns ? b[i] * t.c[i] + a[i] * t.s[i] : b[i]);
+    }
+}
+
 // One row's heads of one kind in strips of 512 / D, of which this wave takes
 // chunk, chunk + chunks, ...: D / 8 lanes a head.
 template <int D>
@@ -334,6 +433,8 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
     Pairs w = {};
     if (norm) w = load_pairs(p.kNorm, pl);
     const Frequencies freq = frequencies_of(p.freq, sub, pl.turns);
+    Turns64 turns = {}, onward = {};
+    bool turned = false;
     Pairs v[PASSES];
     float peak = 0.0f;
 #pragma unroll
@@ -358,9 +459,20 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int t = begin + i * TOKENS + slot;
-        if (!values) {
-            const bool live = slot < TOKENS && t >= t0 && t < t1;
-            norm_turn<D>(v[i], norm, w, live ? turns_of(t, freq) : Turns{}, p.eps);
+        // passes without a new token are skipped by all lanes: a decode step's
+        // block has one; from one pass to the next the angles grow by the same
+        const int from = begin + i * TOKENS;
+        if (!values && from < t1 && from + TOKENS > t0 && (norm || p.rot)) {
+            if (p.rot) {
+                if (!turned) {
+                    turns64_of(turns, t, freq);
+                    if (from + TOKENS < t1) turns64_of(onward, TOKENS, freq);
+                    turned = true;
+                } else {
+                    turn_on(turns, onward);
+                }
+            }
+            norm_turn64<D>(v[i], norm, w, freq.on, turns, (double)p.eps);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -384,7 +496,8 @@ ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int t = begin + i * TOKENS + slot;
-        if (!(slot < TOKENS && t >= t0 && t < t1)) continue;
+        const bool live = slot < TOKENS && t >= t0 && t < t1;
+        if (!live) continue;
         f32x4 lo, hi;
         from_pairs(v[i], pl.neighbours, lo, hi);
         uint8_t *c = codes + (size_t)(t - begin) * D + pl.at;
