@@ -485,7 +485,8 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     };
     NarrowTile<D> t0, t1;
     int T = next_whole(begin + 32 * (int)wave);
-    if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
+    const NarrowPages firstPages = pages;
+    if (D < 256 && T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
     int U = next_whole(T + 128);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
@@ -503,7 +504,9 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
             attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
         }
     } else {
-        // 16 KB a tile: one in registers, and twice the waves
+        // 16 KB a tile: one in registers, and twice the waves; the first waits
+        // until the query's fp32 values have left theirs
+        if (T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
         while (T < end) {
             attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
             T = U;
@@ -599,7 +602,7 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
         if (at >= last) return;
         if (++h == H) {
             h = 0;
-            do l = lane_sequence_at(p, first, ++s);
+            do l = lane_sequence(p, ++s);
             while (l.steps == 0);
             length = shared_length(p, l.steps, sh.aligned);
         }
@@ -1072,15 +1075,18 @@ extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
         kv8_attend_wide<D, P, TERMS>(p, tiles);                                                                    \
     }
 #define ER_KV8_PAGES(D, P, NARROW, WIDE)                                                                           \
-    ER_KV8_NARROW(D, P, 1, bf16, NARROW)                                                                           \
+    ER_KV8_NARROW(D, P, 1, bf16, 2)                                                                                \
     ER_KV8_NARROW(D, P, 2, f32, NARROW)                                                                            \
     ER_KV8_WIDE(D, P, 1, bf16, WIDE)                                                                               \
     ER_KV8_WIDE(D, P, 2, f32, WIDE)
-#define ER_KV8_ATTEND(D, NARROW, WIDE)                                                                             \
-    ER_KV8_PAGES(D, 16, NARROW, WIDE) ER_KV8_PAGES(D, 32, NARROW, WIDE) ER_KV8_PAGES(D, 64, NARROW, WIDE)
-ER_KV8_ATTEND(64, 2, 3)
-ER_KV8_ATTEND(128, 2, 2)
-ER_KV8_ATTEND(256, 2, 1)
+#define ER_KV8_ATTEND(D, WIDE) ER_KV8_PAGES(D, 32, 2, WIDE) ER_KV8_PAGES(D, 64, 2, WIDE)
+ER_KV8_ATTEND(64, 3)
+ER_KV8_ATTEND(128, 2)
+ER_KV8_ATTEND(256, 1)
+ER_KV8_PAGES(64, 16, 2, 3)
+ER_KV8_PAGES(128, 16, 2, 2)
+// two pages a tile, two terms and wide heads need a few registers over the 256 that two waves leave
+ER_KV8_PAGES(256, 16, 1, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_d##D(ErAttendArgs p) {                \
