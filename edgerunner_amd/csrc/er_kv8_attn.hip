@@ -634,23 +634,42 @@ struct WideTile {
     uint32_t v[(D + 127) / 128][8];        // see value_item
 };
 
+// 64 entries of the page table with their scales, one a lane, and a tile's out
+// of them by lane reads.  Loading them tile by tile into scalar registers would
+// have every LDS wait of the tile wait for them too: scalar loads share its
+// counter, and return out of order.
 template <int P>
-ER_DEV void wide_pages(WidePages<P> &w, const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
-#pragma unroll
-    for (int i = 0; i < w.N; ++i) {
-        const int at = T + P * i;
-        w.page[i] = at < hi && at + P > lo ? uniform(page_of(p.b, p.c, s, at)) : -1;
-    }
-}
+struct PageWindow {
+    int first;  // table entry of lane 0
+    int page;
+    float ks, vs;
+};
 template <int P>
-ER_DEV void wide_scales(WidePages<P> &w, const ErAttendArgs &p, uint32_t h) {
-#pragma unroll
-    for (int i = 0; i < w.N; ++i) {
-        const size_t block = (size_t)(uint32_t)max(w.page[i], 0) * p.c.heads + h;
-        w.ks[i] = load_shared(p.c.ks + block);
-        w.vs[i] = load_shared(p.c.vs + block);
-    }
+ER_DEV void fill_window(PageWindow<P> &w, const ErAttendArgs &p, uint32_t s, uint32_t h, int T, int lo, int end,
+                        uint32_t lane) {
+    const int tok = T + P * (int)lane;
+    w.first = T / P;
+    w.page = tok < end && tok + P > lo ? page_of(p.b, p.c, s, tok) : -1;
+    const size_t block = (size_t)(uint32_t)max(w.page, 0) * p.c.heads + h;
+    w.ks = p.c.ks[block];
+    w.vs = p.c.vs[block];
 }
+// The pages of the tile at T; tiles are asked for in order.
+template <int P>
+ER_DEV WidePages<P> pages_at(PageWindow<P> &w, const ErAttendArgs &p, uint32_t s, uint32_t h, int T, int lo, int end,
+                             uint32_t lane) {
+    if (T / P - w.first >= 64) fill_window<P>(w, p, s, h, T, lo, end, lane);
+    WidePages<P> r;
+#pragma unroll
+    for (int i = 0; i < r.N; ++i) {
+        const int at = T / P - w.first + i;
+        r.page[i] = __builtin_amdgcn_readlane(w.page, at);
+        r.ks[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w.ks), at));
+        r.vs[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w.vs), at));
+    }
+    return r;
+}
+
 // Entry of a tile's 16-token part, without an address (which would put v into scratch memory).
 template <int N>
 ER_DEV int of_part(const int (&v)[N], uint32_t part) {
@@ -818,11 +837,10 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     bool seen = false;
     if (begin < end) {
         WideTile<D, P> t;
-        WidePages<P> now, next;  // of the tile in `t`, and of the one behind it
-        wide_pages(now, p, s, begin, w.anyLo, end);
-        wide_pages(next, p, s, begin + 64, w.anyLo, end);
+        PageWindow<P> window;
+        fill_window<P>(window, p, s, h, begin, w.anyLo, end, lane);
+        WidePages<P> now = pages_at<P>(window, p, s, h, begin, w.anyLo, end, lane);  // of the tile in `t`
         load_wide<D, P>(t, now, p, h, tid);
-        wide_scales(now, p, h);
         h8 qb[TERMS][D / 16];
         const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live, p.scale,
                                                    16 * hh, 32, 8, qb, column_max2);
@@ -833,11 +851,9 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
         if (!whole(now, w, begin)) nans |= mask_wide<D, P>(t, now, begin, w.anyLo, end, tid);
         store_wide<D, P>(lds[0], t, tid);
         WidePages<P> parts = now;
-        now = next;
         if (begin + 64 < end) {
+            now = pages_at<P>(window, p, s, h, begin + 64, w.anyLo, end, lane);
             load_wide<D, P>(t, now, p, h, tid);
-            wide_scales(now, p, h);
-            wide_pages(next, p, s, begin + 128, w.anyLo, end);
         }
         uint32_t buf = 0;
         for (int T = begin; T < end; T += 64, buf ^= 1u) {
@@ -916,10 +932,8 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
             }
             parts = now;
             if (T + 128 < end) {
-                now = next;
+                now = pages_at<P>(window, p, s, h, T + 128, w.anyLo, end, lane);
                 load_wide<D, P>(t, now, p, h, tid);
-                wide_scales(now, p, h);
-                wide_pages(next, p, s, T + 192, w.anyLo, end);
             }
         }
         if (__syncthreads_or(nans)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);

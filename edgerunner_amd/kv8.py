@@ -84,37 +84,48 @@ class KV8Batch(_Descriptor):
 
 
 class _Kernel:
+    entry = ""
+
     def __init__(self, ctx: Optional[Context] = None):
         self.ctx = ctx or default_context()
         self.lib = self.ctx.lib
+        self._call = getattr(self.lib, self.entry)  # a decode step's calls are bound by the host: looked up once
 
 
 class QKNormRopeKernel(_Kernel):
     """RMS norm of each query and key head and the position rotation in one pass."""
 
+    entry = "er_hip_qk_norm_rope"
+
     def encode(self, stream: Optional[Stream], q: HeadRows, k: Optional[HeadRows], qOut: HeadRows,
                kOut: Optional[HeadRows], positions: Optional[Buffer], rows: int, headDim: int, rope: Rope,
                qNorm: Optional[Buffer] = None, kNorm: Optional[Buffer] = None, eps: float = 1e-6) -> None:
         """q, k fp32 rows; a norm weight of None leaves that norm out; outputs may be their own inputs."""
-        check(self.lib.er_hip_qk_norm_rope(self.ctx.handle, _sh(stream), q.ref, _ref(k), qOut.ref, _ref(kOut),
-                                           _raw(positions), _raw(qNorm), _raw(kNorm), rope.ref, rows, headDim, eps),
-              self.lib)
+        status = self._call(self.ctx.handle, _sh(stream), q.ref, _ref(k), qOut.ref, _ref(kOut), _raw(positions),
+                            _raw(qNorm), _raw(kNorm), rope.ref, rows, headDim, eps)
+        if status:
+            check(status, self.lib)
 
 
 class KV8AppendKernel(_Kernel):
     """Appends keys (normed and rotated on the way) and values to the cache; queries may ride along."""
 
+    entry = "er_hip_kv8_append"
+
     def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, k: HeadRows, v: HeadRows, rope: Rope,
                kNorm: Optional[Buffer] = None, q: Optional[HeadRows] = None, qOut: Optional[HeadRows] = None,
                qNorm: Optional[Buffer] = None, eps: float = 1e-6, vHalf: bool = False) -> None:
         """k fp32, v fp32 or (vHalf) fp16, with the cache's heads."""
-        check(self.lib.er_hip_kv8_append(self.ctx.handle, _sh(stream), cache.ref, batch.ref, k.ref, v.ref,
-                                         TYPE_F16 if vHalf else TYPE_F32, _ref(q), _ref(qOut), _raw(kNorm),
-                                         _raw(qNorm), rope.ref, eps), self.lib)
+        status = self._call(self.ctx.handle, _sh(stream), cache.ref, batch.ref, k.ref, v.ref,
+                            TYPE_F16 if vHalf else TYPE_F32, _ref(q), _ref(qOut), _raw(kNorm), _raw(qNorm), rope.ref, eps)
+        if status:
+            check(status, self.lib)
 
 
 class KV8AttentionKernel(_Kernel):
     """Causal attention of the batch's rows over the cache."""
+
+    entry = "er_hip_kv8_attention"
 
     def workspaceBytes(self, cache: KV8Cache, batch: KV8Batch, qHeads: int) -> int:
         """Bytes of scratch that encode needs for such a batch, whatever its window and output type."""
@@ -126,6 +137,7 @@ class KV8AttentionKernel(_Kernel):
     def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, q: HeadRows, out: HeadRows,
                scale: float, window: int = 0, workspace: Optional[Buffer] = None, outBF16: bool = False) -> None:
         """q fp32; out fp32 or bf16; window: the latest tokens that a row sees (0: all)."""
-        check(self.lib.er_hip_kv8_attention(self.ctx.handle, _sh(stream), cache.ref, batch.ref, q.ref, out.ref,
-                                            TYPE_BF16 if outBF16 else TYPE_F32, scale, window, _raw(workspace)),
-              self.lib)
+        status = self._call(self.ctx.handle, _sh(stream), cache.ref, batch.ref, q.ref, out.ref,
+                            TYPE_BF16 if outBF16 else TYPE_F32, scale, window, _raw(workspace))
+        if status:
+            check(status, self.lib)
