@@ -259,9 +259,14 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     return p;
 }
 
-er_status check_group(const char *op, const er_kv8_cache *c, uint32_t qHeads) {
+er_status check_group(const char *op, const er_kv8_cache *c, const er_kv8_batch *b, uint32_t qHeads) {
     if (qHeads == 0 || qHeads % c->kv_heads != 0 || qHeads / c->kv_heads > 1024)
         return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u query heads over %u key/value heads", op, qHeads, c->kv_heads);
+    // columns of a sequence, and 64-token steps of all sequences and heads (rounded up to four each), are 32-bit counts
+    const uint64_t steps = (uint64_t)b->sequences * ((most_tokens(c, b) + 63u) / 64u + 4u);
+    if ((uint64_t)b->max_rows * (qHeads / c->kv_heads) > 0x7fffffffull || steps > 0x7fffffffull / c->kv_heads)
+        return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u sequences of up to %u tokens and %u rows: too many to count in 31 bits",
+                    op, b->sequences, most_tokens(c, b), b->max_rows);
     return ER_OK;
 }
 
@@ -375,7 +380,7 @@ er_status er_hip_kv8_attention_workspace(er_hip_ctx *ctx, const er_kv8_cache *ca
     *bytes = 0;
     er_status st = check_cache(op, cache);
     if (st == ER_OK) st = check_batch(op, batch);
-    if (st == ER_OK) st = check_group(op, cache, q_heads);
+    if (st == ER_OK) st = check_group(op, cache, batch, q_heads);
     if (st == ER_OK) st = check_ctx(ctx);
     if (st != ER_OK) return st;
     if (batch->rows == 0 || batch->sequences == 0) return ER_OK;
@@ -399,7 +404,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     if (st == ER_OK) st = check_rows(op, "out", out, batch->rows, d, outBytes);
     if (st != ER_OK) return st;
     if (q->heads != out->heads) return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: q and out differ in heads", op);
-    st = check_group(op, cache, q->heads);
+    st = check_group(op, cache, batch, q->heads);
     if (st == ER_OK) st = check_apart(op, "q and out", q, out, batch->rows, d, 4, outBytes, false);
     if (st == ER_OK) st = check_ctx(ctx);
     if (st == ER_OK) st = bind_device_of(ctx);

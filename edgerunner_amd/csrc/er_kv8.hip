@@ -264,7 +264,7 @@ ER_DEV void norm_turn64(Pairs &p, bool norm, const Pairs &w, bool turns, const T
         for (int i = 0; i < 4; ++i) sum = __builtin_fma(b[i], b[i], __builtin_fma(a[i], a[i], sum));
         // one Newton step doubles the correct bits of the instruction's root, over 20
         const double ms = group_sum64<D / 8>(sum) * (1.0 / D) + eps, r0 = __builtin_amdgcn_rsq(ms);
-        const double r = r0 * __builtin_fma(-0.5 * ms * r0, r0, 1.5);
+        const double r = ms < __builtin_inf() ? r0 * __builtin_fma(-0.5 * ms * r0, r0, 1.5) : r0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             a[i] *= r * (double)w.a[i];

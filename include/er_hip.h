@@ -469,9 +469,10 @@ typedef struct er_kv8_cache {
  * max_rows and max_kv_len bound what any sequence has: more is not looked at
  * (rows beyond the first max_rows, tokens beyond the first max_kv_len or
  * beyond the table).  Rows whose position would be negative are not appended
- * and attend to nothing.  Entries of page_table outside [0, pages) hold no
- * tokens: nothing is read or written there.  A page that gets tokens in a call
- * belongs to one sequence; full pages may be shared by many. */
+ * and attend to nothing (their q_out is left as it is, their output zeros).
+ * Entries of page_table outside [0, pages) hold no tokens: nothing is read or
+ * written there.  A page that gets tokens in a call stands once in the tables:
+ * in one place of one sequence's; full pages may be shared by many. */
 typedef struct er_kv8_batch {
     er_buffer page_table; /* int32 [sequences][table_stride] */
     er_buffer kv_len;     /* int32 [sequences] */
@@ -509,8 +510,10 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
  * visible to gets zeros.  out does not overlap q.
  * workspace: scratch of er_hip_kv8_attention_workspace bytes (which depend on
  * the batch's and cache's sizes and q_heads alone), 16-byte aligned; calls and
- * recorded graphs that may overlap in time need one each.  q->heads is a multiple of
- * kv_heads, at most 1024 a key/value head.  Errors as er_hip_kv8_append's. */
+ * recorded graphs that may overlap in time need one each.  q->heads is a
+ * multiple of kv_heads, at most 1024 a key/value head.  A block of values whose
+ * scale is less than 2^-22 of the largest that a row's tokens have is rounded to
+ * fewer bits.  Errors as er_hip_kv8_append's. */
 er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
                                const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
                                uint32_t out_type, float scale, uint32_t window, er_buffer workspace);

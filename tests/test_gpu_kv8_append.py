@@ -282,6 +282,32 @@ def test_scales(ctx):
     assert np.all((got[2][page[9], 0, 0, 5:8] & 0x7f) == 0x7f)
 
 
+def test_non_finite_keys_under_norm_and_rotation(ctx):
+    """An infinite element makes its head's root infinite: it becomes NaN, and the pair it turns with, the others zeros; a NaN
+    takes the whole head.  Other heads and tokens keep their codes, and the scales ignore what is not finite."""
+    P, d = 16, 64
+    rng = np.random.default_rng(8)
+    c = Case(ctx, rng, [5], [5], P, d, 3, norm=True)
+    c.k[1, 0, 7], c.k[2, 1, 9], c.k[3, 2, 3] = np.inf, np.nan, -np.inf
+    kc, ks, _, _ = c.run()
+    page = c.b.table[0, 0]
+    clean = c.k.copy()
+    for r, h in ((1, 0), (2, 1), (3, 2)):
+        clean[r, h] = 0
+    x = R.norm_rope(clean, np.arange(5), c.f, d, False, c.w)
+    for h in range(3):
+        assert ks[page, h] == R.block_scale(np.abs(x[:, h]).max())
+    got = R.VALUES[kc[page, :, :5]].transpose(1, 0, 2)
+    for r, h, e in ((1, 0, 7), (3, 2, 3)):
+        pair = [e, e + d // 2]
+        assert np.all(np.isnan(got[r, h, pair])) and np.all(np.delete(got[r, h], pair) == 0)
+    assert np.all(np.isnan(got[2, 1]))
+    for r in range(5):
+        for h in range(3):
+            if (r, h) not in ((1, 0), (2, 1), (3, 2)):
+                assert np.array_equal(kc[page, h, r], R.to_e4m3(x[r, h] / ks[page, h]))
+
+
 def test_growth_keeps_exact_codes(ctx):
     """A block of normal codes grows by 2^6 and keeps its values exactly; NaN codes stay."""
     P, d = 32, 64

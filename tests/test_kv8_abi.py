@@ -174,6 +174,18 @@ def test_attention_refusals():
     assert call_attend(o=half, ot=BF16) == OK_BUT_NO_CTX and "null er_hip_ctx" in last()
 
 
+def test_attention_refuses_what_32_bits_cannot_count():
+    wide = 1024 * 64
+    many = rows(1024, wide, 1 << 22)
+    b = batch(rows_=1 << 22, max_rows=1 << 22)
+    assert call_attend(c=cache(heads=1), b=b, q=many, o=rows(1024, wide, 1 << 22, ptr=1 << 60)) == VEC and "31 bits" in last()
+    n = 1 << 20
+    b = _ffi.er_kv8_batch(buf(4 * n * (1 << 18)), buf(4 * n), buf(4 * n + 4), n, 1 << 18, 3, 2, 1 << 22)
+    assert call_attend(b=b) == VEC and "31 bits" in last()
+    b.max_kv_len = 1 << 10
+    assert call_attend(b=b) == OK_BUT_NO_CTX and "null er_hip_ctx" in last()
+
+
 def test_workspace_query():
     n = C.c_uint64(7)
     f = _ffi.load().er_hip_kv8_attention_workspace
