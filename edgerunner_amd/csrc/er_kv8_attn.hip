@@ -833,6 +833,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 31u, hh = lane >> 5;
     const Spans w = spans_of(p, q, col0, min(col0 + 127, cols - 1));
     const uint32_t wcol0 = col0 + 32 * wave;
+    const bool idle = wcol0 >= cols;
     const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 31, cols - 1));
     const Column c = column_of(p, q, h, min(wcol0 + n, cols - 1));
     const bool live = wcol0 + n < cols;
@@ -861,8 +862,22 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
             now = pages_at<P>(window, p, s, h, begin + 64, w.anyLo, end, lane);
             load_wide<D, P>(t, now, p, h, tid);
         }
+        auto bring = [&](uint32_t to, int T) {  // the tile in `t`, which lies at T, into LDS
+            if (!whole(now, w, T)) nans |= mask_wide<D, P>(t, now, T, w.anyLo, end, tid);
+            store_wide<D, P>(lds[to], t, tid);
+        };
+        auto fetch = [&](int T) {
+            now = pages_at<P>(window, p, s, h, T, w.anyLo, end, lane);
+            load_wide<D, P>(t, now, p, h, tid);
+        };
         uint32_t buf = 0;
-        for (int T = begin; T < end; T += 64, buf ^= 1u) {
+        // a wave without columns only brings its part of the tiles
+        for (int T = begin; idle && T < end; T += 64, buf ^= 1u) {
+            __syncthreads();
+            if (T + 64 < end) bring(buf ^ 1u, T + 64);
+            if (T + 128 < end) fetch(T + 128);
+        }
+        for (int T = begin; !idle && T < end; T += 64, buf ^= 1u) {
             __syncthreads();
             const WideLds<D> &in = lds[buf];
             const bool clear = whole(parts, ww, T);
@@ -886,10 +901,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                         sc = mfma32(a1, qb[term][2 * j + 1], sc);
                     }
                 }
-                if (th == 1 && T + 64 < end) {
-                    if (!whole(now, w, T + 64)) nans |= mask_wide<D, P>(t, now, T + 64, w.anyLo, end, tid);
-                    store_wide<D, P>(lds[buf ^ 1u], t, tid);
-                }
+                if (th == 1 && T + 64 < end) bring(buf ^ 1u, T + 64);
                 if (!clear) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -937,10 +949,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                 }
             }
             parts = now;
-            if (T + 128 < end) {
-                now = pages_at<P>(window, p, s, h, T + 128, w.anyLo, end, lane);
-                load_wide<D, P>(t, now, p, h, tid);
-            }
+            if (T + 128 < end) fetch(T + 128);
         }
         if (__syncthreads_or(nans)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);
     }
