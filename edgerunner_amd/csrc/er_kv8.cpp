@@ -221,12 +221,18 @@ struct AttendPlan {
     uint64_t parts;                 // columns that the workspace holds sums of, at the most over all windows
 };
 
-// Columns (rows times query heads of a key/value head) decide the kernel: up
-// to 16 fit the narrow kernel's one matrix tile.
+// Columns (rows times query heads of a key/value head) decide the kernel.  The
+// narrow one reads the cache once for each 16 of them, the wide one once for
+// 128, with products that pay for columns that are not there, and with less
+// work split between fewer workgroups.  Measured narrow / wide, us: 24 columns
+// of 4 sequences of 30000 tokens 26 / 38, 32 of 16 of 8000 59 / 86 (head width
+// 256: 64 / 180), 60 of 16 of 4000 25 / 56, 128 of 4 of 8000 51 / 55, 128 of 16
+// of 4000 98 / 97, and for bf16, whose wide kernel has half the products, 96 /
+// 84; 256 columns 174 / 101.
 AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group, uint32_t window, int cu) {
     AttendPlan p{};
     const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
-    p.narrow = cols <= 16;
+    p.narrow = cols <= (c->head_dim == 256 ? 128 : 64);
     p.splits = 1;
     const uint64_t pairs = (uint64_t)b->sequences * c->kv_heads;
     if (p.narrow) {
@@ -234,10 +240,11 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
         // hundred tokens, so none takes fewer than that, and what a workgroup
         // a sequence and head reads in that time is not shared at all
         const uint64_t resident = (uint64_t)cu * 2;
+        p.tiles = (uint32_t)((cols + 15) / 16);
         if (full > 512) {
             p.shares = (uint32_t)resident;
             p.least = 4;
-            p.parts = 2 * resident * cols;
+            p.parts = 2 * resident * 16;
         }
         return p;
     }
@@ -246,7 +253,9 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     // the tile's rows see window + rows - 1 tokens, and pieces begin at a multiple of 64
     if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
     // the tokens of a (sequence, head, row tile) are cut into pieces where
-    // those alone are too few workgroups
+    // those alone are too few workgroups: to four a CU, as rows and lengths
+    // are ragged (chunks of three prompts, kernel and join: 83 + 8 us in five
+    // pieces, 97 + 6 in three, 73 + 30 in 17), of 256 tokens at the least
     const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 4, least = 256;
     auto pieces = [&](uint64_t tokens) {
         return std::max<uint64_t>(1, std::min<uint64_t>((want + units - 1) / units, (tokens + least - 1) / least));
@@ -262,9 +271,10 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
 er_status check_group(const char *op, const er_kv8_cache *c, const er_kv8_batch *b, uint32_t qHeads) {
     if (qHeads == 0 || qHeads % c->kv_heads != 0 || qHeads / c->kv_heads > 1024)
         return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u query heads over %u key/value heads", op, qHeads, c->kv_heads);
-    // columns of a sequence, and 64-token steps of all sequences and heads (rounded up to four each), are 32-bit counts
+    // columns of a sequence, and 64-token steps of all sequences and heads (rounded up to four each, for up to eight column
+    // blocks), are 32-bit counts
     const uint64_t steps = (uint64_t)b->sequences * ((most_tokens(c, b) + 63u) / 64u + 4u);
-    if ((uint64_t)b->max_rows * (qHeads / c->kv_heads) > 0x7fffffffull || steps > 0x7fffffffull / c->kv_heads)
+    if ((uint64_t)b->max_rows * (qHeads / c->kv_heads) > 0x7fffffffull || steps > 0x0fffffffull / c->kv_heads)
         return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u sequences of up to %u tokens and %u rows: too many to count in 31 bits",
                     op, b->sequences, most_tokens(c, b), b->max_rows);
     return ER_OK;
@@ -431,7 +441,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     const int di = dim_index(d);
     const uint64_t pairs = (uint64_t)batch->sequences * cache->kv_heads;
     if (p.narrow)
-        st = launch(kernels.narrow[di][a.c.shift - 4][a.half], op, p.shares ? p.shares : pairs, 0, stream, &a);
+        st = launch(kernels.narrow[di][a.c.shift - 4][a.half], op, p.shares ? p.shares : pairs * p.tiles, 0, stream, &a);
     else
         st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
     if (st != ER_OK || !joined) return st;

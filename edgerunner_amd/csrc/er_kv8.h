@@ -68,7 +68,8 @@ struct ErAttendArgs {
     // at least `least` 64-token steps each (0: a workgroup a sequence and head)
     uint32_t shares, least;
     // wide kernel: pieces of a row tile's tokens, tokens of a piece (a multiple
-    // of 64), row tiles of a sequence and key/value head
+    // of 64), row tiles of a sequence and key/value head (narrow kernel: blocks
+    // of 16 columns)
     uint32_t splits, chunk, tiles;
     uint32_t window;          // 0: none
     uint32_t half;            // bf16 output

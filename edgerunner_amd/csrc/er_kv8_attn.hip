@@ -156,7 +156,7 @@ ER_DEV size_t part_index(const ErAttendArgs &p, uint32_t piece, int row, uint32_
 // Where some are and l is 0 or NaN (scores without a finite maximum), the
 // quotient is NaN, as the softmax's is.
 
-// ---------------------------------------------------------------- up to 16 columns: decode
+// ---------------------------------------------------------------- few columns: decode, drafts
 
 // One 32-token tile of keys and values in registers, as loaded.
 template <int D>
@@ -361,7 +361,7 @@ struct Const {
 };
 
 // How the tokens of all sequences and heads are shared between workgroups.
-// Units (sequence, head) lie one behind the other, each `length` steps of 64
+// Units (sequence, head, block of 16 columns) lie one behind the other, each `length` steps of 64
 // tokens long, and workgroup w takes steps w * quota .. (w + 1) * quota - 1 of
 // that line: whatever the sequences' lengths, all have the same to read, and a
 // workgroup's start (some microseconds of dependent loads) is paid once for each
@@ -378,6 +378,8 @@ ER_DEV uint32_t steps_of(const ErAttendArgs &p, const Sequence &q) {
     // rows that see nothing take a step all the same, which writes their zeros
     return max(1u, ((uint32_t)max(w.anyHi - (w.anyLo & ~63), 0) + 63u) >> 6);
 }
+// Column blocks of a sequence and key/value head.
+ER_DEV uint32_t blocks_of(const ErAttendArgs &p, const Sequence &q) { return ((uint32_t)q.n * p.group + 15u) >> 4; }
 ER_DEV uint32_t shared_length(const ErAttendArgs &p, uint32_t steps, bool aligned) {
     return aligned ? (steps + p.least - 1) / p.least * p.least : steps;
 }
@@ -422,11 +424,11 @@ ER_DEV LaneSequence lane_sequence_at(const ErAttendArgs &p, const LaneSequence &
     return l;
 }
 ER_DEV Shares shares_of(const ErAttendArgs &p, const LaneSequence &first, uint32_t lane) {
-    uint32_t plain = first.steps, padded = shared_length(p, first.steps, true);
+    uint32_t plain = first.steps * blocks_of(p, first.q), padded = shared_length(p, first.steps, true) * blocks_of(p, first.q);
     for (uint32_t at = 64; at < p.b.sequences; at += 64) {
-        const uint32_t t = lane_sequence(p, at + lane).steps;
-        plain += t;
-        padded += shared_length(p, t, true);
+        const LaneSequence l = lane_sequence(p, at + lane);
+        plain += l.steps * blocks_of(p, l.q);
+        padded += shared_length(p, l.steps, true) * blocks_of(p, l.q);
     }
     plain = wave_sum(plain) * p.c.heads;
     padded = wave_sum(padded) * p.c.heads;
@@ -441,8 +443,8 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bo
                             uint32_t &begins) {
     uint32_t before = 0;
     for (uint32_t s0 = 0;; s0 += 64) {
-        const uint32_t steps = s0 ? lane_sequence(p, s0 + lane).steps : first.steps;
-        const uint32_t mine = shared_length(p, steps, aligned) * p.c.heads, upTo = wave_prefix(mine);
+        const LaneSequence l = s0 ? lane_sequence(p, s0 + lane) : first;
+        const uint32_t mine = shared_length(p, l.steps, aligned) * blocks_of(p, l.q) * p.c.heads, upTo = wave_prefix(mine);
         const uint64_t past = __ballot(before + upTo > at);
         if (past || s0 + 64 >= p.b.sequences) {
             const uint32_t i = past ? (uint32_t)__ffsll((unsigned long long)past) - 1u : 63u;
@@ -453,8 +455,8 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bo
     }
 }
 
-// Up to 16 columns (rows of one sequence times query heads of one key/value
-// head) against steps [from, to) of their tokens: bound by the bytes of the
+// Up to 16 columns from col0 on (rows of one sequence times query heads of one
+// key/value head) against steps [from, to) of their tokens: bound by the bytes of the
 // cache.  Every wave takes each fourth 32-token tile straight into registers,
 // 8 KB of codes at head width 128, with the next tile in flight while it
 // works; keys and values need no exchange between lanes, so nothing passes
@@ -463,13 +465,18 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bo
 // of an 8B layer (675 MB of codes) take 123 us, 131072 tokens of one user (268
 // MB) 50 us: 5.4 to 5.5 TB/s, a large read's rate.
 template <int D, int P, int TERMS>
-ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t from, uint32_t to,
-                        bool complete, uint32_t part, float *lds) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
-    const uint32_t cols = (uint32_t)q.n * p.group;
-    const Spans w = spans_of(p, q, 0, cols - 1);
-    const int base = w.anyLo & ~63, begin = base + 64 * (int)from, end = min(w.anyHi, base + 64 * (int)to);
-    const Column c = column_of(p, q, h, min(n, cols - 1));
+ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t col0, uint32_t from,
+                        uint32_t to, bool complete, uint32_t part, float *lds) {
+    // what follows from the thread's index is formed for each unit: kept from one to the next, it takes registers
+    // that head width 256 needs for its tile
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const uint32_t lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
+    const uint32_t every = (uint32_t)q.n * p.group, cols = min(every - col0, 16u);
+    const Spans w = spans_of(p, q, col0, col0 + cols - 1);
+    const int base = column_of(p, q, h, 0).lo & ~63;  // the steps are those of all columns
+    const int begin = base + 64 * (int)from, end = min(w.anyHi, base + 64 * (int)to);
+    const Column c = column_of(p, q, h, col0 + min(n, cols - 1));
 
     // The tiles that all columns see whole go through a loop of their own, two
     // in registers at a time; the few others (ends, missing pages) follow one
@@ -564,10 +571,10 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
             o += *(const f32x4 *)(lds + (v * cols + col) * PITCH + d) * f;
         }
         if (complete) {
-            const Column k = column_of(p, q, h, col);
+            const Column k = column_of(p, q, h, col0 + col);
             store4(p, k.row, k.head, d, D, visible ? o * (1.0f / total) : f32x4{});
         } else {
-            const size_t at = (size_t)part * (p.b.maxRows * p.group) + col;
+            const size_t at = (size_t)part * 16 + col;
             if (visible) *(f32x4 *)(p.partO + at * D + d) = o;
             if (d == 0) {
                 p.partML[2 * at] = m;
@@ -581,9 +588,9 @@ template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
     if (p.shares == 0) {
-        const uint32_t s = blockIdx.x / H, h = blockIdx.x % H;
+        const uint32_t block = blockIdx.x % p.tiles, h = blockIdx.x / p.tiles % H, s = blockIdx.x / p.tiles / H;
         const LaneSequence l = lane_sequence(p, s);
-        if (l.steps) narrow_unit<D, P, TERMS>(p, s, l.q, h, 0, l.steps, true, 0, lds);
+        if (block < blocks_of(p, l.q)) narrow_unit<D, P, TERMS>(p, s, l.q, h, 16 * block, 0, l.steps, true, 0, lds);
         return;
     }
     const LaneSequence first = lane_sequence(p, lane);
@@ -593,19 +600,20 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     if (at >= last) return;
     uint32_t begins, s = sequence_at(p, first, sh.aligned, at, lane, begins);
     LaneSequence l = lane_sequence_at(p, first, s);
-    uint32_t length = shared_length(p, l.steps, sh.aligned), h = (at - begins) / length;
-    begins += h * length;
+    uint32_t length = shared_length(p, l.steps, sh.aligned), unit = (at - begins) / length;
+    begins += unit * length;
     while (true) {
         // a unit that begins here and goes on in later workgroups leaves its
         // sums in this one's second part, one that began earlier in its first
         const uint32_t from = at - begins, to = min(last - begins, l.steps);
-        narrow_unit<D, P, TERMS>(p, s, l.q, h, from, to, from == 0 && to == l.steps, 2 * blockIdx.x + (from == 0 ? 1u : 0u),
-                              lds);
+        const uint32_t blocks = blocks_of(p, l.q);
+        narrow_unit<D, P, TERMS>(p, s, l.q, unit / blocks, unit % blocks * 16, from, to, from == 0 && to == l.steps,
+                                 2 * blockIdx.x + (from == 0 ? 1u : 0u), lds);
         begins += length;
         at = begins;
         if (at >= last) return;
-        if (++h == H) {
-            h = 0;
+        if (++unit == H * blocks) {
+            unit = 0;
             do l = lane_sequence(p, ++s);
             while (l.steps == 0);
             length = shared_length(p, l.steps, sh.aligned);
@@ -1048,15 +1056,19 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
         return;
     }
     const Shares sh = shares_of(p, first, lane);
-    uint32_t before = lane < s ? shared_length(p, first.steps, sh.aligned) : 0;
-    for (uint32_t i = 64 + lane; i < s; i += 64) before += shared_length(p, lane_sequence(p, i).steps, sh.aligned);
+    uint32_t before = lane < s ? shared_length(p, first.steps, sh.aligned) * blocks_of(p, first.q) : 0;
+    for (uint32_t i = 64 + lane; i < s; i += 64) {
+        const LaneSequence b = lane_sequence(p, i);
+        before += shared_length(p, b.steps, sh.aligned) * blocks_of(p, b.q);
+    }
     before = wave_sum(before) * p.c.heads;
-    const uint32_t begins = before + head / p.group * shared_length(p, l.steps, sh.aligned);
+    const uint32_t col = (row - (uint32_t)q.row0) * p.group + head % p.group;
+    const uint32_t unit = head / p.group * blocks_of(p, q) + (col >> 4);
+    const uint32_t begins = before + unit * shared_length(p, l.steps, sh.aligned);
     const uint32_t w0 = begins / sh.quota, parts = (begins + l.steps - 1) / sh.quota - w0 + 1;
     if (parts == 1) return;  // one workgroup had it all and wrote it
-    const uint32_t cols = p.b.maxRows * p.group, col = (row - (uint32_t)q.row0) * p.group + head % p.group;
     join_parts<D>(p, parts, (int)row, head, lds, [&](uint32_t i) {
-        return (size_t)(2 * (w0 + i) + (i == 0 ? 1u : 0u)) * cols + col;
+        return (size_t)(2 * (w0 + i) + (i == 0 ? 1u : 0u)) * 16 + (col & 15u);
     });
 }
 

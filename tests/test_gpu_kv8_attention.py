@@ -126,6 +126,39 @@ def test_shared_evenly(ctx, d, P, hq, hkv, lens, rows, window):
     c.check(c.run(window=window), window=window)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("d,P,hq,hkv,lens,rows,window", [
+    (64, 16, 7, 1, [5000, 300, 0, 1800], [9, 2, 0, 5], 0), (128, 64, 8, 2, [6000, 2000], [16, 3], 0),
+    (256, 32, 8, 1, [3000, 900], [16, 16], 0), (128, 32, 24, 1, [4000, 40], [2, 2], 1500),
+    (64, 64, 3, 3, [9000, 70, 500], [21, 20, 1], 0), (256, 16, 4, 2, [2000], [32], 300), (128, 16, 17, 1, [2600, 17], [1, 3], 0),
+    (256, 64, 6, 2, [1100, 1064], [43, 5], 1)])
+def test_blocks_of_columns(ctx, d, P, hq, hkv, lens, rows, window, half):
+    """Several blocks of 16 columns to a sequence and head, the last one short, in shares that begin and end inside them."""
+    c = Case(ctx, d + P + hq, lens, rows, P, d, hq, hkv, behind=1)
+    c.check(c.run(half, window), half, window)
+
+
+def test_blocks_of_many_sequences(ctx):
+    """Sequences with one to four blocks of columns among each other, some empty, more of them than a wave has lanes."""
+    rng = np.random.default_rng(70)
+    for most in (600, 2500):
+        lens = [int(x) for x in rng.integers(0, most, 70)]
+        lens[3], lens[69] = 0, most
+        rows = [min(n, int(x)) for n, x in zip(lens, rng.integers(0, 21, 70))]
+        c = Case(ctx, 71, lens, rows, 64, 64, 6, 2)
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("d,P,hq,hkv,lens,rows,window", [
+    (256, 16, 8, 1, [1700, 130], [30, 1], 0), (256, 64, 4, 2, [2500, 90], [70, 90], 900), (256, 32, 4, 1, [100, 65], [40, 33], 0),
+    (256, 32, 4, 1, [100, 65], [40, 33], 30), (128, 64, 20, 1, [2000, 700], [4, 1], 0)])
+def test_many_columns(ctx, d, P, hq, hkv, lens, rows, window, half):
+    """More columns than are taken 16 at a time."""
+    c = Case(ctx, d + P + hq, lens, rows, P, d, hq, hkv)
+    c.check(c.run(half, window), half, window)
+
+
 @pytest.mark.parametrize("many", [150, 64, 65])
 def test_shared_between_many_sequences(ctx, many):
     """More sequences than a wave has lanes, some of them empty, in aligned and in even shares."""
@@ -189,7 +222,7 @@ def test_blocks_of_very_different_scales(ctx, hq, hkv, rows):
     assert np.all(np.abs(got - exp) <= tol)
 
 
-@pytest.mark.parametrize("rows", [[1, 1], [6, 3], [80, 40]])
+@pytest.mark.parametrize("rows", [[1, 1], [6, 3], [25, 10], [80, 40]])
 @pytest.mark.parametrize("hq,hkv", [(2, 1), (4, 4)])
 def test_non_finite_places(ctx, hq, hkv, rows):
     """NaN codes in keys and values of hidden tokens (later ones, ones before the window, bytes behind the last) leave a row
@@ -319,8 +352,15 @@ def test_workspace_covers_every_window(ctx):
             c.check(got, window=window)
 
 
+@pytest.mark.parametrize("rows", [20, 90])
+def test_workspace_covers_every_window_of_many_rows(ctx, rows):
+    c = Case(ctx, 13, [3000], [rows], 16, 64, 2, 1)
+    for window in (0, 1, 64, 65, 500, 1025, 2900, 3000, 2 ** 32 - 1):
+        c.check(c.run(window=window), window=min(window, 3000))
+
+
 def test_repeats_are_the_same_bits(ctx):
-    for rows, hq in (([1, 1], 4), ([90, 30], 4), ([1, 1], 40)):
+    for rows, hq in (([1, 1], 4), ([90, 30], 4), ([1, 1], 40), ([20, 7], 4)):
         c = Case(ctx, 14, [1500, 700], rows, 64, 128, hq, 2)
         first = c.run()
         for _ in range(3):
@@ -329,7 +369,7 @@ def test_repeats_are_the_same_bits(ctx):
 
 def test_captured_and_replayed_with_later_lengths(ctx):
     """A recorded call follows the lengths and tables of its replay; eager work stands between the replays."""
-    for rows, hq in (([1, 1], 4), ([20, 10], 2)):
+    for rows, hq in (([1, 1], 4), ([20, 10], 2), ([32, 30], 4)):
         c = Case(ctx, 15, [900, 300], rows, 16, 64, hq, 1)
         c.upload()
         batch = c.b.upload(ctx)
@@ -376,7 +416,7 @@ def test_two_streams_with_their_own_workspaces(ctx):
         st.destroy()
 
 
-@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("rows", [1, 30, 80])
 def test_cache_beyond_32_bits(ctx, rows):
     """A sequence in the last pages of a pool of more than 2^32 code bytes."""
     P, d, heads = 64, 256, 2
