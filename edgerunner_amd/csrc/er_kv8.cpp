@@ -443,7 +443,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     if (p.narrow)
         st = launch(kernels.narrow[di][a.c.shift - 4][a.half], op, p.shares ? p.shares : pairs * p.tiles, 0, stream, &a);
     else
-        st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, ((pairs * p.splits + 7) & ~7ull) * p.tiles, 0, stream, &a);
+        st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, pairs * p.splits * p.tiles, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
     if (!p.shares && p.splits <= 16) return launch(kernels.joinRow[di], op, batch->rows, 0, stream, &a);
     const uint32_t most = p.shares ? p.shares : p.splits;

@@ -828,13 +828,15 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
 // long prefixes in fp32 (two terms, 35 GFLOP of products) 79 us with the join.
 template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
-    // units (sequence, head, piece) are dealt over a multiple of 8 workgroups,
-    // and workgroups to the 8 XCDs in turn, so that one XCD's L2 serves all
-    // row tiles of a unit; later row tiles see more tokens and start first
-    const uint32_t units = p.b.sequences * p.c.heads * p.splits, dealt = (units + 7u) & ~7u;
-    const uint32_t unit = blockIdx.x % dealt, tile = p.tiles - 1 - blockIdx.x / dealt;
-    if (unit >= units) return;
-    const uint32_t piece = unit % p.splits, h = (unit / p.splits) % p.c.heads, s = unit / p.splits / p.c.heads;
+    // One row tile of all units (sequence, piece, head) after the other, each
+    // begun a sequence's heads later than the one before.  Workgroups go to the
+    // 8 XCDs in turn: with 8 heads (or 16, ..) an XCD's L2 serves all tiles of a
+    // head, with fewer a head's tiles lie on several, and units of very
+    // different lengths load all XCDs alike.  Later tiles see more, and start first.
+    const uint32_t units = p.b.sequences * p.splits * p.c.heads, round = blockIdx.x / units;
+    const uint32_t ahead = round % (p.b.sequences * p.splits) * p.c.heads, at = blockIdx.x % units;
+    const uint32_t unit = at >= ahead ? at - ahead : at + units - ahead, tile = p.tiles - 1 - round;
+    const uint32_t h = unit % p.c.heads, piece = unit / p.c.heads % p.splits, s = unit / p.c.heads / p.splits;
     const Sequence q = sequence_of(p.b, s);
     const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * 128;
     if (col0 >= cols) return;
