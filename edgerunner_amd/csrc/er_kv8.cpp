@@ -234,7 +234,6 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
     p.narrow = cols <= (c->head_dim == 256 ? 128 : 64);
     p.splits = 1;
-    const uint64_t pairs = (uint64_t)b->sequences * c->kv_heads;
     if (p.narrow) {
         // two workgroups a CU are resident; a workgroup's start and its part in the join cost as much as some
         // hundred tokens, so none takes fewer than that, and what a workgroup
@@ -252,19 +251,29 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     uint64_t span = full;
     // the tile's rows see window + rows - 1 tokens, and pieces begin at a multiple of 64
     if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
-    // the tokens of a (sequence, head, row tile) are cut into pieces where
-    // those alone are too few workgroups: to four a CU, as rows and lengths
-    // are ragged (chunks of three prompts, kernel and join: 83 + 8 us in five
-    // pieces, 97 + 6 in three, 73 + 30 in 17), of 256 tokens at the least
-    const uint64_t units = pairs * p.tiles, want = (uint64_t)cu * 4, least = 256;
-    auto pieces = [&](uint64_t tokens) {
-        return std::max<uint64_t>(1, std::min<uint64_t>((want + units - 1) / units, (tokens + least - 1) / least));
+    // The tokens of a (sequence, head, row tile) are cut into as many pieces as
+    // make one workgroup for each that the chip holds, of 256 tokens at the
+    // least: fewer leave it empty, more have more sums to join (a chunk of 256
+    // rows behind 60000 tokens in 8 pieces a tile 458 us, in 12 484, in 16 481;
+    // three ragged chunks in 5, 7 and 10 pieces 79, 65 and 71; a prompt of 4096
+    // rows of 8 heads in one and two 181 and 267).  Of a prompt's pieces half
+    // lie behind its rows, and of several sequences one eighth behind their ends.
+    const uint64_t resident = (uint64_t)cu * (c->head_dim == 64 ? 3 : c->head_dim == 128 ? 2 : 1);
+    const uint64_t filled = std::max<uint64_t>(1, ((uint64_t)b->rows * group + 64ull * b->sequences) / 128);
+    const uint64_t units = c->kv_heads * std::min(filled, (uint64_t)b->sequences * p.tiles);
+    auto pieces = [&](uint64_t tokens, bool windowed) {
+        const double rows = (double)std::min<uint64_t>(b->max_rows, full), length = (double)std::max<uint64_t>(1, full);
+        double seen = windowed ? 1.0 : 1.0 - 0.5 * rows / length;
+        if (b->sequences > 1) seen *= 0.875;
+        const uint64_t even = (uint64_t)((double)resident / ((double)units * seen) + 0.5);
+        return std::max<uint64_t>(1, std::min<uint64_t>(even, (tokens + 255) / 256));
     };
-    const uint64_t splits = pieces(span);
+    const uint64_t splits = pieces(span, span < full);
     p.chunk = (uint32_t)std::max<uint64_t>(64, ((span + splits - 1) / splits + 63) & ~63ull);
     p.splits = (uint32_t)std::max<uint64_t>(1, (span + p.chunk - 1) / p.chunk);
-    // pieces(span) grows with the span, and rounding pieces up to 64 tokens only takes some away
-    if (pieces(full) > 1) p.parts = pieces(full) * b->rows * group * c->kv_heads;
+    // no window has more pieces than the whole length, and rounding them up to 64 tokens only takes some away
+    const uint64_t most = pieces(full, false);
+    if (most > 1) p.parts = most * b->rows * group * c->kv_heads;
     return p;
 }
 

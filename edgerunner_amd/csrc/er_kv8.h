@@ -65,7 +65,8 @@ struct ErAttendArgs {
     uint32_t qStride, outStride;
     uint32_t group;           // query heads of one key/value head
     // narrow kernel: workgroups that share the tokens of all sequences evenly,
-    // at least `least` 64-token steps each (0: a workgroup a sequence and head)
+    // at least `least` 64-token steps each (0: a workgroup a
+    // sequence, head and block of 16 columns)
     uint32_t shares, least;
     // wide kernel: pieces of a row tile's tokens, tokens of a piece (a multiple
     // of 64), row tiles of a sequence and key/value head (narrow kernel: blocks

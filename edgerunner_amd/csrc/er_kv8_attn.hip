@@ -825,7 +825,7 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
 // operands: codes are half the LDS traffic of fp16, and leave more registers
 // (fp16 in LDS spilled at head width 256).  A 4096-token prompt of an 8B layer
 // (137 GFLOP) takes 184 us, 746 TFLOP/s, two waves a SIMD; ragged chunks behind
-// long prefixes in fp32 (two terms, 35 GFLOP of products) 79 us with the join.
+// long prefixes in fp32 (two terms, 35 GFLOP of products) 72 us with the join.
 template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // One row tile of all units (sequence, piece, head) after the other, each
