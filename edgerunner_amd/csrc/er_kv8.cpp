@@ -225,10 +225,10 @@ struct AttendPlan {
 // narrow one reads the cache once for each 16 of them, the wide one once for
 // 128, with products that pay for columns that are not there, and with less
 // work split between fewer workgroups.  Measured narrow / wide, us: 24 columns
-// of 4 sequences of 30000 tokens 26 / 38, 32 of 16 of 8000 59 / 86 (head width
-// 256: 64 / 180), 60 of 16 of 4000 25 / 56, 128 of 4 of 8000 51 / 55, 128 of 16
-// of 4000 98 / 97, and for bf16, whose wide kernel has half the products, 96 /
-// 84; 256 columns 174 / 101.
+// of 4 sequences of 30000 tokens 27 / 37, 32 of 16 of 8000 in bf16 59 / 85, 60
+// of 16 of 4000 25 / 56, but 128 of 4 of 8000 51 / 43 and of 16 of 4000 98 / 73.
+// At head width 256 the wide one has a wave a SIMD: 32 of 16 of 8000 63 / 166,
+// 100 of 8 of 4000 50 / 63.
 AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group, uint32_t window, int cu) {
     AttendPlan p{};
     const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
