@@ -238,7 +238,7 @@ template <int D>
 struct NarrowState {
     f32x4 o[D / 16];  // o[j][i]: value (4 g + i) D/16 + j of column n
     float m, l;       // reference; this lane's part of the sum of weights
-    float vref, vinv; // the largest value scale so far: o is in units of vref / 128; 128 / vref (wave-uniform)
+    float vref, vinv; // reference of the value scales: o is in units of vref / 128; 128 / vref (wave-uniform)
     bool seen;        // a token was visible to the column
     bool nans;        // a masked tile held NaN codes
 };
@@ -261,7 +261,7 @@ ER_DEV void raise_reference(float to, float &m, float &l, ACC (&o)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] *= f;
 }
-// Moves the value scales' reference up to a tile's largest.
+// Moves the value scales' reference.
 template <int N, typename ACC>
 ER_DEV void raise_scale(float to, float &vref, float &vinv, ACC (&o)[N]) {
     const float f = vref / to;
@@ -271,14 +271,41 @@ ER_DEV void raise_scale(float to, float &vref, float &vinv, ACC (&o)[N]) {
     for (int j = 0; j < N; ++j) o[j] *= f;
 }
 
+// Value scales as integers, which order as the (positive) floats do.  More than
+// 2^22 below the reference, a part's smallest codes fall below fp16's.
+#define ER_SCALE_APART (22u << 23)
+struct ScaleRange {
+    uint32_t most, least;  // of the parts that are there; least: of those that are not 0, less one
+    __device__ __forceinline__ void add(uint32_t scale) {
+        most = max(most, scale);
+        least = min(least, scale - 1u);
+    }
+    __device__ __forceinline__ bool apart() const { return most > least && most - least > ER_SCALE_APART; }
+};
+// Moves the reference of the value scales for the parts at hand: up to the
+// largest; and down to it where one lies too far below, since the reference may
+// stem from tokens that only others of the wave's columns see.  Sums, at most
+// 2^61, are rescaled exactly: by at most 2^60 below the largest reference, `top`.
+template <int N, typename ACC>
+ER_DEV void follow_scale(const ScaleRange &r, float &top, float &vref, float &vinv, ACC (&o)[N]) {
+    const uint32_t ref = __float_as_uint(vref);
+    const bool up = r.most > ref, down = r.most < ref && ref > ER_SCALE_APART && r.least < ref - ER_SCALE_APART;
+    if (!up && !down) return;
+    const float to = fmaxf(__uint_as_float(r.most), top * 0x1p-60f);
+    top = fmaxf(top, to);
+    raise_scale(to, vref, vinv, o);
+}
+
 // One tile into the state.  MASKED: some column does not see all of it, or a
 // page is missing.  Hidden tokens get the score -inf there, and those that no
 // column sees have their bytes taken as zeros, whatever they hold.  NaN codes
 // count as zeros too, since a column may not see them and 0 * NaN is NaN:
 // st.nans remembers that there were some, and mark_nans brings them back.
+// vtop: the largest reference of the value scales, for masked tiles, which come
+// last.
 template <int D, int TERMS, bool MASKED>
 ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
-                          int lo, int hi, const Spans &w, uint32_t g) {
+                          int lo, int hi, const Spans &w, uint32_t g, float &vtop) {
     const bool ok0 = !MASKED || t.page[0] >= 0, ok1 = !MASKED || t.page[1] >= 0;
     f32x4 s[2];
 #pragma unroll
@@ -314,7 +341,14 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
                             fmaxf(fmaxf(s[1].x, s[1].y), fmaxf(s[1].z, s[1].w)) * f1);
     if (__any(top > st.m + 8.0f)) raise_reference(fmaxf(st.m, column_max4(top)), st.m, st.l, st.o);
     const float vs0 = ok0 ? t.vs[0] : t.vs[1], vs1 = ok1 ? t.vs[1] : t.vs[0];
-    if (fmaxf(vs0, vs1) > st.vref) raise_scale(fmaxf(vs0, vs1), st.vref, st.vinv, st.o);
+    if constexpr (MASKED) {
+        ScaleRange r = {0u, ~0u};
+        r.add(__float_as_uint(uniform(vs0)));
+        r.add(__float_as_uint(uniform(vs1)));
+        follow_scale(r, vtop, st.vref, st.vinv, st.o);
+    } else if (fmaxf(vs0, vs1) > st.vref) {
+        raise_scale(fmaxf(vs0, vs1), st.vref, st.vinv, st.o);
+    }
     const float v0 = vs0 * st.vinv, v1 = vs1 * st.vinv, m7 = st.m - 7.0f;
     float x[8];
 #pragma unroll
@@ -503,33 +537,48 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
                                                p.scale, 16 * g, 64, 8, qb, column_max4);
     NarrowState<D> st = {};
+    float vtop = 0.0f;
     st.m = ER_NO_MAX;
     if constexpr (D < 256) {
         while (T < end) {
             if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
             T = next_whole(U + 128);
-            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
             if (U >= end) break;
             if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
             U = next_whole(T + 128);
-            attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g);
+            attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g, vtop);
         }
     } else {
         // 16 KB a tile: one in registers, and twice the waves; the first waits
         // until the query's fp32 values have left theirs
         if (T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
         while (T < end) {
-            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g);
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
             T = U;
             if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
             U = next_whole(T + 128);
         }
     }
-    for (T = rest; T < end; T += 128) {
+    vtop = st.vref;  // it has only gone up
+    bool second = false;  // of a tile whose halves' value scales lie far apart: a column may see the small one alone
+    for (T = rest; T < end;) {
         pages = narrow_pages<P>(p, s, T, w.anyLo, end);
-        if (whole(pages, T) || (pages.page[0] < 0 && pages.page[1] < 0)) continue;
-        load_narrow<D, P>(t0, pages, p, h, T, n, g);
-        attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g);
+        if (!whole(pages, T) && (pages.page[0] >= 0 || pages.page[1] >= 0)) {
+            load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            if constexpr (P < 32) {
+                ScaleRange r = {0u, ~0u};
+                r.add(__float_as_uint(uniform(t0.vs[0])));
+                r.add(__float_as_uint(uniform(t0.vs[1])));
+                if (pages.page[0] >= 0 && pages.page[1] >= 0 && r.apart()) {
+                    t0.page[0] = second ? -1 : t0.page[0];
+                    t0.page[1] = second ? t0.page[1] : -1;
+                    second = !second;
+                }
+            }
+            attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g, vtop);
+        }
+        if (!second) T += 128;
     }
     // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
     if (__any(st.nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, g);
@@ -632,14 +681,24 @@ struct WidePages {
     static constexpr int N = ER_WIDE_TOKENS / P;
     int page[N];
     float ks[N], vs[N];
-    // all of the tile is there
-    __device__ __forceinline__ bool all() const {
-        bool r = true;
-#pragma unroll
-        for (int i = 0; i < N; ++i) r &= page[i] >= 0;
-        return r;
-    }
 };
+// What the products need of them: a bit for each part that is there, and the scales (values' as integers, 0 where it is not).
+template <int P>
+struct WideParts {
+    static constexpr uint32_t ALL = (1u << WidePages<P>::N) - 1u;
+    uint32_t there, vs[WidePages<P>::N];
+    float ks[WidePages<P>::N];
+};
+template <int P>
+ER_DEV void parts_of(WideParts<P> &r, const WidePages<P> &w) {
+    r.there = 0;
+#pragma unroll
+    for (int i = 0; i < w.N; ++i) {
+        r.there |= (w.page[i] >= 0 ? 1u : 0u) << i;
+        r.ks[i] = w.ks[i];
+        r.vs[i] = w.page[i] >= 0 ? __float_as_uint(w.vs[i]) : 0u;
+    }
+}
 template <int D, int P>
 struct WideTile {
     u32x4 k[D / 64];                       // token tid / 4, bytes [(tid & 3) D/4, + D/4)
@@ -683,16 +742,16 @@ ER_DEV WidePages<P> pages_at(PageWindow<P> &w, const ErAttendArgs &p, uint32_t s
 }
 
 // Entry of a tile's 16-token part, without an address (which would put v into scratch memory).
-template <int N>
-ER_DEV int of_part(const int (&v)[N], uint32_t part) {
+template <int N, typename T>
+ER_DEV T of_part(const T (&v)[N], uint32_t part) {
     if constexpr (N == 1) {
         return v[0];
     } else if constexpr (N == 2) {
-        const int a = v[0], b = v[1];
+        const T a = v[0], b = v[1];
         return part & 2u ? b : a;
     } else {
-        const int a = v[0], b = v[1], c = v[2], d = v[3];
-        const int x = part & 1u ? b : a, y = part & 1u ? d : c;
+        const T a = v[0], b = v[1], c = v[2], d = v[3];
+        const T x = part & 1u ? b : a, y = part & 1u ? d : c;
         return part & 2u ? y : x;
     }
 }
@@ -748,19 +807,19 @@ struct WideLds {
 };
 
 // The values of a tile that some column of the workgroup does not see whole,
-// as attend_narrow's masked tiles; true where there were NaN codes.
+// as attend_narrow's masked tiles; not 0 where there were NaN codes.
 template <int D, int P>
-ER_DEV bool mask_wide(WideTile<D, P> &t, const WidePages<P> &w, int T, int lo, int hi, uint32_t tid) {
-    bool nan = false;
+ER_DEV uint32_t mask_wide(WideTile<D, P> &t, uint32_t there, int T, int lo, int hi, uint32_t tid) {
+    uint32_t nan = 0;
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
         const ValueItem it = value_item<D>(tid, r);
-        const bool ok = of_part(w.page, it.part) >= 0;
+        const bool ok = there >> 16 * it.part / P & 1u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
             const uint32_t c = ok && tok >= lo && tok < hi ? t.v[r][i] : 0u, nans = nan_codes(c);
-            nan |= nans != 0;
+            nan |= nans;
             t.v[r][i] = c & ~nans;
         }
     }
@@ -825,7 +884,7 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
 // operands: codes are half the LDS traffic of fp16, and leave more registers
 // (fp16 in LDS spilled at head width 256).  A 4096-token prompt of an 8B layer
 // (137 GFLOP) takes 184 us, 746 TFLOP/s, two waves a SIMD; ragged chunks behind
-// long prefixes in fp32 (two terms, 35 GFLOP of products) 72 us with the join.
+// long prefixes in fp32 (two terms, 35 GFLOP of products) 75 us with the join.
 template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // One row tile of all units (sequence, piece, head) after the other, each
@@ -850,54 +909,71 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
 
     f32x16 o[D / 32] = {};  // o[d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n, in units of vref / 128
-    float m = ER_NO_MAX, l = 0.0f, vref = 0.0f, vinv = 0.0f;
-    bool seen = false;
+    float m = ER_NO_MAX, l = 0.0f, vref = 0.0f, vinv = 0.0f, vtop = 0.0f;
+    uint32_t seen = 0;  // not a mask, which would take two scalar registers
     if (begin < end) {
         WideTile<D, P> t;
         PageWindow<P> window;
         fill_window<P>(window, p, s, h, begin, w.anyLo, end, lane);
-        WidePages<P> now = pages_at<P>(window, p, s, h, begin, w.anyLo, end, lane);  // of the tile in `t`
-        load_wide<D, P>(t, now, p, h, tid);
+        // The next tile to load, and the one in `t`.  A tile that not all columns see
+        // whole, and whose parts' value scales lie far apart, is taken part by part (`part`: a bit), since a column may see
+        // the small ones alone.
+        int next = begin, at = begin;
+        uint32_t part = 0;
+        WideParts<P> now;
+        auto fetch = [&]() {
+            at = next;
+            if (next >= end) return;
+            WidePages<P> pages = pages_at<P>(window, p, s, h, next, w.anyLo, end, lane);
+            parts_of(now, pages);
+            if constexpr (P < 64) {
+                ScaleRange range = {0u, ~0u};
+#pragma unroll
+                for (int i = 0; i < pages.N; ++i) range.add(now.vs[i]);
+                if (range.apart() && !(now.there == now.ALL && next >= w.allLo && next + 64 <= w.allHi)) {
+                    part = max(part, 1u);
+#pragma unroll
+                    for (int i = 0; i < pages.N; ++i) pages.page[i] = part >> i & 1u ? pages.page[i] : -1;
+                    parts_of(now, pages);
+                    part = part <= now.ALL / 2 ? part << 1 : 0u;
+                }
+            }
+            load_wide<D, P>(t, pages, p, h, tid);
+            if (part == 0) next += 64;
+        };
+        fetch();
         h8 qb[TERMS][D / 16];
         const float qf = load_query<D / 16, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, live, p.scale,
                                                    16 * hh, 32, 8, qb, column_max2);
-        bool nans = false;
-        auto whole = [&](const WidePages<P> &k, const Spans &w, int T) {
-            return k.all() && T >= w.allLo && T + 64 <= w.allHi;
+        uint32_t nans = 0;
+        auto whole = [&](const WideParts<P> &k, const Spans &w, int T) {
+            return k.there == k.ALL && T >= w.allLo && T + 64 <= w.allHi;
         };
-        if (!whole(now, w, begin)) nans |= mask_wide<D, P>(t, now, begin, w.anyLo, end, tid);
-        store_wide<D, P>(lds[0], t, tid);
-        WidePages<P> parts = now;
-        if (begin + 64 < end) {
-            now = pages_at<P>(window, p, s, h, begin + 64, w.anyLo, end, lane);
-            load_wide<D, P>(t, now, p, h, tid);
-        }
-        auto bring = [&](uint32_t to, int T) {  // the tile in `t`, which lies at T, into LDS
-            if (!whole(now, w, T)) nans |= mask_wide<D, P>(t, now, T, w.anyLo, end, tid);
+        auto bring = [&](uint32_t to) {  // the tile in `t` into LDS
+            if (!whole(now, w, at)) nans |= mask_wide<D, P>(t, now.there, at, w.anyLo, end, tid);
             store_wide<D, P>(lds[to], t, tid);
         };
-        auto fetch = [&](int T) {
-            now = pages_at<P>(window, p, s, h, T, w.anyLo, end, lane);
-            load_wide<D, P>(t, now, p, h, tid);
-        };
+        bring(0);
+        int T = at;
+        WideParts<P> parts = now;
+        fetch();
         uint32_t buf = 0;
         // a wave without columns only brings its part of the tiles
-        for (int T = begin; idle && T < end; T += 64, buf ^= 1u) {
+        for (; idle && T < end; buf ^= 1u) {
             __syncthreads();
-            if (T + 64 < end) bring(buf ^ 1u, T + 64);
-            if (T + 128 < end) fetch(T + 128);
+            if (at < end) bring(buf ^ 1u);
+            T = at;
+            fetch();
         }
-        for (int T = begin; !idle && T < end; T += 64, buf ^= 1u) {
+        for (; T < end; buf ^= 1u) {
             __syncthreads();
             const WideLds<D> &in = lds[buf];
             const bool clear = whole(parts, ww, T);
             seen |= clear;
-            // the value scales' reference; positive floats order as their bits, which scalar registers compare
-            uint32_t most = __float_as_uint(vref);
+            ScaleRange range = {0u, ~0u};
 #pragma unroll
-            for (int i = 0; i < parts.N; ++i)
-                most = parts.page[i] >= 0 ? max(most, __float_as_uint(parts.vs[i])) : most;
-            if (most > __float_as_uint(vref)) raise_scale(__uint_as_float(most), vref, vinv, o);
+            for (int i = 0; i < WidePages<P>::N; ++i) range.add(parts.vs[i]);
+            follow_scale(range, vtop, vref, vinv, o);
 #pragma unroll
             for (int th = 0; th < 2; ++th) {
                 f32x16 sc = {};
@@ -911,13 +987,13 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                         sc = mfma32(a1, qb[term][2 * j + 1], sc);
                     }
                 }
-                if (th == 1 && T + 64 < end) bring(buf ^ 1u, T + 64);
+                if (th == 1 && at < end) bring(buf ^ 1u);
                 if (!clear) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int tok = T + 32 * th + 8 * (i >> 2) + 4 * (int)hh + (i & 3);
-                        const bool shown = parts.page[(32 * th + 16 * (i >> 3)) / P] >= 0 && tok >= c.lo && tok < c.hi;
-                        seen |= shown;
+                        const bool shown = (parts.there >> (32 * th + 16 * (i >> 3)) / P & 1u) && tok >= c.lo && tok < c.hi;
+                        seen |= shown ? 1u : 0u;
                         sc[i] = shown ? sc[i] : -__builtin_inff();
                     }
                 }
@@ -925,9 +1001,9 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int e = (32 * th + 16 * i) / P;
-                    const bool there = parts.page[e] >= 0;  // a missing page's values are zeros: any finite scale does
-                    f[i] = score_factor(qf, there ? parts.ks[e] : 1.0f);
-                    v[i] = there ? parts.vs[e] * vinv : 1.0f;
+                    const bool here = parts.there >> e & 1u;  // a missing part's values are zeros: any finite scale does
+                    f[i] = score_factor(qf, here ? of_part(parts.ks, 2 * th + i) : 1.0f);
+                    v[i] = here ? __uint_as_float(of_part(parts.vs, 2 * th + i)) * vinv : 1.0f;
                     float peak = sc[8 * i];
 #pragma unroll
                     for (int j = 1; j < 8; ++j) peak = fmaxf(peak, sc[8 * i + j]);
@@ -958,13 +1034,14 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                     }
                 }
             }
+            T = at;
             parts = now;
-            if (T + 128 < end) fetch(T + 128);
+            fetch();
         }
-        if (__syncthreads_or(nans)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);
+        if (__syncthreads_or(nans != 0)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);
     }
     l = column_sum2(l);
-    seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f;
+    seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f ? 1u : 0u;
     if (!live) return;
     const float f = p.splits == 1 ? vref * 0.0078125f / l : vref * 0.0078125f;
     const size_t to = part_index(p, piece, c.row, c.head);

@@ -512,8 +512,8 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
  * the batch's and cache's sizes and q_heads alone), 16-byte aligned; calls and
  * recorded graphs that may overlap in time need one each.  q->heads is a
  * multiple of kv_heads, at most 1024 a key/value head.  A block of values whose
- * scale is less than 2^-22 of the largest that a row's tokens have is rounded to
- * fewer bits.  Errors as er_hip_kv8_append's. */
+ * scale is less than 2^-22 of the largest that a row's tokens have, or 2^-82 of
+ * the largest that its sequence's other rows of the call have, is rounded to fewer bits.  Errors as er_hip_kv8_append's. */
 er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
                                const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
                                uint32_t out_type, float scale, uint32_t window, er_buffer workspace);
