@@ -506,7 +506,8 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
  * window where window is not 0) of its sequence and key/value head h /
  * (q->heads / kv_heads), w = softmax(scale * q . k_t).  q fp32; out of
  * out_type ER_TYPE_F32 (products of fp32 accuracy) or ER_TYPE_BF16 (queries
- * and weights rounded to fp16 for the products).  A row that no token is
+ * and weights rounded to fp16 for the products); either holds a weight to
+ * 2^-38 of its row's largest.  A row that no token is
  * visible to gets zeros.  out does not overlap q.
  * workspace: scratch of er_hip_kv8_attention_workspace bytes (which depend on
  * the batch's and cache's sizes and q_heads alone), 16-byte aligned; calls and

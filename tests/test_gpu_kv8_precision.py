@@ -1,6 +1,8 @@
 """Where the operators between the projections could lose bits, against 64-bit forms."""
+import numpy as np
 import pytest
 
+from edgerunner_amd import HeadRows, KV8AttentionKernel, KV8Batch, KV8Cache
 from test_gpu_kv8_attention import Case
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +34,34 @@ def test_scales_of_hidden_values(ctx, d, P, hq, hkv, lens, rows, window, every, 
     c = Case(ctx, d + P + ratio, lens, rows, P, d, hq, hkv)
     page_scales(c, lambda p: ratio - 5 if p % every == first else p % 4 - 6)
     c.check(c.run(half, window), half, window)
+
+
+# Weights are held as two fp16 terms of up to 2^15 for the largest of a row and 2^13 at the least, so one of 2^-33 of the
+# largest is 2^-20 there at the least, off by at most half of fp16's smallest step, 2^-25
+@pytest.mark.parametrize("seqs,rows", [(512, 1), (800, 80)])
+def test_long_tail_of_small_weights(ctx, seqs, rows):
+    """Four tokens with a score 33 powers of two above those of 2^18 others, whose values make up the whole output."""
+    d, P, n = 64, 64, 1 << 18
+    kc, vc = np.zeros((2, 1, P, d), np.uint8), np.full((2, 1, P, d), 0x38, np.uint8)  # 0x38: 1
+    kc[..., 0] = 0xb8  # -1
+    for t in (0, 32):
+        kc[0, 0, t], vc[0, 0, t] = 0, 0
+    table = np.ones((seqs, n // P), np.int32)
+    table[:, :2] = 0
+    total = seqs * rows
+    q = np.zeros((total, d), np.float32)
+    q[:, 0] = 33
+    ones = np.ones((2, 1), np.float32)
+    cache = KV8Cache(*[ctx.upload(a) for a in (kc, vc, ones, ones)], 2, 1, P, d)
+    batch = KV8Batch(ctx.upload(table), ctx.upload(np.full(seqs, n, np.int32)),
+                     ctx.upload(np.arange(seqs + 1, dtype=np.int32) * rows), seqs, n // P, total, rows, n)
+    kern = KV8AttentionKernel(ctx)
+    ws = ctx.alloc(max(16, kern.workspaceBytes(cache, batch, 1)))
+    ob = ctx.alloc(4 * q.size)
+    kern.encode(None, cache, batch, HeadRows(ctx.upload(q), 1, d), HeadRows(ob, 1, d), float(np.log(2.0)), workspace=ws)
+    ctx.synchronize()
+    got = ob.download(np.float32).reshape(seqs, rows, d)
+    tail = (n - rows + np.arange(rows) + 1 - 4) * 2.0 ** -33
+    exp = (tail / (4 + tail))[None, :, None]
+    # beside the terms: 33 * 2^-23 of the exponent, and sums of fp32
+    assert np.all(np.abs(got - exp) <= exp * (2.0 ** -5 + 2.0 ** -8))
