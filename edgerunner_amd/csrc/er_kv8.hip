@@ -98,18 +98,20 @@ ER_DEV Pairs load_pairs(const float *p, const PairPlace &pl) {
     return to_pairs(lo, hi, pl.neighbours);
 }
 
-// cos and sin of a fraction of a turn, |x| <= 1/2: the nearest quarter turn is
-// taken off exactly, and the Taylor series of the rest, |a| <= pi / 4, end
-// where their next terms are below 2^-25 (a^11 / 11! and a^10 / 10!).  About
-// half the instructions of two library calls, which reduce each on its own.
-ER_DEV void cos_sin_turn(float x, float &c, float &s) {
-    const float q = rintf(4.0f * x);
-    const float a = (x - 0.25f * q) * 6.283185307f, z = a * a;
+// cos and sin of a fraction of a turn, |x| <= 1/2.  The nearest quarter turn is taken off
+// exactly, in 64 bits, and the angle that is left, |a| <= pi / 4, rounded once
+// to fp32 (2^-25); the Taylor series end where their next terms are below
+// 2^-28 (a^11 / 11! and a^12 / 12!).  At most 7e-8 off; about half the
+// instructions of two library calls, which reduce each on its own.
+ER_DEV void cos_sin_turn(double x, float &c, float &s) {
+    const double q = rint(4.0 * x);
+    const float a = (float)((x - 0.25 * q) * 6.283185307179586477), z = a * a;
     float sn = __builtin_fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
     sn = __builtin_fmaf(z, sn, 8.3333333e-3f);
     sn = __builtin_fmaf(z, sn, -1.6666667e-1f);
     sn = __builtin_fmaf(a * z, sn, a);
-    float cs = __builtin_fmaf(z, 2.4801587e-5f, -1.3888889e-3f);
+    float cs = __builtin_fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+    cs = __builtin_fmaf(z, cs, -1.3888889e-3f);
     cs = __builtin_fmaf(z, cs, 4.1666667e-2f);
     cs = __builtin_fmaf(z, cs, -0.5f);
     cs = __builtin_fmaf(z, cs, 1.0f);
@@ -120,9 +122,8 @@ ER_DEV void cos_sin_turn(float x, float &c, float &s) {
 }
 
 // The four pairs' frequencies in turns, and their cos and sin at a position.
-// position * frequency is formed and brought to a fraction of a turn in 64
-// bits (at position 10^6 an fp32 product is off by 0.03 rad); the fraction goes
-// to fp32, off by at most 2^-25 turns.
+// position * frequency is formed and reduced in 64 bits (at position 10^6 an
+// fp32 product is off by 0.03 rad).
 struct Frequencies {
     double f[4];
     bool on;
@@ -148,7 +149,7 @@ ER_DEV Turns turns_of(int position, const Frequencies &f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const double turn = (double)position * f.f[i];
-            cos_sin_turn((float)(turn - rint(turn)), t.c[i], t.s[i]);
+            cos_sin_turn(turn - rint(turn), t.c[i], t.s[i]);
         }
     }
     return t;

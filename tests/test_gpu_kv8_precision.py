@@ -2,7 +2,9 @@
 import numpy as np
 import pytest
 
-from edgerunner_amd import HeadRows, KV8AttentionKernel, KV8Batch, KV8Cache
+import kv8_ref as R
+from edgerunner_amd import HeadRows, KV8AttentionKernel, KV8Batch, KV8Cache, QKNormRopeKernel, Rope
+from test_gpu_kv8_append import freqs
 from test_gpu_kv8_attention import Case
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +67,24 @@ def test_long_tail_of_small_weights(ctx, seqs, rows):
     exp = (tail / (4 + tail))[None, :, None]
     # beside the terms: 33 * 2^-23 of the exponent, and sums of fp32
     assert np.all(np.abs(got - exp) <= exp * (2.0 ** -5 + 2.0 ** -8))
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+def test_rotation_angles(ctx, pairs):
+    """cos and sin of far positions as the rotation uses them.  The angle, at most a quarter turn's half, is rounded once from
+    64 bits (2^-25, times 0.71 for a cosine and 0.76 for a sine of that size); the series adds 2.7e-8 and 1.9e-8 to it, and
+    the result is rounded once (2^-25): at most 8.1e-8."""
+    d, rows = 128, 20000
+    rng = np.random.default_rng(3)
+    x = np.zeros((rows, d), np.float32)
+    a = np.arange(0, d, 2) if pairs else np.arange(d // 2)
+    x[:, a] = 1
+    pos = rng.integers(0, 1 << 20, rows).astype(np.int32)
+    f = freqs(d)
+    xb = ctx.upload(x)
+    h = HeadRows(xb, 1, d)
+    QKNormRopeKernel(ctx).encode(None, h, None, h, None, ctx.upload(pos), rows, d, Rope(ctx.upload(f), d, pairs))
+    ctx.synchronize()
+    got = xb.download(np.float32).reshape(rows, d)
+    exp = R.norm_rope(x[:, None], pos, f, d, pairs)[:, 0]
+    assert np.abs(got - exp).max() <= 8.1e-8
