@@ -155,20 +155,47 @@ ER_DEV Turns turns_of(int position, const Frequencies &f) {
     return t;
 }
 
+template <int CTRL>
+ER_DEV double dpp_of(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int W>
+ER_DEV double group_sum64(double v) {  // W = 8, 16 or 32 lanes
+    v += dpp_of<ER_DPP_QUAD_XOR1>(v);
+    v += dpp_of<ER_DPP_QUAD_XOR2>(v);
+    v += dpp_of<ER_DPP_ROW_HALF_MIRROR>(v);
+    if constexpr (W >= 16) v += dpp_of<ER_DPP_ROW_MIRROR>(v);
+    if constexpr (W == 32) v += __shfl_xor(v, 16);
+    return v;
+}
+// 1 / sqrt of the mean of a head's D squares plus eps; `sum` is this lane's part
+// of the sum.  In 64 bits, where the squares of no fp32 values leave the range. One Newton
+// step doubles the correct bits of the instruction's root, over 20.
+template <int D>
+ER_DEV double head_rsqrt(double sum, double eps) {
+    const double ms = group_sum64<D / 8>(sum) * (1.0 / D) + eps, r0 = __builtin_amdgcn_rsq(ms);
+    return ms < __builtin_inf() ? r0 * __builtin_fma(-0.5 * ms * r0, r0, 1.5) : r0;
+}
+
 // The head's values normed (w: this lane's norm weights) and rotated.  D / 8
 // lanes hold the head, so its sum of squares is a sum over that lane group.
 template <int D>
 ER_DEV void norm_turn(Pairs &v, bool norm, const Pairs &w, const Turns &t, float eps) {
     if (norm) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v.a[i] * v.a[i] + v.b[i] * v.b[i];
-        sum = group_sum<D / 8>(sum);
-        const float r = 1.0f / sqrtf(sum * (1.0f / D) + eps);
+        double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v.a[i] *= r * w.a[i];
-            v.b[i] *= r * w.b[i];
+            const double a = (double)v.a[i], b = (double)v.b[i];
+            sum = __builtin_fma(b, b, __builtin_fma(a, a, sum));
+        }
+        const double r = head_rsqrt<D>(sum, (double)eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v.a[i] = (float)((double)v.a[i] * r) * w.a[i];
+            v.b[i] = (float)((double)v.b[i] * r) * w.b[i];
         }
     }
 #pragma unroll
@@ -186,22 +213,6 @@ ER_DEV void norm_turn(Pairs &v, bool norm, const Pairs &w, const Turns &t, float
 // took 14 us for three ragged prompts of an 8B layer, this one 16); the
 // results go to fp32 by rounding to odd, which no later rounding to fewer bits
 // notices.
-template <int CTRL>
-ER_DEV double dpp_of(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-template <int W>
-ER_DEV double group_sum64(double v) {  // W = 8, 16 or 32 lanes
-    v += dpp_of<ER_DPP_QUAD_XOR1>(v);
-    v += dpp_of<ER_DPP_QUAD_XOR2>(v);
-    v += dpp_of<ER_DPP_ROW_HALF_MIRROR>(v);
-    if constexpr (W >= 16) v += dpp_of<ER_DPP_ROW_MIRROR>(v);
-    if constexpr (W == 32) v += __shfl_xor(v, 16);
-    return v;
-}
 ER_DEV float round_to_odd(double v) {
     float f = (float)v;
     const double back = (double)f;
@@ -263,9 +274,7 @@ ER_DEV void norm_turn64(Pairs &p, bool norm, const Pairs &w, bool turns, const T
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum = __builtin_fma(b[i], b[i], __builtin_fma(a[i], a[i], sum));
-        // one Newton step doubles the correct bits of the instruction's root, over 20
-        const double ms = group_sum64<D / 8>(sum) * (1.0 / D) + eps, r0 = __builtin_amdgcn_rsq(ms);
-        const double r = ms < __builtin_inf() ? r0 * __builtin_fma(-0.5 * ms * r0, r0, 1.5) : r0;
+        const double r = head_rsqrt<D>(sum, eps);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             a[i] *= r * (double)w.a[i];

@@ -4,7 +4,7 @@ import pytest
 
 import kv8_ref as R
 from edgerunner_amd import HeadRows, KV8AttentionKernel, KV8Batch, KV8Cache, QKNormRopeKernel, Rope
-from test_gpu_kv8_append import freqs
+from test_gpu_kv8_append import Case as AppendCase, freqs, turn_tol
 from test_gpu_kv8_attention import Case
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +88,27 @@ def test_rotation_angles(ctx, pairs):
     got = xb.download(np.float32).reshape(rows, d)
     exp = R.norm_rope(x[:, None], pos, f, d, pairs)[:, 0]
     assert np.abs(got - exp).max() <= 8.1e-8
+
+
+@pytest.mark.parametrize("d,power,eps", [(64, 70, 1e-6), (128, 120, 1e-6), (256, 100, 1e-5), (64, -80, 0.0), (128, -120, 0.0),
+                                         (256, -40, 1e-30), (128, -141, 0.0)])
+def test_norms_of_large_and_small_heads(ctx, d, power, eps):
+    """Heads whose squares pass fp32's range at either end are normed as the others, alone and on the way of an append."""
+    rng = np.random.default_rng(d + abs(power))
+    rows, hq, hk = 7, 5, 3
+    x = rng.standard_normal((rows, hq + hk, d)).astype(np.float32)
+    x[::2, ::2] = np.clip(x[::2, ::2], -3, 3) * np.float32(2.0 ** max(power, -126)) * np.float32(2.0 ** min(power + 126, 0))
+    pos, w, f = rng.integers(0, 9000, rows).astype(np.int32), (rng.random(d) + 0.5).astype(np.float32), freqs(d)
+    xb, wb, fb, pb = ctx.upload(x), ctx.upload(w), ctx.upload(f), ctx.upload(pos)
+    width = (hq + hk) * d
+    q, k = HeadRows(xb, hq, width), HeadRows(xb.view(4 * hq * d), hk, width)
+    QKNormRopeKernel(ctx).encode(None, q, k, q, k, pb, rows, d, Rope(fb, d), wb, wb, eps)
+    ctx.synchronize()
+    got = xb.download(np.float32).reshape(x.shape)
+    assert np.all(np.abs(got - R.norm_rope(x, pos, f, d, False, w, eps)) <= turn_tol(x, d, False, w, eps))
+    c = AppendCase(ctx, rng, [rows], [rows], 16, d, hk, norm=True, hq=hq)
+    c.q, c.w = x[:, :hq].copy(), w
+    c.run(eps=eps)
+    got = c.io[3].download(np.float32).reshape(c.q.shape)
+    exp = R.norm_rope(c.q, np.arange(rows), c.f, d, False, w, eps)
+    assert np.all(np.abs(got - exp) <= turn_tol(c.q, d, False, w, eps))
