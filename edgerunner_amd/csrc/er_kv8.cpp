@@ -454,7 +454,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     else
         st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, pairs * p.splits * p.tiles, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
-    if (!p.shares && p.splits <= 16) return launch(kernels.joinRow[di], op, batch->rows, 0, stream, &a);
+    if (!p.shares && p.splits <= ER_KV8_ROW_PARTS) return launch(kernels.joinRow[di], op, batch->rows, 0, stream, &a);
     const uint32_t most = p.shares ? p.shares : p.splits;
     return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
 }

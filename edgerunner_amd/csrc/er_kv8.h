@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #define ER_KV8_THREADS 256
+#define ER_KV8_ROW_PARTS 16  // parts that the join of a whole row takes at the most
 
 // Norm and rotation of one kind of heads.
 struct ErTurn {

@@ -7,6 +7,7 @@
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -364,7 +365,6 @@ ER_DEV uint32_t codes4(float a, float b, float c, float d) {
 }
 // Four codes times a power of two up to 1, to nearest even.
 ER_DEV uint32_t recode4(uint32_t c, float f) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
     return codes4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
 }

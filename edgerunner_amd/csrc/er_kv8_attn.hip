@@ -158,9 +158,16 @@ ER_DEV void store4(const ErAttendArgs &p, int row, uint32_t head, uint32_t d, ui
 ER_DEV size_t part_index(const ErAttendArgs &p, uint32_t piece, int row, uint32_t head) {
     return ((size_t)piece * p.b.rows + (size_t)row) * (p.group * p.c.heads) + head;
 }
-// A column's output is its sums times 1 / l; zeros where no token is visible.
+// A column's output is its sums over l; zeros where no token is visible.
 // Where some are and l is 0 or NaN (scores without a finite maximum), the
-// quotient is NaN, as the softmax's is.
+// quotient is NaN, as the softmax's is.  Sums that are joined are divided by
+// their own l first and weighted by its share of the whole, so that a mean of
+// values near fp32's largest stays inside its range.
+ER_DEV float over(float l) { return l != 0.0f ? 1.0f / l : 1.0f; }
+ER_DEV float share_of(float l, float total) { return total != 0.0f ? l / total : 0.0f; }
+ER_DEV f32x4 joined(f32x4 o, bool visible, float total) {
+    return !visible ? f32x4{} : total != 0.0f ? o : o + __builtin_nanf("");
+}
 
 // ---------------------------------------------------------------- few columns: decode, drafts
 
@@ -596,7 +603,7 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     const bool seen = column_max4(st.seen ? 1.0f : 0.0f) > 0.0f;
     if (n < cols) {
         float *at = lds + (wave * cols + n) * PITCH;
-        const float f = st.vref * 0.0078125f;
+        const float f = st.vref * 0.0078125f * over(l);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -615,19 +622,21 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
         bool visible = false;
 #pragma unroll
         for (int v = 0; v < 4; ++v) m = fmaxf(m, sm[v * 16 + col]);
-        f32x4 o = {};
+        float f[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const float l = sl[v * 16 + col];
-            if (l < 0.0f) continue;
-            visible = true;
-            const float f = __builtin_amdgcn_exp2f(sm[v * 16 + col] - m);
-            total += l * f;
-            o += *(const f32x4 *)(lds + (v * cols + col) * PITCH + d) * f;
+            f[v] = l < 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(sm[v * 16 + col] - m);
+            visible |= !(l < 0.0f);
+            total += f[v];
         }
+        f32x4 o = {};
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            if (!(sl[v * 16 + col] < 0.0f)) o += *(const f32x4 *)(lds + (v * cols + col) * PITCH + d) * share_of(f[v], total);
         if (complete) {
             const Column k = column_of(p, q, h, col0 + col);
-            store4(p, k.row, k.head, d, D, visible ? o * (1.0f / total) : f32x4{});
+            store4(p, k.row, k.head, d, D, joined(o, visible, total));
         } else {
             const size_t at = (size_t)part * 16 + col;
             if (visible) *(f32x4 *)(p.partO + at * D + d) = o;
@@ -1049,7 +1058,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     l = column_sum2(l);
     seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f ? 1u : 0u;
     if (!live) return;
-    const float f = p.splits == 1 ? vref * 0.0078125f / l : vref * 0.0078125f;
+    const float f = p.splits == 1 ? vref * 0.0078125f / l : vref * 0.0078125f * over(l);
     const size_t to = part_index(p, piece, c.row, c.head);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -1081,7 +1090,7 @@ ER_DEV float wave_top(float v) {
     return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
 }
 
-// One column's parts: weights 2^(m - max) / sum from the references and sums,
+// One column's parts: weights l 2^(m - max) / sum from the references and sums,
 // then the weighted outputs, D / 4 lanes a part.  index(i): where part i lies.
 template <int D, typename INDEX>
 ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t head, float *lds, INDEX index) {
@@ -1096,14 +1105,16 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
         const size_t at = 2 * index(i);
         const float l = p.partML[at + 1];
         const bool some = !(l < 0.0f);
-        const float f = some ? __builtin_amdgcn_exp2f(p.partML[at] - top) : -1.0f;
-        if (some) total += l * f;
+        const float f = some ? l * __builtin_amdgcn_exp2f(p.partML[at] - top) : -1.0f;
+        if (some) total += f;
         seen |= some;
         if (tid < 64) weight[i] = f;
     }
     // every wave has the sum, of the same terms in the same order
     total = group_sum<64>(total);
     seen = __any(seen);
+    for (uint32_t i = tid; i < parts && tid < 64; i += 64)
+        if (!(weight[i] < 0.0f)) weight[i] = share_of(weight[i], total);
     __syncthreads();
     constexpr uint32_t LANES = D / 4, AT_ONCE = ER_KV8_THREADS / LANES;
     const uint32_t mine = tid / LANES, d = (tid % LANES) * 4;
@@ -1119,7 +1130,7 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
         f32x4 v = {};
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; ++k) v += *(const f32x4 *)(red + 4 * (k * LANES + tid));
-        store4(p, row, head, 4 * tid, D, seen ? v * (1.0f / total) : f32x4{});
+        store4(p, row, head, 4 * tid, D, joined(v, seen, total));
     }
 }
 
@@ -1169,20 +1180,30 @@ ER_DEV void kv8_join_row(const ErAttendArgs &p) {
     if ((int)row < q.row0 || (int)row >= q.row0 + q.n) return;
     for (uint32_t at = threadIdx.x; at < heads * (D / 4); at += ER_KV8_THREADS) {
         const uint32_t head = at / (D / 4), d = (at % (D / 4)) * 4;
-        float top = ER_NO_MAX, total = 0.0f;
+        // all parts' references and sums at once
+        float m[ER_KV8_ROW_PARTS], l[ER_KV8_ROW_PARTS], top = ER_NO_MAX, total = 0.0f;
         bool seen = false;
-        for (uint32_t i = 0; i < p.splits; ++i) top = fmaxf(top, p.partML[2 * part_index(p, i, (int)row, head)]);
-        f32x4 o = {};
-        for (uint32_t i = 0; i < p.splits; ++i) {
-            const size_t part = part_index(p, i, (int)row, head);
-            const float l = p.partML[2 * part + 1];
-            if (l < 0.0f) continue;
-            const float f = __builtin_amdgcn_exp2f(p.partML[2 * part] - top);
-            total += l * f;
-            o += *(const f32x4 *)(p.partO + part * D + d) * f;
-            seen = true;
+#pragma unroll
+        for (uint32_t i = 0; i < ER_KV8_ROW_PARTS; ++i) {
+            const f32x2 ml = i < p.splits ? *(const f32x2 *)(p.partML + 2 * part_index(p, i, (int)row, head)) : f32x2{ER_NO_MAX, -1.0f};
+            m[i] = ml.x;
+            l[i] = ml.y;
+            top = fmaxf(top, ml.x);
         }
-        store4(p, (int)row, head, d, D, seen ? o * (1.0f / total) : f32x4{});
+#pragma unroll
+        for (uint32_t i = 0; i < ER_KV8_ROW_PARTS; ++i) {
+            const bool some = !(l[i] < 0.0f);
+            l[i] = some ? l[i] * __builtin_amdgcn_exp2f(m[i] - top) : -1.0f;
+            total += some ? l[i] : 0.0f;
+            seen |= some;
+        }
+        const float inverse = over(total);
+        f32x4 o = {};
+#pragma unroll
+        for (uint32_t i = 0; i < ER_KV8_ROW_PARTS; ++i)
+            if (i < p.splits && !(l[i] < 0.0f))
+                o += *(const f32x4 *)(p.partO + part_index(p, i, (int)row, head) * D + d) * (l[i] * inverse);
+        store4(p, (int)row, head, d, D, joined(o, seen, total));
     }
 }
 

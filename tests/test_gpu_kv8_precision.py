@@ -1,11 +1,14 @@
-"""Where the operators between the projections could lose bits, against 64-bit forms."""
+"""Where the operators between the projections could lose bits: value scales of
+tokens that a row does not see, weights far below a row's largest, rotation
+angles, head norms of very large and very small heads, values near fp32's
+largest.  All against 64-bit forms."""
 import numpy as np
 import pytest
 
 import kv8_ref as R
 from edgerunner_amd import HeadRows, KV8AttentionKernel, KV8Batch, KV8Cache, QKNormRopeKernel, Rope
 from test_gpu_kv8_append import Case as AppendCase, freqs, turn_tol
-from test_gpu_kv8_attention import Case
+from test_gpu_kv8_attention import LONE, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -36,6 +39,26 @@ def test_scales_of_hidden_values(ctx, d, P, hq, hkv, lens, rows, window, every, 
     c = Case(ctx, d + P + ratio, lens, rows, P, d, hq, hkv)
     page_scales(c, lambda p: ratio - 5 if p % every == first else p % 4 - 6)
     c.check(c.run(half, window), half, window)
+
+
+@pytest.mark.parametrize("down", [20, 22])
+@pytest.mark.parametrize("d,P,hq,hkv,lens,rows", [
+    (64, 16, 4, 2, [400, 300], [1, 1]), (128, 32, 4, 2, [500], [5]), (256, 64, 2, 1, [700, 90], [3, 2]),
+    (64, 16, 4, 2, [400, 300], [70, 30]), (128, 64, 4, 1, [600], [100]), (256, 32, 2, 1, [350], [200])])
+def test_codes_below_the_largest_scale(ctx, d, P, hq, hkv, lens, rows, down):
+    """A block of values whose scale is 2^-22 of the largest that a row sees keeps its codes whole, subnormal ones too: the pages
+    of the large scale have values in element 0 alone, so the other elements are held to the small ones' own bound."""
+    c = Case(ctx, d + down, lens, rows, P, d, hq, hkv)
+    page_scales(c, lambda p: 10 if p % 4 == 1 else 10 - down)
+    for s in range(len(lens)):
+        for p in range(c.b.stride):
+            page = c.b.table[s, p]
+            if page >= 0 and p % 4 == 1:
+                c.vc[page, ..., 1:] = 0
+            elif page >= 0:  # the smallest codes, whose last bit is the one at stake
+                keep = (c.vc[page] & 0x7f) == 0x7f
+                c.vc[page] = np.where(keep, c.vc[page], c.vc[page] & 0x87)
+    c.check(c.run())
 
 
 # Weights are held as two fp16 terms of up to 2^15 for the largest of a row and 2^13 at the least, so one of 2^-33 of the
@@ -112,3 +135,18 @@ def test_norms_of_large_and_small_heads(ctx, d, power, eps):
     got = c.io[3].download(np.float32).reshape(c.q.shape)
     exp = R.norm_rope(c.q, np.arange(rows), c.f, d, False, w, eps)
     assert np.all(np.abs(got - exp) <= turn_tol(c.q, d, False, w, eps))
+
+
+@pytest.mark.parametrize("lens,rows,hq,hkv", [([1], [1], 2, 1), ([40, 3], [1, 1], 4, 2), ([2000], [3], 2, 1), ([90], [70], 2, 1),
+                                              ([1500], [80], 2, 1), ([50000], [1], 1, 1)])
+def test_values_near_the_largest(ctx, lens, rows, hq, hkv):
+    """Values of up to 240 * 2^120, next to fp32's largest: a mean of them is no larger, however many there are."""
+    c = Case(ctx, 21, lens, rows, 32, 64, hq, hkv)
+    nan = (c.vc & 0x7f) == 0x7f
+    c.vc = np.where(nan, c.vc, 0x70 + (c.vc & 7)).astype(np.uint8)  # 128 .. 240
+    c.vs[:] = np.where(np.isnan(c.vs), c.vs, 2.0 ** 120)
+    if lens == [1]:
+        got = c.run()
+        exp = R.VALUES[c.vc[c.b.table[0, 0], 0, 0]] * 2.0 ** 120
+        assert np.all(np.abs(got[0] - exp) <= LONE * exp)
+    c.check(c.run())
