@@ -191,9 +191,18 @@ ErTurn turn_args(const er_head_rows *in, const er_head_rows *out, const er_buffe
     return t;
 }
 
-er_status launch(hipFunction_t f, const char *op, uint64_t blocks, uint32_t lds, er_stream stream, void *args) {
-    if (blocks > 0x7fffffffull)
+// Kernels count a launch's threads in 32 bits.
+constexpr uint64_t kMostBlocks = (1ull << 32) / ER_KV8_THREADS - 1;
+
+er_status check_blocks(const char *op, uint64_t blocks) {
+    if (blocks > kMostBlocks)
         return fail(ER_ERR_ENCODING_FAILED, "%s: %llu workgroups exceed a launch", op, (ull)blocks);
+    return ER_OK;
+}
+
+er_status launch(hipFunction_t f, const char *op, uint64_t blocks, uint32_t lds, er_stream stream, void *args) {
+    const er_status st = check_blocks(op, blocks);
+    if (st != ER_OK) return st;
     void *params[] = {args};
     const hipError_t e = hipModuleLaunchKernel(f, (uint32_t)blocks, 1, 1, ER_KV8_THREADS, 1, 1, lds,
                                                (hipStream_t)stream, params, nullptr);
@@ -386,8 +395,8 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
         a.chunks = row_chunks((a.q.heads + per - 1) / per, batch->rows, cu_count_of(ctx));
         blocks += ((uint64_t)batch->rows * a.chunks + 3) / 4;
     }
-    if (blocks > 0x7fffffffull)
-        return fail(ER_ERR_ENCODING_FAILED, "%s: %llu workgroups exceed a launch", op, (ull)blocks);
+    st = check_blocks(op, blocks);
+    if (st != ER_OK) return st;
     a.cacheBlocks = (uint32_t)cacheBlocks;
     return launch(kv8_of(ctx).append[dim_index(d)], op, blocks, 0, stream, &a);
 }
@@ -449,14 +458,18 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     const Kv8Kernels &kernels = kv8_of(ctx);
     const int di = dim_index(d);
     const uint64_t pairs = (uint64_t)batch->sequences * cache->kv_heads;
-    if (p.narrow)
-        st = launch(kernels.narrow[di][a.c.shift - 4][a.half], op, p.shares ? p.shares : pairs * p.tiles, 0, stream, &a);
-    else
-        st = launch(kernels.wide[di][a.c.shift - 4][a.half], op, pairs * p.splits * p.tiles, 0, stream, &a);
+    const uint64_t blocks = p.shares ? p.shares : pairs * p.splits * p.tiles;  // narrow: one split
+    const bool byRow = !p.shares && p.splits <= ER_KV8_ROW_PARTS;
+    const uint64_t joins = !joined ? 0 : byRow ? batch->rows : (uint64_t)batch->rows * q->heads;
+    // both, before the first is queued
+    st = check_blocks(op, blocks);
+    if (st == ER_OK) st = check_blocks(op, joins);
+    if (st != ER_OK) return st;
+    st = launch((p.narrow ? kernels.narrow : kernels.wide)[di][a.c.shift - 4][a.half], op, blocks, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
-    if (!p.shares && p.splits <= ER_KV8_ROW_PARTS) return launch(kernels.joinRow[di], op, batch->rows, 0, stream, &a);
+    if (byRow) return launch(kernels.joinRow[di], op, joins, 0, stream, &a);
     const uint32_t most = p.shares ? p.shares : p.splits;
-    return launch(kernels.join[di], op, (uint64_t)batch->rows * q->heads, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
+    return launch(kernels.join[di], op, joins, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
 }
 
 }  // extern "C"

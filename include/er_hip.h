@@ -437,7 +437,8 @@ typedef struct er_rope {
  * k and k_out NULL: queries alone.  An output may be its own input (same
  * data, heads and stride); otherwise they do not overlap.  head_dim 64, 128
  * or 256 and rotary_dim as above, else INVALID_VECTOR_SHAPE; a buffer shorter
- * than its rows -> ENCODING_FAILED; rows 0 does nothing. */
+ * than its rows, or more work than one launch counts (2^24 - 1 workgroups, of at
+ * least 4 rows each) -> ENCODING_FAILED; rows 0 does nothing. */
 er_status er_hip_qk_norm_rope(er_hip_ctx *ctx, er_stream stream, const er_head_rows *q, const er_head_rows *k,
                               const er_head_rows *q_out, const er_head_rows *k_out, er_buffer positions,
                               er_buffer q_norm, er_buffer k_norm, const er_rope *rope, uint32_t rows,
@@ -495,7 +496,8 @@ typedef struct er_kv8_batch {
  * first; codes round to nearest even.  NaN and infinities become the NaN code
  * 0xff and do not enter the scale.  Slots behind the last token keep their bytes.
  * Sizes -> INVALID_VECTOR_SHAPE, a cache buffer too short ->
- * INVALID_MATRIX_SHAPE, other buffers too short -> ENCODING_FAILED. */
+ * INVALID_MATRIX_SHAPE, other buffers too short -> ENCODING_FAILED, as is more
+ * than 2^24 - 1 workgroups (two a page and head of the new tokens; four rows of queries one). */
 er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache, const er_kv8_batch *batch,
                             const er_head_rows *k, const er_head_rows *v, uint32_t v_type, const er_head_rows *q,
                             const er_head_rows *q_out, er_buffer k_norm, er_buffer q_norm, const er_rope *rope,
