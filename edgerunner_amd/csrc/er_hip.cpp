@@ -1904,12 +1904,9 @@ er_status er_hip_create(int device, er_hip_ctx **out_ctx) {
                     return fail(ER_ERR_FUNCTION_NOT_FOUND, "functionNotFound(%s): %s", name, hipGetErrorString(e));
                 }
             }
-    const er_status kv8 = er_detail::kv8_load(ctx->kv8);
-    if (kv8 != ER_OK) {
-        (void)hipModuleUnload(ctx->module);
-        delete ctx;
-        return kv8;
-    }
+    // Now rather than at their first call, which may be recorded.  A context whose cache kernels do not load
+    // has everything else; their calls say so.
+    (void)er_detail::kv8_load(ctx->kv8);
     set_tok_mode(ctx, std::getenv("ER_HIP_GEMV_TOK"));
     if (const char *gv = std::getenv("ER_HIP_GEMM_VARIANT")) ctx->gemm_variant = std::atoi(gv);
     if (const char *fv = std::getenv("ER_HIP_GEMV_FP32")) ctx->gemv_fp32 = std::atoi(fv);

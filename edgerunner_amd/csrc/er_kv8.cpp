@@ -214,6 +214,14 @@ er_status check_ctx(const er_hip_ctx *ctx) {
     return ctx ? ER_OK : fail(ER_ERR_INVALID_ARGUMENT, "null er_hip_ctx");
 }
 
+// The context's device current, its kernels there.
+er_status make_ready(const char *op, const er_hip_ctx *ctx) {
+    const er_status st = check_ctx(ctx);
+    if (st != ER_OK) return st;
+    if (!kv8_of(ctx).module) return fail(ER_ERR_LIBRARY_NOT_FOUND, "%s: the cache kernels did not load with this context", op);
+    return bind_device_of(ctx);
+}
+
 // Waves that a row's strips of heads are cut into: with few rows one strip a
 // wave (the shortest chain), with many as few as keep 16 waves a CU, so that a
 // row's angles are formed as seldom as they can be.
@@ -329,8 +337,7 @@ er_status er_hip_qk_norm_rope(er_hip_ctx *ctx, er_stream stream, const er_head_r
     if (st == ER_OK && rope->rotary_dim) st = check_buffer(op, "positions", positions, (uint64_t)rows * 4, 4);
     if (st == ER_OK) st = check_norm(op, "q_norm", q_norm, head_dim);
     if (st == ER_OK) st = check_norm(op, "k_norm", k_norm, head_dim);
-    if (st == ER_OK) st = check_ctx(ctx);
-    if (st == ER_OK) st = bind_device_of(ctx);
+    if (st == ER_OK) st = make_ready(op, ctx);
     if (st != ER_OK) return st;
     ErRopeArgs a{};
     a.q = turn_args(q, q_out, q_norm);
@@ -373,8 +380,7 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
     }
     if (st == ER_OK) st = check_norm(op, "k_norm", k_norm, d);
     if (st == ER_OK) st = check_norm(op, "q_norm", q_norm, d);
-    if (st == ER_OK) st = check_ctx(ctx);
-    if (st == ER_OK) st = bind_device_of(ctx);
+    if (st == ER_OK) st = make_ready(op, ctx);
     if (st != ER_OK) return st;
     ErAppendArgs a{};
     a.c = cache_args(cache), a.b = batch_args(cache, batch);
@@ -434,8 +440,7 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     if (q->heads != out->heads) return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: q and out differ in heads", op);
     st = check_group(op, cache, batch, q->heads);
     if (st == ER_OK) st = check_apart(op, "q and out", q, out, batch->rows, d, 4, outBytes, false);
-    if (st == ER_OK) st = check_ctx(ctx);
-    if (st == ER_OK) st = bind_device_of(ctx);
+    if (st == ER_OK) st = make_ready(op, ctx);
     if (st != ER_OK) return st;
     ErAttendArgs a{};
     a.c = cache_args(cache), a.b = batch_args(cache, batch);

@@ -17,7 +17,8 @@ struct Kv8Kernels {
     hipFunction_t narrow[kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};  // [fp32, bf16 output]
 };
 
-// Loads the cache's code object on the current device and resolves its kernels.
+// Loads the cache's code object on the current device and resolves its kernels;
+// where it fails, nothing of it stays.
 er_status kv8_load(Kv8Kernels &k);
 void kv8_unload(Kv8Kernels &k);
 

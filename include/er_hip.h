@@ -409,7 +409,9 @@ er_status er_hip_encode_projection(er_hip_ctx *ctx, er_stream stream,
  * key/value cache and attention over it ----
  * No counterpart on the reference's quantised path; they stand between the
  * q/k/v projections (fp32 q and k, fp32 or fp16 v) and the output projection
- * (fp32 x for the GEMV, bf16 x for the prefill GEMM) of this header. */
+ * (fp32 x for the GEMV, bf16 x for the prefill GEMM) of this header.  Where their
+ * code object did not load when the context was created, they alone fail:
+ * LIBRARY_NOT_FOUND. */
 
 /* Rows of heads: element e of head h in row r is data[r * row_stride + h *
  * head_dim + e] (row_stride in elements, >= heads * head_dim, so the heads may

@@ -9,7 +9,7 @@ import pytest
 from edgerunner_amd import _ffi
 from edgerunner_amd.build import CSRC, ROCM, ROOT
 
-F32, ENC = 0, 3
+F32, NOLIB, ENC = 0, 1, 3
 NULL = _ffi.er_buffer(None, 0)
 MOST = (1 << 24) - 1  # workgroups whose threads 32 bits count
 STUB = Path(__file__).with_name("kv8_host_stub.cpp")
@@ -117,3 +117,13 @@ def test_attention_that_a_launch_does_not_count(host, ctx):
     assert refused(host, attend(host, ctx, 2, 16, batch(n, n, 1, 640), n))  # the join: a workgroup a row and query head
     assert attend(host, ctx, 2, 4, batch(n, n, 1, 640), n) == 0 and launches(host) == [512, 8 * n]
     assert refused(host, attend(host, ctx, 16, 1, batch(n, 128 * n, 128, 128), 128 * n))  # 128 columns a workgroup
+
+
+def test_kernels_that_did_not_load_are_not_launched(host):
+    """A context without the cache's kernels stays usable for the rest; the operators that need them say so."""
+    ctx = host.stub_create(256, 0)
+    launches(host)
+    b = batch(2, 2, 1, 100)
+    for call in (lambda: norm_rope(host, ctx, 8), lambda: append(host, ctx, 2, b, 2, 4), lambda: attend(host, ctx, 2, 2, b, 2)):
+        assert call() == NOLIB and b"did not load" in host.stub_error() and launches(host) == []
+    host.stub_destroy(ctx)
