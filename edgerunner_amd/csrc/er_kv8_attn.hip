@@ -664,7 +664,11 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     if (at >= last) return;
     uint32_t begins, s = sequence_at(p, first, sh.aligned, at, lane, begins);
     LaneSequence l = lane_sequence_at(p, first, s);
+    // Sequences behind the 64th are read again.  Should the batch's arrays change meanwhile,
+    // the outputs mean nothing, but every workgroup ends and stays inside the buffers.
+    if (l.steps == 0) return;
     uint32_t length = shared_length(p, l.steps, sh.aligned), unit = (at - begins) / length;
+    if (unit >= H * blocks_of(p, l.q)) return;
     begins += unit * length;
     while (true) {
         // a unit that begins here and goes on in later workgroups leaves its
@@ -678,8 +682,10 @@ ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
         if (at >= last) return;
         if (++unit == H * blocks) {
             unit = 0;
-            do l = lane_sequence(p, ++s);
-            while (l.steps == 0);
+            do {
+                if (++s >= p.b.sequences) return;
+                l = lane_sequence(p, s);
+            } while (l.steps == 0);
             length = shared_length(p, l.steps, sh.aligned);
         }
         __syncthreads();  // the sums in LDS have been read
@@ -1163,6 +1169,7 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
     const uint32_t begins = before + unit * shared_length(p, l.steps, sh.aligned);
     const uint32_t w0 = begins / sh.quota, parts = (begins + l.steps - 1) / sh.quota - w0 + 1;
     if (parts == 1) return;  // one workgroup had it all and wrote it
+    if (w0 + parts > p.shares) return;  // as in kv8_attend_narrow
     join_parts<D>(p, parts, (int)row, head, lds, [&](uint32_t i) {
         return (size_t)(2 * (w0 + i) + (i == 0 ? 1u : 0u)) * 16 + (col & 15u);
     });

@@ -463,7 +463,7 @@ typedef struct er_kv8_cache {
 } er_kv8_cache;
 
 /* The sequences of a call, read on the device (a recorded graph follows later
- * contents).  Rows row_start[s] .. row_start[s + 1] - 1 of the row buffers are
+ * contents; the arrays stay as they are while a call runs).  Rows row_start[s] .. row_start[s + 1] - 1 of the row buffers are
  * sequence s's newest tokens: of the kv_len[s] tokens that it has in the cache
  * once they are appended, they are the last, and the i-th of n rows has the
  * position kv_len[s] - n + i.  Token t lies in page page_table[s][t /
