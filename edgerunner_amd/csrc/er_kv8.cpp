@@ -254,7 +254,9 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     if (p.narrow) {
         // two workgroups a CU are resident; a workgroup's start and its part in the join cost as much as some
         // hundred tokens, so none takes fewer than that, and what a workgroup
-        // a sequence and head reads in that time is not shared at all
+        // a sequence and head reads in that time is not shared at all.  By 1, 2, 4 and 8 steps of 64 tokens, us: 16
+        // draft checks at head width 256 (17 steps a unit) 26.2, 26.2, 20.7, 21.3; a user of 8000 tokens at width 128
+        // 19.4, 17.0, 13.9, 14.6; 16 of up to 4000 at width 64 15.2, 15.5, 13.6, 13.5
         const uint64_t resident = (uint64_t)cu * 2;
         p.tiles = (uint32_t)((cols + 15) / 16);
         if (full > 512) {
@@ -270,11 +272,12 @@ AttendPlan plan_attend(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     if (window) span = std::min<uint64_t>(span, (uint64_t)window + 128 / group + 2 + 63);
     // The tokens of a (sequence, head, row tile) are cut into as many pieces as
     // make one workgroup for each that the chip holds, of 256 tokens at the
-    // least: fewer leave it empty, more have more sums to join (a chunk of 256
-    // rows behind 60000 tokens in 8 pieces a tile 458 us, in 12 484, in 16 481;
-    // three ragged chunks in 5, 7 and 10 pieces 79, 65 and 71; a prompt of 4096
-    // rows of 8 heads in one and two 181 and 267).  Of a prompt's pieces half
-    // lie behind its rows, and of several sequences one eighth behind their ends.
+    // least: fewer leave it empty, more have more sums to join (bf16, a chunk of 256
+    // rows behind 60000 tokens in 4, 8, 12 and 16 pieces a tile 384, 323, 339 and 337
+    // us; a prompt of 4096 rows of 8 heads in one and two 193 and 284).  Of a
+    // prompt's pieces half lie behind its rows, and of several sequences one
+    // eighth behind their ends: a guess, since lengths are known on the device
+    // alone.  Three ragged chunks take 86 us in 5 pieces, 73 in 7, 78 in 8 and in 10; the rule takes 8.
     const uint64_t resident = (uint64_t)cu * (c->head_dim == 64 ? 3 : c->head_dim == 128 ? 2 : 1);
     const uint64_t filled = std::max<uint64_t>(1, ((uint64_t)b->rows * group + 64ull * b->sequences) / 128);
     const uint64_t units = c->kv_heads * std::min(filled, (uint64_t)b->sequences * p.tiles);

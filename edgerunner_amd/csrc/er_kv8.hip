@@ -322,8 +322,8 @@ ER_DEV void turn_heads(const ErTurn &h, uint32_t row, uint32_t chunk, uint32_t c
 // row's angles (64-bit products, a sine and a cosine for every pair) are
 // formed once for all of them.  All of a head's loads precede its stores and no
 // other lane reads the head, so an output may be its own input.  4096 rows of 32
-// + 8 heads of 128 take 38.6 us: 4.35 TB/s in and out, where a copy of as much
-// reaches 4.7; one row 2.9 us, a launch.
+// + 8 heads of 128 take 38.3 us: 4.38 TB/s in and out, where a copy of as much
+// reaches 4.7; one row 3.0 us, a launch.
 template <int D>
 ER_DEV void qk_norm_rope(const ErRopeArgs &p) {
     const uint32_t wave = uniform((blockIdx.x * ER_KV8_THREADS + threadIdx.x) >> 6);
@@ -415,7 +415,9 @@ ER_DEV void turn_query_row(const ErAppendArgs &p) {
 // are powers of two, growing one costs them nothing but subnormals.  No other
 // workgroup touches the block, so nothing is ordered between workgroups.
 // Three ragged prompts of an 8B layer (43 MB in and out, 9 us at a copy's rate)
-// take 16 us, bound by the keys' 64-bit rotations; a token of each of 64 users
+// take 16 us: 2.3 of it are the keys' 64-bit rotations, which the workgroup of every
+// head forms again, and the rest over the copy a workgroup's own chain, in which loads, norm,
+// maximum and stores follow each other; a token of each of 64 users
 // 5.8 us, bound by the chain start, table, scale, row.
 template <int D, int P>
 ER_DEV void append_block(const ErAppendArgs &p, float *peaks) {

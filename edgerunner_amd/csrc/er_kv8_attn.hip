@@ -21,7 +21,7 @@
 // fp16's smallest step, 2^-24, is then 2^-37 of the row's largest weight at the
 // most: what the rounding of smaller weights leaves out of 2^18 tokens is 2^-20
 // of their values.  By 8 and + 7, which rescales less, it was 2^-14; a prompt of
-// 4096 rows then took 183.4 us, now 185.3.
+// 4096 rows then took 183.4 us where it takes 185.3 so.
 
 #define ER_SLACK 2.0f
 #define ER_LIFT 13.0f
@@ -904,8 +904,9 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
 // into LDS while the tile before is worked on, and convert them as they read
 // operands: codes are half the LDS traffic of fp16, and leave more registers
 // (fp16 in LDS spilled at head width 256).  A 4096-token prompt of an 8B layer
-// (137 GFLOP) takes 185 us, 742 TFLOP/s, two waves a SIMD; ragged chunks behind
-// long prefixes in fp32 (two terms, 35 GFLOP of products) 75 us with the join.
+// (137 GFLOP) takes 187 to 193 us, up to 735 TFLOP/s, two waves a SIMD; ragged chunks behind
+// long prefixes in fp32 (two terms, 35 GFLOP of products) 75 us with the join, and the
+// prompt in fp32 270.
 template <int D, int P, int TERMS>
 ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     // One row tile of all units (sequence, piece, head) after the other, each
@@ -1141,7 +1142,7 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
 }
 
 // One row and query head after the wide kernel (a part a piece) or the narrow
-// one (a part a workgroup that had some of the unit's steps): 8 us for 64 users
+// one (a part a workgroup that had some of the unit's steps): 9 us for 64 users
 // of 32 heads, 7 for one of 64 parts, a launch and a chain of loads.
 template <int D>
 ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
@@ -1176,8 +1177,8 @@ ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
 }
 
 // All heads of one row after the wide kernel, where the parts are few: four
-// values a thread, its column's references and sums read by all its lanes.  Five
-// parts of 1033 rows of 14 heads of 64 take 7.7 us, a workgroup a column 24.
+// values a thread, its column's references and sums read by all its lanes.  Eight
+// parts of 1033 rows of 14 heads of 64 take 9 us; a workgroup a column took 24 for five.
 template <int D>
 ER_DEV void kv8_join_row(const ErAttendArgs &p) {
     const uint32_t row = blockIdx.x, heads = p.group * p.c.heads, lane = threadIdx.x & 63u;

@@ -471,7 +471,7 @@ typedef struct er_kv8_cache {
  * are left as they are; a sequence may have no rows, no tokens, or both.
  * max_rows and max_kv_len bound what any sequence has: more is not looked at
  * (rows beyond the first max_rows, tokens beyond the first max_kv_len or
- * beyond the table).  Rows whose position would be negative are not appended
+ * beyond the table), and positions count from the bounded kv_len[s] and n.  Rows whose position would be negative are not appended
  * and attend to nothing (their q_out is left as it is, their output zeros).
  * Entries of page_table outside [0, pages) hold no tokens: nothing is read or
  * written there.  A page that gets tokens in a call stands once in the tables:
