@@ -71,6 +71,18 @@ class er_kv8_batch(C.Structure):
                 ("max_rows", C.c_uint32), ("max_kv_len", C.c_uint32)]
 
 
+class er_drafts(C.Structure):
+    _fields_ = [("seen", er_buffer), ("position", er_buffer), ("parent", er_buffer), ("token", er_buffer),
+                ("seen_words", C.c_uint32)]
+
+
+class er_logit_rules(C.Structure):
+    _fields_ = [("row_start", er_buffer), ("penalty", er_buffer), ("history", er_buffer), ("history_len", er_buffer),
+                ("bias_token", er_buffer), ("bias", er_buffer), ("bias_len", er_buffer), ("allowed", er_buffer),
+                ("sequences", C.c_uint32), ("max_rows", C.c_uint32), ("history_stride", C.c_uint32),
+                ("bias_stride", C.c_uint32), ("allowed_stride", C.c_uint32)]
+
+
 class er_gguf_value(C.Structure):
     _fields_ = [
         ("type", C.c_uint32),
@@ -217,6 +229,16 @@ SIGNATURES = {
                   C.c_float, _u32, er_buffer]),
     "er_hip_kv8_attention_workspace": (
         C.c_int, [_ctx_p, _p(er_kv8_cache), _p(er_kv8_batch), _u32, C.POINTER(_u64)]),
+    "er_hip_kv8_attention_masked": (
+        C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_head_rows), _p(er_head_rows), _u32,
+                  C.c_float, _u32, _u32, _p(er_drafts), er_buffer]),
+    "er_hip_kv8_accept": (
+        C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_drafts), er_buffer, er_buffer, er_buffer,
+                  er_buffer, er_buffer]),
+    "er_hip_choose_logits": (
+        C.c_int, [_ctx_p, _stream, er_buffer, _u32, _u32, _u32, _p(er_logit_rules), _p(er_drafts), er_buffer, er_buffer,
+                  er_buffer]),
+    "er_hip_choose_logits_workspace": (C.c_int, [_ctx_p, _u32, _u32, C.POINTER(_u64)]),
     "er_gguf_parse_memory": (C.c_int, [C.c_void_p, C.c_uint64, _u32, C.POINTER(C.c_void_p)]),
     "er_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "er_gguf_close": (None, [C.c_void_p]),

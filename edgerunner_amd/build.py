@@ -43,7 +43,8 @@ SYNTH = PKG / "liber_synth.so"
 CODE_OBJECT = BUILD / "er_kernels.hsaco"
 PROBE_CODE_OBJECT = BUILD / "er_kernels_probe.hsaco"
 KV8_CODE_OBJECT = BUILD / "er_kv8.hsaco"  # the 8-bit cache's kernels, the same in both libraries
-HOST_SOURCES = ("er_hip.cpp", "er_kv8.cpp", "er_gguf.cpp")
+DRAFT_CODE_OBJECT = BUILD / "er_draft.hsaco"  # attention under masks, drafts, logits; the same in both
+HOST_SOURCES = ("er_hip.cpp", "er_kv8.cpp", "er_draft.cpp", "er_gguf.cpp")
 PROBE_DEFINES = ["-DER_WITH_PROBES=1"]
 
 
@@ -69,12 +70,19 @@ def build_kv8_code_object() -> Path:
     return KV8_CODE_OBJECT
 
 
+def build_draft_code_object() -> Path:
+    BUILD.mkdir(exist_ok=True)
+    _run(_code_object_cmd(DRAFT_CODE_OBJECT, source="er_draft.hip"))
+    return DRAFT_CODE_OBJECT
+
+
 def build_code_objects() -> None:
-    """The product and the measurement code objects and the 8-bit cache's,
-    compiled concurrently (one hipcc process each)."""
+    """The product and the measurement code objects, the 8-bit cache's and the
+    drafts', compiled concurrently (one hipcc process each)."""
     BUILD.mkdir(exist_ok=True)
     cmds = [_code_object_cmd(CODE_OBJECT), _code_object_cmd(PROBE_CODE_OBJECT, PROBE_DEFINES),
-            _code_object_cmd(KV8_CODE_OBJECT, source="er_kv8.hip")]
+            _code_object_cmd(KV8_CODE_OBJECT, source="er_kv8.hip"),
+            _code_object_cmd(DRAFT_CODE_OBJECT, source="er_draft.hip")]
     procs = []
     for c in cmds:
         print("+", " ".join(c), flush=True)
@@ -85,8 +93,8 @@ def build_code_objects() -> None:
 
 
 def _blob_source(code_object: Path) -> str:
-    """Assembly that embeds the code object as er_kernels_blob[_end] and the
-    8-bit cache's as er_kv8_blob."""
+    """Assembly that embeds the code object as er_kernels_blob[_end], the 8-bit
+    cache's as er_kv8_blob and the drafts' as er_draft_blob."""
     return ("    .section .rodata\n"
             "    .balign 4096\n"
             "    .globl er_kernels_blob\n"
@@ -99,6 +107,11 @@ def _blob_source(code_object: Path) -> str:
             "    .globl er_kv8_blob\n"
             "er_kv8_blob:\n"
             f"    .incbin \"{KV8_CODE_OBJECT}\"\n"
+            "    .byte 0\n"
+            "    .balign 4096\n"
+            "    .globl er_draft_blob\n"
+            "er_draft_blob:\n"
+            f"    .incbin \"{DRAFT_CODE_OBJECT}\"\n"
             "    .byte 0\n"
             "    .section .note.GNU-stack,\"\",@progbits\n")
 
@@ -132,7 +145,7 @@ SAN_FLAGS = ["-fsanitize=address,undefined", "-fno-sanitize-recover=undefined", 
 
 def build_sanitized(out_dir: Path) -> tuple[Path, Path]:
     """AddressSanitizer + UndefinedBehaviorSanitizer builds of the host code:
-    the C-ABI library (er_hip.cpp, er_kv8.cpp, er_gguf.cpp, with the gfx950
+    the C-ABI library (er_hip.cpp, er_kv8.cpp, er_draft.cpp, er_gguf.cpp, with the gfx950
     code objects embedded unchanged) and the CPU oracle.  For CPU runs of the host-side
     tests (argument validation, GGUF parsing); the GPU kernels are never
     built with a sanitizer.  Returns (library, oracle library)."""
@@ -141,6 +154,8 @@ def build_sanitized(out_dir: Path) -> tuple[Path, Path]:
         build_code_object()
     if not KV8_CODE_OBJECT.exists():
         build_kv8_code_object()
+    if not DRAFT_CODE_OBJECT.exists():
+        build_draft_code_object()
     blob = out_dir / "er_blob.S"
     blob.write_text(_blob_source(CODE_OBJECT))
     blob_o = out_dir / "er_blob.o"

@@ -17,6 +17,7 @@
 #endif
 #include "er_error.h"
 #include "er_gemv_cfg.h"
+#include "er_draft_host.h"
 #include "er_kv8_host.h"
 #include "er_scratch.h"
 
@@ -276,6 +277,7 @@ struct er_hip_ctx {
     // entry points pass it to kernels in place of caller scratch buffers
     void *scratch = nullptr;
     er_detail::Kv8Kernels kv8;  // the 8-bit cache's kernels (er_kv8.cpp)
+    er_detail::DraftKernels draft;  // attention under masks, drafts, logits (er_draft.cpp)
     er_device_info info{};
 };
 
@@ -301,10 +303,11 @@ er_status bind_device(const er_hip_ctx *ctx) {
 
 }  // namespace
 
-// what er_kv8.cpp needs of a context
+// what er_kv8.cpp and er_draft.cpp need of a context
 namespace er_detail {
 
 const Kv8Kernels &kv8_of(const er_hip_ctx *ctx) { return ctx->kv8; }
+const DraftKernels &draft_of(const er_hip_ctx *ctx) { return ctx->draft; }
 int cu_count_of(const er_hip_ctx *ctx) { return ctx->cu_count; }
 er_status bind_device_of(const er_hip_ctx *ctx) { return bind_device(ctx); }
 
@@ -1904,9 +1907,10 @@ er_status er_hip_create(int device, er_hip_ctx **out_ctx) {
                     return fail(ER_ERR_FUNCTION_NOT_FOUND, "functionNotFound(%s): %s", name, hipGetErrorString(e));
                 }
             }
-    // Now rather than at their first call, which may be recorded.  A context whose cache kernels do not load
-    // has everything else; their calls say so.
+    // Now rather than at their first call, which may be recorded.  A context whose cache or draft kernels do not
+    // load has everything else; their calls say so.
     (void)er_detail::kv8_load(ctx->kv8);
+    (void)er_detail::draft_load(ctx->draft);
     set_tok_mode(ctx, std::getenv("ER_HIP_GEMV_TOK"));
     if (const char *gv = std::getenv("ER_HIP_GEMM_VARIANT")) ctx->gemm_variant = std::atoi(gv);
     if (const char *fv = std::getenv("ER_HIP_GEMV_FP32")) ctx->gemv_fp32 = std::atoi(fv);
@@ -1954,6 +1958,7 @@ void er_hip_destroy(er_hip_ctx *ctx) {
     if (bind_device(ctx) == ER_OK) {
         if (ctx->module) (void)hipModuleUnload(ctx->module);
         er_detail::kv8_unload(ctx->kv8);
+        er_detail::draft_unload(ctx->draft);
     }
     delete ctx;
 }

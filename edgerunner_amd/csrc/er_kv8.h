@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #define ER_KV8_THREADS 256
+#define ER_MOST_DRAFTS 1024  // rows of a sequence that are drafts
 #define ER_KV8_ROW_PARTS 16  // parts that the join of a whole row takes at the most
 
 // Norm and rotation of one kind of heads.
@@ -57,6 +58,7 @@ struct ErAppendArgs {
 };
 
 struct ErAttendArgs {
+    static constexpr bool MASKED = false;
     ErKv8Cache c;
     ErKv8Batch b;
     const float *q;
@@ -76,4 +78,13 @@ struct ErAttendArgs {
     uint32_t window;          // 0: none
     uint32_t half;            // bf16 output
     float scale;              // times log2(e)
+};
+
+// Attention where not every earlier token is visible.
+struct ErMaskedArgs : ErAttendArgs {
+    static constexpr bool MASKED = true;
+    const uint32_t *seen;     // [rows][words]: bit j, the sequence's row j is visible; null: no drafts, the rows are causal
+    const int32_t *position;  // [rows]; read where there are drafts and a window
+    uint32_t words;
+    uint32_t sinks;           // first tokens that stay visible
 };

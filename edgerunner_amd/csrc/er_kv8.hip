@@ -544,8 +544,10 @@ ER_DEV void kv8_append(const ErAppendArgs &p) {
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_append_d##D(ErAppendArgs p) {              \
         kv8_append<D>(p);                                                                                          \
     }
+#ifndef ER_KV8_MASKED
 ER_KV8_KERNELS(64)
 ER_KV8_KERNELS(128)
 ER_KV8_KERNELS(256)
+#endif
 
 #include "er_kv8_attn.hip"

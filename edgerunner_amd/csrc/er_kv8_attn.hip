@@ -61,20 +61,73 @@ ER_DEV uint32_t nan_codes(uint32_t c) {
     return (top << 1) - (top >> 7);
 }
 
-// A column of a tile: its row, its query head, and the tokens [lo, hi) that it sees.
+// A column of a tile: its row, its query head, and the tokens [lo, hi) that it
+// sees; under masks (ErMaskedArgs) also the sinks in front of hi, and the
+// drafts that drafts_at gives.
 struct Column {
     int row, lo, hi;
     uint32_t head;
 };
-ER_DEV Column column_of(const ErAttendArgs &p, const Sequence &q, uint32_t kvHead, uint32_t col) {
+template <class A>
+ER_DEV Column column_of(const A &p, const Sequence &q, uint32_t kvHead, uint32_t col) {
     Column c;
     const uint32_t r = col / p.group;
     const int pos = q.len - q.n + (int)r;
     c.row = q.row0 + (int)r;
     c.head = kvHead * p.group + (col - r * p.group);
     c.hi = max(pos + 1, 0);
-    c.lo = p.window && c.hi > (int)p.window ? c.hi - (int)p.window : 0;
+    if constexpr (A::MASKED) {
+        int from = c.hi;  // behind the last token that the window counts
+        if (p.seen) {
+            const int base = q.len - q.n;
+            c.hi = max(base, 0);
+            if (p.window) from = min(max(p.position[c.row], base), q.len - 1) + 1;
+        }
+        c.lo = p.window && from > (int)p.window ? from - (int)p.window : 0;
+    } else {
+        c.lo = p.window && c.hi > (int)p.window ? c.hi - (int)p.window : 0;
+    }
     return c;
+}
+// Whether tokens from .. to - 1 lie in [lo, hi) or, in front of hi, among the sinks.
+template <class A>
+ER_DEV bool within(const A &p, int from, int to, int lo, int hi) {
+    if constexpr (A::MASKED) return to <= hi && (from >= lo || to <= (int)p.sinks);
+    return from >= lo && to <= hi;
+}
+// Whether one of the tokens from .. to - 1 does.
+template <class A>
+ER_DEV bool touches(const A &p, int from, int to, int lo, int hi) {
+    if constexpr (A::MASKED) return from < hi && (to > lo || from < (int)p.sinks);
+    return from < hi && to > lo;
+}
+// The same for one token of a column, and a bit for each of the tokens at ..
+// at + 31.
+template <class A>
+ER_DEV bool sees(const A &p, const Column &c, int tok) {
+    if constexpr (A::MASKED) return within(p, tok, tok + 1, c.lo, c.hi);
+    return tok >= c.lo && tok < c.hi;
+}
+ER_DEV uint32_t bits_below(int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; }
+ER_DEV uint32_t sees32(const ErMaskedArgs &p, const Column &c, int at) {
+    return bits_below(c.hi - at) & (~bits_below(c.lo - at) | bits_below((int)p.sinks - at));
+}
+// Which of the tokens at .. at + 31 are drafts that a column's row sees, a bit
+// each: 32 bits of the row's mask from any bit on.
+template <class A>
+ER_DEV uint32_t drafts_at(const A &p, const Sequence &q, const Column &c, int at) {
+    if constexpr (A::MASKED) {
+        const int base = q.len - q.n, from = at - base;
+        // a row in front of the first token (base < 0) sees nothing
+        if (!p.seen || from <= -32 || from >= q.n || c.row - q.row0 + base < 0) return 0;
+        const uint32_t *words = p.seen + (size_t)c.row * p.words;
+        const int k = from >> 5;  // -1 where the tile begins in front of the drafts
+        const uint32_t lo = k >= 0 ? words[k] : 0u, hi = 32 * (k + 1) < q.n ? words[k + 1] : 0u;
+        const uint32_t v = __builtin_amdgcn_alignbit(hi, lo, (uint32_t)from & 31u);
+        return q.n - from < 32 ? v & ((1u << (q.n - from)) - 1u) : v;
+    } else {
+        return 0;
+    }
 }
 
 // A column's query times the softmax's scale (and log2 e) as B operands: eight
@@ -184,11 +237,11 @@ struct NarrowTile {
 struct NarrowPages {
     int page[2];
 };
-template <int P>
-ER_DEV NarrowPages narrow_pages(const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
+template <int P, class A>
+ER_DEV NarrowPages narrow_pages(const A &p, uint32_t s, int T, int lo, int hi) {
     NarrowPages w;
     constexpr int AT = P < 32 ? 16 : 32;  // tokens that one entry covers
-    auto page = [&](int at) { return at < hi && at + AT > lo ? uniform(page_of(p.b, p.c, s, at)) : -1; };
+    auto page = [&](int at) { return touches(p, at, at + AT, lo, hi) ? uniform(page_of(p.b, p.c, s, at)) : -1; };
     w.page[0] = page(T);
     w.page[1] = P < 32 ? page(T + 16) : w.page[0];
     return w;
@@ -256,14 +309,38 @@ struct NarrowState {
     bool nans;        // a masked tile held NaN codes
 };
 
-// Tokens that some column sees, and tokens that every column sees.
+// Tokens that some column sees, and tokens that every column sees, but for sinks.
 struct Spans {
     int anyLo, anyHi, allLo, allHi;
 };
-ER_DEV Spans spans_of(const ErAttendArgs &p, const Sequence &q, uint32_t firstCol, uint32_t lastCol) {
+template <class A>
+ER_DEV Spans spans_of(const A &p, const Sequence &q, uint32_t firstCol, uint32_t lastCol) {
+    if constexpr (A::MASKED) {
+        if (p.seen) {
+            // positions lie between the first and the last row's token, and windows end there
+            const int base = q.len - q.n, window = (int)p.window;
+            return Spans{window ? max(base + 1 - window, 0) : 0, q.len, window ? max(q.len - window, 0) : 0, max(base, 0)};
+        }
+    }
     const Column a = column_of(p, q, 0, firstCol), b = column_of(p, q, 0, lastCol);
     return Spans{a.lo, b.hi, b.lo, a.hi};
 }
+// The tokens that some column sees, in steps of 64: the first `head` of the
+// sequence, and behind them, `skip` further on, the rest.  Where the window
+// begins inside or right behind the sinks' last step there is no gap.
+struct Reach {
+    int head, skip;
+};
+template <class A>
+ER_DEV Reach reach_of(const A &p, const Spans &w) {
+    const int lo = w.anyLo & ~63;
+    if constexpr (A::MASKED) {
+        const int head = (min((int)p.sinks, w.anyHi) + 63) & ~63;
+        return lo > head ? Reach{head, lo - head} : Reach{0, 0};
+    }
+    return Reach{0, lo};
+}
+ER_DEV int token_of(const Reach &r, int x) { return x < r.head ? x : x + r.skip; }
 
 // Moves a column's reference up to its scores' largest.
 template <int N, typename ACC>
@@ -316,9 +393,10 @@ ER_DEV void follow_scale(const ScaleRange &r, float &top, float &vref, float &vi
 // st.nans remembers that there were some, and mark_nans brings them back.
 // vtop: the largest reference of the value scales, for masked tiles, which come
 // last.
-template <int D, int TERMS, bool MASKED>
-ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
-                          int lo, int hi, const Spans &w, uint32_t g, float &vtop) {
+// shown32 (under masks): what the column sees of the tile, from the lane's first token on.
+template <int D, int TERMS, bool MASKED, class A>
+ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, const A &p,
+                          int T, const Column &c, uint32_t shown32, const Spans &w, uint32_t g, float &vtop) {
     const bool ok0 = !MASKED || t.page[0] >= 0, ok1 = !MASKED || t.page[1] >= 0;
     f32x4 s[2];
 #pragma unroll
@@ -338,14 +416,19 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + 16 * (i / 4) + 4 * (int)g + (i & 3);
-            const bool ok = i < 4 ? ok0 : ok1, shown = ok && tok >= lo && tok < hi;
+            const bool ok = i < 4 ? ok0 : ok1;
+            bool shown;
+            if constexpr (A::MASKED)
+                shown = ok && (shown32 >> (16 * (i / 4) + (i & 3)) & 1u);
+            else
+                shown = ok && sees(p, c, tok);
             st.seen |= shown;
             s[i / 4][i & 3] = shown ? s[i / 4][i & 3] : -__builtin_inff();
 #pragma unroll
             for (int d = 0; d < D / 64; ++d) {
-                const uint32_t c = ok && tok >= w.anyLo && tok < w.anyHi ? t.v[d][i] : 0u, nan = nan_codes(c);
+                const uint32_t v = ok && touches(p, tok, tok + 1, w.anyLo, w.anyHi) ? t.v[d][i] : 0u, nan = nan_codes(v);
                 st.nans |= nan != 0;
-                t.v[d][i] = c & ~nan;
+                t.v[d][i] = v & ~nan;
             }
         }
     }
@@ -382,10 +465,12 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
 
 // The sums that a visible NaN code of the masked tiles belongs to become NaN.
 // Reached only where such a tile held one, so it takes the tokens one by one.
-template <int D>
-ER_DEV void mark_nans(NarrowState<D> &st, const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
-                      int hi, uint32_t g) {
-    for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
+template <int D, class A>
+ER_DEV void mark_nans(NarrowState<D> &st, const A &p, uint32_t s, const Sequence &q, uint32_t h, const Reach &r, int begin,
+                      int end, const Column &c, uint32_t g) {
+    for (int at = A::MASKED ? begin : max(begin, c.lo); at < (A::MASKED ? end : min(end, c.hi)); ++at) {
+        const int tok = A::MASKED ? token_of(r, at) : at;
+        if (A::MASKED && !(sees(p, c, tok) || (drafts_at(p, q, c, tok) & 1u))) continue;
         const int page = page_of(p.b, p.c, s, tok);
         if (page < 0) continue;
         const size_t slot = (((size_t)page * p.c.heads + h) << p.c.shift) + ((uint32_t)tok & ((1u << p.c.shift) - 1u));
@@ -419,11 +504,12 @@ struct Shares {
     uint32_t quota, total;
     bool aligned;
 };
-ER_DEV uint32_t steps_of(const ErAttendArgs &p, const Sequence &q) {
+template <class A>
+ER_DEV uint32_t steps_of(const A &p, const Sequence &q) {
     if (q.n == 0) return 0;
     const Spans w = spans_of(p, q, 0, (uint32_t)q.n * p.group - 1);
     // rows that see nothing take a step all the same, which writes their zeros
-    return max(1u, ((uint32_t)max(w.anyHi - (w.anyLo & ~63), 0) + 63u) >> 6);
+    return max(1u, ((uint32_t)max(w.anyHi - reach_of(p, w).skip, 0) + 63u) >> 6);
 }
 // Column blocks of a sequence and key/value head.
 ER_DEV uint32_t blocks_of(const ErAttendArgs &p, const Sequence &q) { return ((uint32_t)q.n * p.group + 15u) >> 4; }
@@ -453,7 +539,8 @@ struct LaneSequence {
     Sequence q;
     uint32_t steps;
 };
-ER_DEV LaneSequence lane_sequence(const ErAttendArgs &p, uint32_t s) {
+template <class A>
+ER_DEV LaneSequence lane_sequence(const A &p, uint32_t s) {
     LaneSequence l = {};
     if (s < p.b.sequences) {
         l.q = sequence_of(p.b, s);
@@ -461,7 +548,8 @@ ER_DEV LaneSequence lane_sequence(const ErAttendArgs &p, uint32_t s) {
     }
     return l;
 }
-ER_DEV LaneSequence lane_sequence_at(const ErAttendArgs &p, const LaneSequence &first, uint32_t s) {
+template <class A>
+ER_DEV LaneSequence lane_sequence_at(const A &p, const LaneSequence &first, uint32_t s) {
     if (s >= 64) return lane_sequence(p, s);
     LaneSequence l;
     l.q.row0 = (int)lane_of((uint32_t)first.q.row0, s);
@@ -470,7 +558,8 @@ ER_DEV LaneSequence lane_sequence_at(const ErAttendArgs &p, const LaneSequence &
     l.steps = lane_of(first.steps, s);
     return l;
 }
-ER_DEV Shares shares_of(const ErAttendArgs &p, const LaneSequence &first, uint32_t lane) {
+template <class A>
+ER_DEV Shares shares_of(const A &p, const LaneSequence &first, uint32_t lane) {
     uint32_t plain = first.steps * blocks_of(p, first.q), padded = shared_length(p, first.steps, true) * blocks_of(p, first.q);
     for (uint32_t at = 64; at < p.b.sequences; at += 64) {
         const LaneSequence l = lane_sequence(p, at + lane);
@@ -486,7 +575,8 @@ ER_DEV Shares shares_of(const ErAttendArgs &p, const LaneSequence &first, uint32
     return s;
 }
 // The sequence that step `at` of the line belongs to, and where it begins.
-ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bool aligned, uint32_t at, uint32_t lane,
+template <class A>
+ER_DEV uint32_t sequence_at(const A &p, const LaneSequence &first, bool aligned, uint32_t at, uint32_t lane,
                             uint32_t &begins) {
     uint32_t before = 0;
     for (uint32_t s0 = 0;; s0 += 64) {
@@ -511,8 +601,8 @@ ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bo
 // steps are the columns' outputs; else they go to part `part`.  64 ragged users
 // of an 8B layer (675 MB of codes) take 123 us, 131072 tokens of one user (268
 // MB) 50 us: 5.4 to 5.5 TB/s, a large read's rate.
-template <int D, int P, int TERMS>
-ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t col0, uint32_t from,
+template <int D, int P, int TERMS, class A>
+ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t col0, uint32_t from,
                         uint32_t to, bool complete, uint32_t part, float *lds) {
     // what follows from the thread's index is formed for each unit: kept from one to the next, it takes registers
     // that head width 256 needs for its tile
@@ -521,21 +611,26 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     const uint32_t lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t every = (uint32_t)q.n * p.group, cols = min(every - col0, 16u);
     const Spans w = spans_of(p, q, col0, col0 + cols - 1);
-    const int base = column_of(p, q, h, 0).lo & ~63;  // the steps are those of all columns
-    const int begin = base + 64 * (int)from, end = min(w.anyHi, base + 64 * (int)to);
+    // The steps are those of all columns.  Places are tokens; under masks they
+    // are counted without the gap behind the sinks.
+    const Reach reach = A::MASKED ? reach_of(p, spans_of(p, q, 0, every - 1)) : Reach{};
+    const int base = A::MASKED ? 0 : column_of(p, q, h, 0).lo & ~63;
+    const int begin = base + 64 * (int)from, end = min(A::MASKED ? w.anyHi - reach.skip : w.anyHi, base + 64 * (int)to);
+    auto token_at = [&](int at) { return A::MASKED ? token_of(reach, at) : at; };
     const Column c = column_of(p, q, h, col0 + min(n, cols - 1));
 
     // The tiles that all columns see whole go through a loop of their own, two
     // in registers at a time; the few others (ends, missing pages) follow one
     // by one.  A branch between the two around the sums would have them copied.
     auto whole = [&](const NarrowPages &k, int T) {
-        return k.page[0] >= 0 && k.page[1] >= 0 && T >= w.allLo && T + 32 <= w.allHi;
+        return k.page[0] >= 0 && k.page[1] >= 0 && within(p, token_at(T), token_at(T) + 32, w.allLo, w.allHi);
     };
+    auto pages_of = [&](int T) { return narrow_pages<P>(p, s, token_at(T), w.anyLo, A::MASKED ? w.anyHi : end); };
     NarrowPages pages;
     int rest = end;  // the first tile that is not whole
     auto next_whole = [&](int T) {  // the wave's next whole tile from T on, its pages in `pages`; `end` if there is none
         for (; T < end; T += 128) {
-            pages = narrow_pages<P>(p, s, T, w.anyLo, end);
+            pages = pages_of(T);
             if (whole(pages, T)) return T;
             rest = min(rest, T);
         }
@@ -544,7 +639,7 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     NarrowTile<D> t0, t1;
     int T = next_whole(begin + 32 * (int)wave);
     const NarrowPages firstPages = pages;
-    if (D < 256 && T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
+    if (D < 256 && T < end) load_narrow<D, P>(t0, firstPages, p, h, token_at(T), n, g);
     int U = next_whole(T + 128);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
@@ -554,31 +649,34 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     st.m = ER_NO_MAX;
     if constexpr (D < 256) {
         while (T < end) {
-            if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
+            if (U < end) load_narrow<D, P>(t1, pages, p, h, token_at(U), n, g);
             T = next_whole(U + 128);
-            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false, A>(st, t0, qb, qf, p, 0, c, 0, w, g, vtop);
             if (U >= end) break;
-            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, token_at(T), n, g);
             U = next_whole(T + 128);
-            attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false, A>(st, t1, qb, qf, p, 0, c, 0, w, g, vtop);
         }
     } else {
         // 16 KB a tile: one in registers, and twice the waves; the first waits
         // until the query's fp32 values have left theirs
-        if (T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
+        if (T < end) load_narrow<D, P>(t0, firstPages, p, h, token_at(T), n, g);
         while (T < end) {
-            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false, A>(st, t0, qb, qf, p, 0, c, 0, w, g, vtop);
             T = U;
-            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, token_at(T), n, g);
             U = next_whole(T + 128);
         }
     }
     vtop = st.vref;  // it has only gone up
     bool second = false;  // of a tile whose halves' value scales lie far apart: a column may see the small one alone
     for (T = rest; T < end;) {
-        pages = narrow_pages<P>(p, s, T, w.anyLo, end);
+        pages = pages_of(T);
         if (!whole(pages, T) && (pages.page[0] >= 0 || pages.page[1] >= 0)) {
-            load_narrow<D, P>(t0, pages, p, h, T, n, g);
+            const int token = token_at(T);
+            uint32_t shown = 0;
+            if constexpr (A::MASKED) shown = (sees32(p, c, token) | drafts_at(p, q, c, token)) >> (4 * g);
+            load_narrow<D, P>(t0, pages, p, h, token, n, g);
             if constexpr (P < 32) {
                 ScaleRange r = {0u, ~0u};
                 r.add(__float_as_uint(uniform(t0.vs[0])));
@@ -589,12 +687,12 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
                     second = !second;
                 }
             }
-            attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g, vtop);
+            attend_narrow<D, TERMS, true, A>(st, t0, qb, qf, p, token, c, shown, w, g, vtop);
         }
         if (!second) T += 128;
     }
     // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
-    if (__any(st.nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, g);
+    if (__any(st.nans)) mark_nans<D>(st, p, s, q, h, reach, begin, end, c, g);
 
     // the waves' columns, [wave][column][D + 4], and their references and sums (-1: nothing seen)
     constexpr uint32_t PITCH = D + 4;
@@ -648,8 +746,8 @@ ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, ui
     }
 }
 
-template <int D, int P, int TERMS>
-ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
+template <int D, int P, int TERMS, class A>
+ER_DEV void kv8_attend_narrow(const A &p, float *lds) {
     const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
     if (p.shares == 0) {
         const uint32_t block = blockIdx.x % p.tiles, h = blockIdx.x / p.tiles % H, s = blockIdx.x / p.tiles / H;
@@ -736,19 +834,19 @@ struct PageWindow {
     int page;
     float ks, vs;
 };
-template <int P>
-ER_DEV void fill_window(PageWindow<P> &w, const ErAttendArgs &p, uint32_t s, uint32_t h, int T, int lo, int end,
+template <int P, class A>
+ER_DEV void fill_window(PageWindow<P> &w, const A &p, uint32_t s, uint32_t h, int T, int lo, int end,
                         uint32_t lane) {
     const int tok = T + P * (int)lane;
     w.first = T / P;
-    w.page = tok < end && tok + P > lo ? page_of(p.b, p.c, s, tok) : -1;
+    w.page = touches(p, tok, tok + P, lo, end) ? page_of(p.b, p.c, s, tok) : -1;
     const size_t block = (size_t)(uint32_t)max(w.page, 0) * p.c.heads + h;
     w.ks = p.c.ks[block];
     w.vs = p.c.vs[block];
 }
 // The pages of the tile at T; tiles are asked for in order.
-template <int P>
-ER_DEV WidePages<P> pages_at(PageWindow<P> &w, const ErAttendArgs &p, uint32_t s, uint32_t h, int T, int lo, int end,
+template <int P, class A>
+ER_DEV WidePages<P> pages_at(PageWindow<P> &w, const A &p, uint32_t s, uint32_t h, int T, int lo, int end,
                              uint32_t lane) {
     if (T / P - w.first >= 64) fill_window<P>(w, p, s, h, T, lo, end, lane);
     WidePages<P> r;
@@ -829,8 +927,8 @@ struct WideLds {
 
 // The values of a tile that some column of the workgroup does not see whole,
 // as attend_narrow's masked tiles; not 0 where there were NaN codes.
-template <int D, int P>
-ER_DEV uint32_t mask_wide(WideTile<D, P> &t, uint32_t there, int T, int lo, int hi, uint32_t tid) {
+template <int D, int P, class A>
+ER_DEV uint32_t mask_wide(WideTile<D, P> &t, const A &p, uint32_t there, int T, int lo, int hi, uint32_t tid) {
     uint32_t nan = 0;
 #pragma unroll
     for (int r = 0; r < (D + 127) / 128; ++r) {
@@ -839,7 +937,7 @@ ER_DEV uint32_t mask_wide(WideTile<D, P> &t, uint32_t there, int T, int lo, int 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + it.first + (i & 3) + 8 * (i >> 2);
-            const uint32_t c = ok && tok >= lo && tok < hi ? t.v[r][i] : 0u, nans = nan_codes(c);
+            const uint32_t c = ok && touches(p, tok, tok + 1, lo, hi) ? t.v[r][i] : 0u, nans = nan_codes(c);
             nan |= nans;
             t.v[r][i] = c & ~nans;
         }
@@ -878,10 +976,12 @@ ER_DEV float column_sum2(float v) {
 }
 
 // As the narrow kernel's.
-template <int D>
-ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
-                      int hi, uint32_t hh) {
-    for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
+template <int D, class A>
+ER_DEV void mark_nans(f32x16 (&o)[D / 32], const A &p, uint32_t s, const Sequence &q, uint32_t h, const Reach &r, int begin,
+                      int end, const Column &c, uint32_t hh) {
+    for (int at = A::MASKED ? begin : max(begin, c.lo); at < (A::MASKED ? end : min(end, c.hi)); ++at) {
+        const int tok = A::MASKED ? token_of(r, at) : at;
+        if (A::MASKED && !(sees(p, c, tok) || (drafts_at(p, q, c, tok) & 1u))) continue;
         const int page = page_of(p.b, p.c, s, tok);
         if (page < 0) continue;
         const size_t slot = (((size_t)page * p.c.heads + h) << p.c.shift) + ((uint32_t)tok & ((1u << p.c.shift) - 1u));
@@ -907,17 +1007,51 @@ ER_DEV void mark_nans(f32x16 (&o)[D / 32], const ErAttendArgs &p, uint32_t s, ui
 // (137 GFLOP) takes 187 to 193 us, up to 735 TFLOP/s, two waves a SIMD; ragged chunks behind
 // long prefixes in fp32 (two terms, 35 GFLOP of products) 75 us with the join, and the
 // prompt in fp32 270.
-template <int D, int P, int TERMS>
-ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
+// The piece of a sequence's tokens, and the row tile, of a workgroup.
+struct WidePlace {
+    uint32_t h, s, piece, tile;
+};
+ER_DEV WidePlace wide_place(const ErAttendArgs &p, uint32_t block) {
     // One row tile of all units (sequence, piece, head) after the other, each
     // begun a sequence's heads later than the one before.  Workgroups go to the
     // 8 XCDs in turn: with 8 heads (or 16, ..) an XCD's L2 serves all tiles of a
     // head, with fewer a head's tiles lie on several, and units of very
     // different lengths load all XCDs alike.  Later tiles see more, and start first.
-    const uint32_t units = p.b.sequences * p.splits * p.c.heads, round = blockIdx.x / units;
-    const uint32_t ahead = round % (p.b.sequences * p.splits) * p.c.heads, at = blockIdx.x % units;
-    const uint32_t unit = at >= ahead ? at - ahead : at + units - ahead, tile = p.tiles - 1 - round;
-    const uint32_t h = unit % p.c.heads, piece = unit / p.c.heads % p.splits, s = unit / p.c.heads / p.splits;
+    const uint32_t units = p.b.sequences * p.splits * p.c.heads, round = block / units;
+    const uint32_t ahead = round % (p.b.sequences * p.splits) * p.c.heads, at = block % units;
+    const uint32_t unit = at >= ahead ? at - ahead : at + units - ahead;
+    return WidePlace{unit % p.c.heads, unit / p.c.heads / p.splits, unit / p.c.heads % p.splits, p.tiles - 1 - round};
+}
+
+// Words of drafts that a column can see: ER_MOST_DRAFTS from any place in the
+// first one on to the end of their last 64-token tile; an odd number, so that
+// columns lie in different banks.
+#define ER_DRAFT_WORDS (ER_MOST_DRAFTS / 32 + 3)
+
+// What is seldom needed of a workgroup's place and columns is formed anew from
+// the indices of the workgroup and the thread, since the products need the registers.
+struct WideAgain {
+    WidePlace at;
+    Sequence q;
+    Column c;
+};
+template <class A>
+ER_DEV WideAgain wide_again(const A &p) {
+    uint32_t block = blockIdx.x, tid = threadIdx.x;
+    asm volatile("" : "+s"(block));
+    asm volatile("" : "+v"(tid));
+    WideAgain a;
+    a.at = wide_place(p, block);
+    a.q = sequence_of(p.b, a.at.s);
+    const uint32_t col = a.at.tile * 128 + (tid >> 6) * 32 + (tid & 31u);
+    a.c = column_of(p, a.q, a.at.h, min(col, (uint32_t)a.q.n * p.group - 1));
+    return a;
+}
+
+template <int D, int P, int TERMS, class A>
+ER_DEV void kv8_attend_wide(const A &p, WideLds<D> *lds, uint32_t (*drafts)[ER_DRAFT_WORDS]) {
+    const WidePlace block = wide_place(p, blockIdx.x);
+    const uint32_t h = block.h, s = block.s, piece = block.piece, tile = block.tile;
     const Sequence q = sequence_of(p.b, s);
     const uint32_t cols = (uint32_t)q.n * p.group, col0 = tile * 128;
     if (col0 >= cols) return;
@@ -928,11 +1062,29 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
     const Spans ww = spans_of(p, q, min(wcol0, cols - 1), min(wcol0 + 31, cols - 1));
     const Column c = column_of(p, q, h, min(wcol0 + n, cols - 1));
     const bool live = wcol0 + n < cols;
-    const int begin = (w.anyLo & ~63) + (int)(piece * p.chunk), end = min(w.anyHi, begin + (int)p.chunk);
+    // under masks a piece's tokens are counted without the gap behind the sinks
+    const Reach reach = reach_of(p, w);
+    const int place = (int)(piece * p.chunk), until = min(w.anyHi - reach.skip, place + (int)p.chunk);
+    const int begin = A::MASKED ? token_of(reach, place) : reach.skip + place;
+    const int end = !A::MASKED ? min(w.anyHi, begin + (int)p.chunk) : place < until ? token_of(reach, until - 1) + 1 : begin;
 
     f32x16 o[D / 32] = {};  // o[d][i]: value 32 d + (i & 3) + 8 (i >> 2) + 4 hh of column n, in units of vref / 128
     float m = ER_NO_MAX, l = 0.0f, vref = 0.0f, vinv = 0.0f, vtop = 0.0f;
     uint32_t seen = 0;  // not a mask, which would take two scalar registers
+    int draftsFrom = 0x7fffffff;
+    if constexpr (A::MASKED) {
+        // Drafts lie behind what all columns see.  Their bits go to LDS, 32 tokens of a column a word: formed where they are
+        // used, they take registers that the products need (head widths 64 and 256 spilled).
+        if (p.seen && end > w.allHi) {
+            draftsFrom = w.allHi & ~31;
+            const int words = (((w.anyHi + 63) & ~63) - draftsFrom) >> 5;
+            for (int i = (int)tid; i < 128 * words; i += ER_KV8_THREADS) {
+                const uint32_t col = (uint32_t)(i / words);
+                const int word = i - (int)col * words;
+                drafts[col][word] = drafts_at(p, q, column_of(p, q, h, min(col0 + col, cols - 1)), draftsFrom + 32 * word);
+            }
+        }
+    }
     if (begin < end) {
         WideTile<D, P> t;
         PageWindow<P> window;
@@ -952,7 +1104,7 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                 ScaleRange range = {0u, ~0u};
 #pragma unroll
                 for (int i = 0; i < pages.N; ++i) range.add(now.vs[i]);
-                if (range.apart() && !(now.there == now.ALL && next >= w.allLo && next + 64 <= w.allHi)) {
+                if (range.apart() && !(now.there == now.ALL && within(p, next, next + 64, w.allLo, w.allHi))) {
                     part = max(part, 1u);
 #pragma unroll
                     for (int i = 0; i < pages.N; ++i) pages.page[i] = part >> i & 1u ? pages.page[i] : -1;
@@ -961,7 +1113,10 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                 }
             }
             load_wide<D, P>(t, pages, p, h, tid);
-            if (part == 0) next += 64;
+            if (part == 0) {
+                next += 64;
+                if constexpr (A::MASKED) next += next == reach.head ? reach.skip : 0;
+            }
         };
         fetch();
         h8 qb[TERMS][D / 16];
@@ -969,10 +1124,10 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                                                    16 * hh, 32, 8, qb, column_max2);
         uint32_t nans = 0;
         auto whole = [&](const WideParts<P> &k, const Spans &w, int T) {
-            return k.there == k.ALL && T >= w.allLo && T + 64 <= w.allHi;
+            return k.there == k.ALL && within(p, T, T + 64, w.allLo, w.allHi);
         };
         auto bring = [&](uint32_t to) {  // the tile in `t` into LDS
-            if (!whole(now, w, at)) nans |= mask_wide<D, P>(t, now.there, at, w.anyLo, end, tid);
+            if (!whole(now, w, at)) nans |= mask_wide<D, P>(t, p, now.there, at, w.anyLo, end, tid);
             store_wide<D, P>(lds[to], t, tid);
         };
         bring(0);
@@ -1011,10 +1166,20 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
                 }
                 if (th == 1 && at < end) bring(buf ^ 1u);
                 if (!clear) {
+                    uint32_t bits = 0;
+                    if constexpr (A::MASKED) {
+                        bits = sees32(p, c, T + 32 * th);
+                        if (T + 32 * th >= draftsFrom) bits |= drafts[32 * wave + n][(T + 32 * th - draftsFrom) >> 5];
+                        bits >>= 4 * hh;
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int tok = T + 32 * th + 8 * (i >> 2) + 4 * (int)hh + (i & 3);
-                        const bool shown = (parts.there >> (32 * th + 16 * (i >> 3)) / P & 1u) && tok >= c.lo && tok < c.hi;
+                        bool shown;
+                        if constexpr (A::MASKED)
+                            shown = bits >> (8 * (i >> 2) + (i & 3)) & 1u;
+                        else
+                            shown = sees(p, c, T + 32 * th + 8 * (i >> 2) + 4 * (int)hh + (i & 3));
+                        shown = (parts.there >> (32 * th + 16 * (i >> 3)) / P & 1u) && shown;
                         seen |= shown ? 1u : 0u;
                         sc[i] = shown ? sc[i] : -__builtin_inff();
                     }
@@ -1060,7 +1225,18 @@ ER_DEV void kv8_attend_wide(const ErAttendArgs &p, WideLds<D> *lds) {
             parts = now;
             fetch();
         }
-        if (__syncthreads_or(nans != 0)) mark_nans<D>(o, p, s, h, begin, end, c.lo, c.hi, hh);
+        if (__syncthreads_or(nans != 0)) {
+            if constexpr (A::MASKED) {
+                const WideAgain a = wide_again(p);
+                const uint32_t last = min(a.at.tile * 128 + 127, (uint32_t)a.q.n * p.group - 1);
+                const Spans any = spans_of(p, a.q, a.at.tile * 128, last);
+                const Reach r = reach_of(p, any);
+                const int from = (int)(a.at.piece * p.chunk);
+                mark_nans<D>(o, p, a.at.s, a.q, a.at.h, r, from, min(any.anyHi - r.skip, from + (int)p.chunk), a.c, hh);
+            } else {
+                mark_nans<D>(o, p, s, q, h, reach, begin, end, c, hh);
+            }
+        }
     }
     l = column_sum2(l);
     seen = column_max2(seen ? 1.0f : 0.0f) > 0.0f ? 1u : 0u;
@@ -1144,8 +1320,8 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
 // One row and query head after the wide kernel (a part a piece) or the narrow
 // one (a part a workgroup that had some of the unit's steps): 9 us for 64 users
 // of 32 heads, 7 for one of 64 parts, a launch and a chain of loads.
-template <int D>
-ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
+template <int D, class A>
+ER_DEV void kv8_join(const A &p, float *lds) {
     const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
     const uint32_t lane = threadIdx.x & 63u;
     const LaneSequence first = lane_sequence(p, lane);
@@ -1217,19 +1393,31 @@ ER_DEV void kv8_join_row(const ErAttendArgs &p) {
 
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
 
+// The same code under masks goes by other names, in a code object of its own.
+#ifdef ER_KV8_MASKED
+#define ER_KV8_NAME(NAME) er_kv8_masked_##NAME
+#define ER_KV8_ARGS ErMaskedArgs
+#define ER_KV8_DRAFTS __shared__ uint32_t drafts[128][ER_DRAFT_WORDS];
+#else
+#define ER_KV8_NAME(NAME) er_kv8_##NAME
+#define ER_KV8_ARGS ErAttendArgs
+#define ER_KV8_DRAFTS uint32_t(*drafts)[ER_DRAFT_WORDS] = nullptr;
+#endif
+
 // One kernel for each head width, page size and output type.  WAVES: waves a
 // SIMD that the registers leave room for.
 #define ER_KV8_NARROW(D, P, TERMS, NAME, WAVES)                                                                    \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        er_kv8_attend_narrow_d##D##_p##P##_##NAME(ErAttendArgs p) {                                                \
+        ER_KV8_NAME(attend_narrow_d##D##_p##P##_##NAME)(ER_KV8_ARGS p) {                                                \
         __shared__ __attribute__((aligned(16))) float sums[64 * (D + 4) + 128];                                    \
         kv8_attend_narrow<D, P, TERMS>(p, sums);                                                                   \
     }
 #define ER_KV8_WIDE(D, P, TERMS, NAME, WAVES)                                                                      \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        er_kv8_attend_wide_d##D##_p##P##_##NAME(ErAttendArgs p) {                                                  \
+        ER_KV8_NAME(attend_wide_d##D##_p##P##_##NAME)(ER_KV8_ARGS p) {                                                  \
         __shared__ __attribute__((aligned(16))) WideLds<D> tiles[2];                                               \
-        kv8_attend_wide<D, P, TERMS>(p, tiles);                                                                    \
+        ER_KV8_DRAFTS                                                                                              \
+        kv8_attend_wide<D, P, TERMS>(p, tiles, drafts);                                                            \
     }
 #define ER_KV8_PAGES(D, P, NARROW, WIDE)                                                                           \
     ER_KV8_NARROW(D, P, 1, bf16, 2)                                                                                \
@@ -1246,10 +1434,10 @@ ER_KV8_PAGES(128, 16, 2, 2)
 ER_KV8_PAGES(256, 16, 1, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_d##D(ErAttendArgs p) {                \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_d##D)(ER_KV8_ARGS p) {                \
         kv8_join<D>(p, er_kv8_lds);                                                                                \
     }                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) er_kv8_join_row_d##D(ErAttendArgs p) {            \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_row_d##D)(ER_KV8_ARGS p) {            \
         kv8_join_row<D>(p);                                                                                        \
     }
 ER_KV8_JOIN(64)

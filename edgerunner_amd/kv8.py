@@ -83,6 +83,17 @@ class KV8Batch(_Descriptor):
                                            maxRows, maxKvLen), pageTable, kvLen, rowStart)
 
 
+class Drafts(_Descriptor):
+    """The rows of a call as a tree of drafted tokens, at most 1024 of a sequence: uint32 masks [rows][seenWords] of the rows
+    of its sequence that each sees (its ancestors and itself), and int32 positions, parents (index in the sequence, -1:
+    none) and tokens [rows], each where an operator reads it."""
+
+    def __init__(self, seen: Optional[Buffer], seenWords: int, position: Optional[Buffer] = None,
+                 parent: Optional[Buffer] = None, token: Optional[Buffer] = None):
+        super().__init__(_ffi.er_drafts(_raw(seen), _raw(position), _raw(parent), _raw(token), seenWords), seen, position,
+                         parent, token)
+
+
 class _Kernel:
     entry = ""
 
@@ -135,9 +146,32 @@ class KV8AttentionKernel(_Kernel):
         return int(n.value)
 
     def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, q: HeadRows, out: HeadRows,
-               scale: float, window: int = 0, workspace: Optional[Buffer] = None, outBF16: bool = False) -> None:
-        """q fp32; out fp32 or bf16; window: the latest tokens that a row sees (0: all)."""
+               scale: float, window: int = 0, workspace: Optional[Buffer] = None, outBF16: bool = False, sinks: int = 0,
+               drafts: Optional["Drafts"] = None) -> None:
+        """q fp32; out fp32 or bf16; window: the latest tokens that a row sees (0: all); sinks: the first tokens, which
+        stay visible; drafts: the rows are a tree of drafted tokens (Drafts: seen, and position under a window)."""
+        if sinks or drafts is not None:
+            status = self.lib.er_hip_kv8_attention_masked(
+                self.ctx.handle, _sh(stream), cache.ref, batch.ref, q.ref, out.ref, TYPE_BF16 if outBF16 else TYPE_F32, scale,
+                window, sinks, _ref(drafts), _raw(workspace))
+            if status:
+                check(status, self.lib)
+            return
         status = self._call(self.ctx.handle, _sh(stream), cache.ref, batch.ref, q.ref, out.ref,
                             TYPE_BF16 if outBF16 else TYPE_F32, scale, window, _raw(workspace))
+        if status:
+            check(status, self.lib)
+
+
+class KV8AcceptKernel(_Kernel):
+    """Keeps the chosen drafts: their keys and values move behind the sequence's earlier tokens."""
+
+    entry = "er_hip_kv8_accept"
+
+    def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, drafts: Drafts, chosen: Buffer, path: Buffer,
+               count: Buffer, next: Buffer, kvLen: Buffer) -> None:
+        """drafts: parent and token; chosen int32 [rows].  Writes path int32 [rows] and count, next, kvLen int32 [sequences]."""
+        status = self._call(self.ctx.handle, _sh(stream), cache.ref, batch.ref, drafts.ref, chosen.raw, path.raw, count.raw,
+                            next.raw, kvLen.raw)
         if status:
             check(status, self.lib)

@@ -525,6 +525,105 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
 er_status er_hip_kv8_attention_workspace(er_hip_ctx *ctx, const er_kv8_cache *cache, const er_kv8_batch *batch,
                                          uint32_t q_heads, uint64_t *bytes);
 
+/* ---- drafted tokens, endless streams, rules on logits ----
+ * No counterpart on the reference's quantised path.  A step that checks a tree
+ * of drafts appends them (er_hip_qk_norm_rope with their positions, then
+ * er_hip_kv8_append without rotation), attends to them with
+ * er_hip_kv8_attention_masked, chooses a token at each with
+ * er_hip_choose_logits after the LM head, and keeps what was chosen with
+ * er_hip_kv8_accept.  Where their code object did not load when the context
+ * was created, they alone fail: LIBRARY_NOT_FOUND. */
+
+/* The rows of a call as a tree of drafted tokens, in the order of its
+ * er_kv8_batch (or er_logit_rules) rows, at most 1024 of a sequence: else
+ * INVALID_VECTOR_SHAPE.  Bit j of seen[row] (word j / 32, lowest bit first):
+ * draft j of the row's sequence is visible to the row; usually its ancestors'
+ * and its own.  seen_words * 32 >= max_rows.  Each operator names the arrays
+ * that it reads; the others may be null. */
+typedef struct er_drafts {
+    er_buffer seen;      /* uint32 [rows][seen_words] */
+    er_buffer position;  /* int32 [rows]: positions of the rows' tokens, which siblings share */
+    er_buffer parent;    /* int32 [rows]: index in its sequence of the row before; -1: none */
+    er_buffer token;     /* int32 [rows] */
+    uint32_t seen_words;
+} er_drafts;
+
+/* er_hip_kv8_attention where not every earlier token is visible.  With drafts
+ * NULL the row at position p sees the tokens t <= p with t < sinks or, where
+ * window is not 0, t > p - window (0: all).  With drafts it sees, of the tokens before its
+ * sequence's n rows (t < kv_len - n), those with t < sinks or t > position -
+ * window, and of the rows those that `seen` says, whatever the window; reads
+ * seen and, where window is not 0, position, which counts as no less than the
+ * first row's token (kv_len - n) and no more than the last's.  A row that
+ * nothing is visible to gets zeros.  Types, precision, workspace (of
+ * er_hip_kv8_attention_workspace), limits and errors are er_hip_kv8_attention's. */
+er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
+                                      const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
+                                      uint32_t out_type, float scale, uint32_t window, uint32_t sinks,
+                                      const er_drafts *drafts, er_buffer workspace);
+
+/* Keeps of each sequence's rows those that were chosen: the first row (the
+ * token that was known), then, as long as there is one, the lowest later row
+ * whose parent is the row kept last and whose token is chosen[] there (int32 [rows],
+ * as er_hip_choose_logits leaves it; a negative one ends the walk).  Their keys and
+ * values, wherever they lie, become the tokens behind the sequence's earlier
+ * ones: a token that changes its place is appended anew as the value that its
+ * code stands for, with er_hip_kv8_append's rule for scales; the others, and
+ * slots behind the last kept token, keep their bytes.  A token whose place or
+ * whose former place has no page is left out.  Reads parent and token of drafts;
+ * rows have no other buffers here.
+ * path (int32 [rows]): the kept rows of each sequence, in the places of its
+ * first rows, -1 in those of the others; count, next, kv_len (int32
+ * [sequences]): how many they are, the token chosen at the last one (no row:
+ * -1), and the tokens that the sequence now has.  Rows of no sequence are left
+ * as they were.  Outputs overlap neither each other nor what the call reads
+ * (kv_len is not the batch's own): INVALID_ARGUMENT.  Other errors as
+ * er_hip_kv8_append's. */
+er_status er_hip_kv8_accept(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache, const er_kv8_batch *batch,
+                            const er_drafts *drafts, er_buffer chosen, er_buffer path, er_buffer count, er_buffer next,
+                            er_buffer kv_len);
+
+/* Rules on logits.  A null data pointer leaves a rule out.  Rows row_start[s]
+ * .. row_start[s + 1] - 1 (of which the first max_rows count) are sequence s's;
+ * row_start null: row r is sequence r, and sequences and max_rows are unused. */
+typedef struct er_logit_rules {
+    er_buffer row_start;    /* int32 [sequences + 1], ascending */
+    er_buffer penalty;      /* fp32 [sequences][3]: repetition, presence, frequency */
+    er_buffer history;      /* int32 [sequences][history_stride]: tokens of the context */
+    er_buffer history_len;  /* int32 [sequences] */
+    er_buffer bias_token;   /* int32 [sequences][bias_stride] */
+    er_buffer bias;         /* fp32, the same */
+    er_buffer bias_len;     /* int32 [sequences] */
+    er_buffer allowed;      /* uint32 [rows][allowed_stride]: bit v % 32 of word v / 32; 0 forbids token v */
+    uint32_t sequences;
+    uint32_t max_rows;
+    uint32_t history_stride;
+    uint32_t bias_stride;
+    uint32_t allowed_stride; /* >= vocab / 32, rounded up */
+} er_logit_rules;
+
+/* Applies rules to logits and chooses the largest.  Row r's logit x of token v,
+ * which the row's context has c times (its sequence's history, and with drafts
+ * the tokens of the rows that `seen` says; reads seen and token), becomes
+ *   c > 0: (x > 0 ? x / repetition : x * repetition) - presence - frequency * c;
+ *   then + bias, of the last entry that v has in the sequence's list;
+ *   then -inf where v is not allowed.
+ * Formed in 64 bits, rounded once; a value that no rule changes keeps its
+ * bits.  Entries outside [0, vocab) count for no token.
+ * logits: fp32 [rows][row_stride] (row_stride >= vocab, INVALID_VECTOR_SHAPE).
+ * out: the same, and may be logits itself; null data: not written.  chosen
+ * (int32 [rows], null data: not found): the lowest token of the largest
+ * resulting value among the allowed ones, NaN never taken; -1 where none is left.
+ * rules NULL: none.  Rows of no sequence are left as they were.  With chosen,
+ * workspace holds er_hip_choose_logits_workspace bytes; calls and recorded
+ * graphs that may overlap in time need one each.  Buffers too short, or rows
+ * times slices of at least 1024 tokens beyond 2^24 - 1 -> ENCODING_FAILED; out,
+ * chosen or workspace overlapping another buffer -> INVALID_ARGUMENT. */
+er_status er_hip_choose_logits(er_hip_ctx *ctx, er_stream stream, er_buffer logits, uint32_t rows, uint32_t vocab,
+                               uint32_t row_stride, const er_logit_rules *rules, const er_drafts *drafts, er_buffer out,
+                               er_buffer chosen, er_buffer workspace);
+er_status er_hip_choose_logits_workspace(er_hip_ctx *ctx, uint32_t rows, uint32_t vocab, uint64_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif
