@@ -232,6 +232,8 @@ SIGNATURES = {
     "er_hip_kv8_attention_masked": (
         C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_head_rows), _p(er_head_rows), _u32,
                   C.c_float, _u32, _u32, _p(er_drafts), er_buffer]),
+    "er_hip_kv8_attention_masked_workspace": (
+        C.c_int, [_ctx_p, _p(er_kv8_cache), _p(er_kv8_batch), _u32, C.POINTER(_u64)]),
     "er_hip_kv8_accept": (
         C.c_int, [_ctx_p, _stream, _p(er_kv8_cache), _p(er_kv8_batch), _p(er_drafts), er_buffer, er_buffer, er_buffer,
                   er_buffer, er_buffer]),

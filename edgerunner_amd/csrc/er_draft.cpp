@@ -23,25 +23,31 @@ er_status draft_load(DraftKernels &k) {
     static const int dims[kKv8Dims] = {64, 128, 256};
     static const char *const outs[2] = {"f32", "bf16"};
     er_status st = ER_OK;
-    auto find = [&](hipFunction_t &f, const char *form, int d, int page, const char *out) {
+    char name[64];
+    auto find = [&](hipFunction_t &f, const char *form, auto... values) {
         if (st != ER_OK) return;
-        char name[64];
-        std::snprintf(name, sizeof(name), form, d, page, out);
+        std::snprintf(name, sizeof(name), form, values..., 0);
         const hipError_t r = hipModuleGetFunction(&f, k.module, name);
         if (r != hipSuccess) st = fail(ER_ERR_FUNCTION_NOT_FOUND, "functionNotFound(%s): %s", name, hipGetErrorString(r));
     };
     for (int d = 0; d < kKv8Dims; ++d) {
         for (int page = 0; page < kKv8Pages; ++page)
             for (int out = 0; out < 2; ++out) {
-                find(k.narrow[d][page][out], "er_kv8_masked_attend_narrow_d%d_p%d_%s", dims[d], 16 << page, outs[out]);
+                for (int nb = 0; nb < 2; ++nb)
+                    if (nb == 0 || dims[d] < 256)
+                        find(k.few[nb][d][page][out], "er_kv8_masked_attend_c%d_d%d_p%d_%s", nb + 1, dims[d], 16 << page, outs[out]);
                 find(k.wide[d][page][out], "er_kv8_masked_attend_wide_d%d_p%d_%s", dims[d], 16 << page, outs[out]);
             }
-        find(k.join[d], "er_kv8_masked_join_d%d", dims[d], 0, "");
-        find(k.joinRow[d], "er_kv8_masked_join_row_d%d", dims[d], 0, "");
-        find(k.accept[d], "er_kv8_accept_d%d", dims[d], 0, "");
+        for (int nb = 0; nb < (dims[d] < 256 ? 2 : 1); ++nb) {
+            find(k.joinFew[nb][d], "er_kv8_masked_join_c%d_d%d", nb + 1, dims[d]);
+            find(k.joinColumn[nb][d], "er_kv8_masked_join_column_c%d_d%d", nb + 1, dims[d]);
+        }
+        find(k.join[d], "er_kv8_masked_join_d%d", dims[d]);
+        find(k.joinRow[d], "er_kv8_masked_join_row_d%d", dims[d]);
+        find(k.accept[d], "er_kv8_accept_d%d", dims[d]);
     }
-    find(k.choose, "er_choose_slices", 0, 0, "");
-    find(k.chooseJoin, "er_choose_join", 0, 0, "");
+    find(k.choose, "er_choose_slices");
+    find(k.chooseJoin, "er_choose_join");
     if (st != ER_OK) draft_unload(k);
     return st;
 }
@@ -73,6 +79,41 @@ er_status check_drafts(const char *op, const er_drafts *d, uint32_t rows, uint32
     if (d->seen_words > kMostHeads || (uint64_t)d->seen_words * 32 < maxRows)
         return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u mask words a row for %u drafts", op, d->seen_words, maxRows);
     return check_buffer(op, "seen", d->seen, (uint64_t)rows * d->seen_words * 4, 4);
+}
+
+// How an attention call under masks is cut up: in shares as the narrow kernel's,
+// with 16 or 32 columns a wave, or as the wide kernel's.
+struct MaskedPlan : AttendPlan {
+    uint32_t blocks;  // of 16 columns that a wave has; 0: the wide kernel
+};
+MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group, uint32_t window, int cu, uint32_t sinks,
+                       bool drafts) {
+    MaskedPlan p{};
+    const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
+    // Shares against the wide kernel, us: trees of 128 columns of 32 sequences of up to 6000 tokens 149 / 196, of 192
+    // of 8 of 4000 58 / 60, of 256 (bf16) 62 / 58, of 512 of 2 of 20000 122 / 107; of 256 of width 256 of 16 of 4000
+    // 117 / 176.
+    if (cols > (c->head_dim == 256 ? 256 : 128)) {
+        (AttendPlan &)p = plan_attend(c, b, group, window, cu, sinks, drafts);
+        return p;
+    }
+    p.narrow = true;
+    p.splits = 1;
+    // 32 columns convert a tile's codes once for what 16 do twice, but leave half as many units, with twice as long a
+    // start and end: taken where even so each share has some tiles.  16 / 32, us, by 64-token steps of 16 columns a
+    // share: 1 (one user's tree) 13.8 / 16.5, 16 (three cases) 30.3 / 37.4, 29.8 / 32.4, 31.9 / 41.2, 170 (width 64)
+    // 50.0 / 48.7, 390 214 / 149, 500 229 / 145.  At width 256 they do not fit: 117 / 133.
+    const uint64_t steps = (uint64_t)b->sequences * c->kv_heads * ((cols + 15) / 16) * ((full + 63) / 64);
+    p.blocks = c->head_dim < 256 && cols > 16 && steps >= 64ull * 2 * (uint64_t)cu ? 2 : 1;
+    p.tiles = (uint32_t)((cols + 16 * p.blocks - 1) / (16 * p.blocks));
+    if (full > 512) {
+        p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
+        // by 2, 3, 4, 6 steps, us: a user of 8000 tokens 18.3, 17.0, 14.0, 15.7; where 2 leave half the workgroups without
+        // work, one user's tree of 26 drafts 13.7, 13.7, 14.6, 15.0, a window of 1020 tokens 12.4, 12.9, 12.8, 13.5
+        p.least = 4;
+        p.parts = 2ull * p.shares * 16 * p.blocks;
+    }
+    return p;
 }
 
 struct Range {
@@ -162,13 +203,37 @@ er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const e
         a.words = drafts->seen_words;
         a.position = (const int32_t *)drafts->position.data;
     }
-    const AttendPlan p = plan_attend(cache, batch, a.group, a.window, cu_count_of(ctx), a.sinks, drafts != nullptr);
+    const MaskedPlan p = plan_masked(cache, batch, a.group, a.window, cu_count_of(ctx), a.sinks, drafts != nullptr);
     a.shares = p.shares, a.least = p.least;
     a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
     const DraftKernels &kernels = draft_of(ctx);
-    const int di = dim_index(d);
-    return launch_attend(op, (p.narrow ? kernels.narrow : kernels.wide)[di][a.c.shift - 4][a.half], kernels.join[di],
-                         kernels.joinRow[di], a, p, batch, q->heads, d, workspace, stream);
+    const int di = dim_index(d), nb = (int)p.blocks - 1;
+    if (p.blocks == 0)
+        return launch_attend(op, kernels.wide[di][a.c.shift - 4][a.half],
+                             join_of(p, kernels.join[di], kernels.joinRow[di], batch->rows, q->heads), a, p, d, workspace, stream);
+    // A workgroup a column where the chip holds as many at once (8 a CU); else one for some of a row's heads.  By
+    // columns, us: 416 13.8 / 19.9, 512 29.8 / 45.3, 832 35.8 / 43.2, 1536 149 / 151, 2560 30.9 / 30.3, 6720 59 / 50
+    const uint32_t together = ER_KV8_THREADS / (d / 4);
+    JoinLaunch join = join_of(p, kernels.joinColumn[nb][di], nullptr, batch->rows, q->heads);
+    if (join.blocks > 8ull * (uint64_t)cu_count_of(ctx))
+        join = JoinLaunch{kernels.joinFew[nb][di], (uint64_t)batch->rows * ((q->heads + together - 1) / together), 0};
+    return launch_attend(op, kernels.few[nb][di][a.c.shift - 4][a.half], join, a, p, d, workspace, stream);
+}
+
+er_status er_hip_kv8_attention_masked_workspace(er_hip_ctx *ctx, const er_kv8_cache *cache, const er_kv8_batch *batch,
+                                                uint32_t q_heads, uint64_t *bytes) {
+    const char *op = "kv8_attention_masked_workspace";
+    if (!bytes) return fail(ER_ERR_INVALID_ARGUMENT, "%s: null bytes", op);
+    *bytes = 0;
+    er_status st = check_cache(op, cache);
+    if (st == ER_OK) st = check_batch(op, batch);
+    if (st == ER_OK) st = check_group(op, cache, batch, q_heads);
+    if (st == ER_OK) st = check_ctx(ctx);
+    if (st != ER_OK) return st;
+    if (batch->rows == 0 || batch->sequences == 0) return ER_OK;
+    const MaskedPlan p = plan_masked(cache, batch, q_heads / cache->kv_heads, 0, cu_count_of(ctx), 0, false);
+    *bytes = p.parts * (cache->head_dim + 2) * 4;
+    return ER_OK;
 }
 
 er_status er_hip_kv8_accept(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache, const er_kv8_batch *batch,

@@ -5,5 +5,6 @@
 #define ER_KV8_MASKED
 #include "er_kv8.hip"
 #include "er_draft.h"
+#include "er_kv8_few.hip"
 #include "er_accept.hip"
 #include "er_choose.hip"

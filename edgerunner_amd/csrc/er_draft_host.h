@@ -8,8 +8,10 @@ namespace er_detail {
 
 struct DraftKernels {
     hipModule_t module = nullptr;
-    hipFunction_t narrow[kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};  // [fp32, bf16 output]
-    hipFunction_t join[kKv8Dims] = {}, joinRow[kKv8Dims] = {}, accept[kKv8Dims] = {};
+    // [16, 32 columns a wave][..][..][fp32, bf16 output]; 32 up to width 128
+    hipFunction_t few[2][kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};
+    hipFunction_t joinFew[2][kKv8Dims] = {}, joinColumn[2][kKv8Dims] = {}, join[kKv8Dims] = {}, joinRow[kKv8Dims] = {};
+    hipFunction_t accept[kKv8Dims] = {};
     hipFunction_t choose = nullptr, chooseJoin = nullptr;
 };
 

@@ -242,8 +242,8 @@ er_status er_hip_kv8_attention(er_hip_ctx *ctx, er_stream stream, const er_kv8_c
     a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
     const Kv8Kernels &kernels = kv8_of(ctx);
     const int di = dim_index(d);
-    return launch_attend(op, (p.narrow ? kernels.narrow : kernels.wide)[di][a.c.shift - 4][a.half], kernels.join[di],
-                         kernels.joinRow[di], a, p, batch, q->heads, d, workspace, stream);
+    return launch_attend(op, (p.narrow ? kernels.narrow : kernels.wide)[di][a.c.shift - 4][a.half],
+                         join_of(p, kernels.join[di], kernels.joinRow[di], batch->rows, q->heads), a, p, d, workspace, stream);
 }
 
 }  // extern "C"

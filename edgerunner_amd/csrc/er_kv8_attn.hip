@@ -237,11 +237,11 @@ struct NarrowTile {
 struct NarrowPages {
     int page[2];
 };
-template <int P, class A>
-ER_DEV NarrowPages narrow_pages(const A &p, uint32_t s, int T, int lo, int hi) {
+template <int P>
+ER_DEV NarrowPages narrow_pages(const ErAttendArgs &p, uint32_t s, int T, int lo, int hi) {
     NarrowPages w;
     constexpr int AT = P < 32 ? 16 : 32;  // tokens that one entry covers
-    auto page = [&](int at) { return touches(p, at, at + AT, lo, hi) ? uniform(page_of(p.b, p.c, s, at)) : -1; };
+    auto page = [&](int at) { return at < hi && at + AT > lo ? uniform(page_of(p.b, p.c, s, at)) : -1; };
     w.page[0] = page(T);
     w.page[1] = P < 32 ? page(T + 16) : w.page[0];
     return w;
@@ -393,10 +393,9 @@ ER_DEV void follow_scale(const ScaleRange &r, float &top, float &vref, float &vi
 // st.nans remembers that there were some, and mark_nans brings them back.
 // vtop: the largest reference of the value scales, for masked tiles, which come
 // last.
-// shown32 (under masks): what the column sees of the tile, from the lane's first token on.
-template <int D, int TERMS, bool MASKED, class A>
-ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, const A &p,
-                          int T, const Column &c, uint32_t shown32, const Spans &w, uint32_t g, float &vtop) {
+template <int D, int TERMS, bool MASKED>
+ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[TERMS][D / 32], float qf, int T,
+                          int lo, int hi, const Spans &w, uint32_t g, float &vtop) {
     const bool ok0 = !MASKED || t.page[0] >= 0, ok1 = !MASKED || t.page[1] >= 0;
     f32x4 s[2];
 #pragma unroll
@@ -416,19 +415,14 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int tok = T + 16 * (i / 4) + 4 * (int)g + (i & 3);
-            const bool ok = i < 4 ? ok0 : ok1;
-            bool shown;
-            if constexpr (A::MASKED)
-                shown = ok && (shown32 >> (16 * (i / 4) + (i & 3)) & 1u);
-            else
-                shown = ok && sees(p, c, tok);
+            const bool ok = i < 4 ? ok0 : ok1, shown = ok && tok >= lo && tok < hi;
             st.seen |= shown;
             s[i / 4][i & 3] = shown ? s[i / 4][i & 3] : -__builtin_inff();
 #pragma unroll
             for (int d = 0; d < D / 64; ++d) {
-                const uint32_t v = ok && touches(p, tok, tok + 1, w.anyLo, w.anyHi) ? t.v[d][i] : 0u, nan = nan_codes(v);
+                const uint32_t c = ok && tok >= w.anyLo && tok < w.anyHi ? t.v[d][i] : 0u, nan = nan_codes(c);
                 st.nans |= nan != 0;
-                t.v[d][i] = v & ~nan;
+                t.v[d][i] = c & ~nan;
             }
         }
     }
@@ -465,12 +459,10 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
 
 // The sums that a visible NaN code of the masked tiles belongs to become NaN.
 // Reached only where such a tile held one, so it takes the tokens one by one.
-template <int D, class A>
-ER_DEV void mark_nans(NarrowState<D> &st, const A &p, uint32_t s, const Sequence &q, uint32_t h, const Reach &r, int begin,
-                      int end, const Column &c, uint32_t g) {
-    for (int at = A::MASKED ? begin : max(begin, c.lo); at < (A::MASKED ? end : min(end, c.hi)); ++at) {
-        const int tok = A::MASKED ? token_of(r, at) : at;
-        if (A::MASKED && !(sees(p, c, tok) || (drafts_at(p, q, c, tok) & 1u))) continue;
+template <int D>
+ER_DEV void mark_nans(NarrowState<D> &st, const ErAttendArgs &p, uint32_t s, uint32_t h, int begin, int end, int lo,
+                      int hi, uint32_t g) {
+    for (int tok = max(begin, lo); tok < min(end, hi); ++tok) {
         const int page = page_of(p.b, p.c, s, tok);
         if (page < 0) continue;
         const size_t slot = (((size_t)page * p.c.heads + h) << p.c.shift) + ((uint32_t)tok & ((1u << p.c.shift) - 1u));
@@ -558,8 +550,7 @@ ER_DEV LaneSequence lane_sequence_at(const A &p, const LaneSequence &first, uint
     l.steps = lane_of(first.steps, s);
     return l;
 }
-template <class A>
-ER_DEV Shares shares_of(const A &p, const LaneSequence &first, uint32_t lane) {
+ER_DEV Shares shares_of(const ErAttendArgs &p, const LaneSequence &first, uint32_t lane) {
     uint32_t plain = first.steps * blocks_of(p, first.q), padded = shared_length(p, first.steps, true) * blocks_of(p, first.q);
     for (uint32_t at = 64; at < p.b.sequences; at += 64) {
         const LaneSequence l = lane_sequence(p, at + lane);
@@ -575,8 +566,7 @@ ER_DEV Shares shares_of(const A &p, const LaneSequence &first, uint32_t lane) {
     return s;
 }
 // The sequence that step `at` of the line belongs to, and where it begins.
-template <class A>
-ER_DEV uint32_t sequence_at(const A &p, const LaneSequence &first, bool aligned, uint32_t at, uint32_t lane,
+ER_DEV uint32_t sequence_at(const ErAttendArgs &p, const LaneSequence &first, bool aligned, uint32_t at, uint32_t lane,
                             uint32_t &begins) {
     uint32_t before = 0;
     for (uint32_t s0 = 0;; s0 += 64) {
@@ -601,8 +591,8 @@ ER_DEV uint32_t sequence_at(const A &p, const LaneSequence &first, bool aligned,
 // steps are the columns' outputs; else they go to part `part`.  64 ragged users
 // of an 8B layer (675 MB of codes) take 123 us, 131072 tokens of one user (268
 // MB) 50 us: 5.4 to 5.5 TB/s, a large read's rate.
-template <int D, int P, int TERMS, class A>
-ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t col0, uint32_t from,
+template <int D, int P, int TERMS>
+ER_DEV void narrow_unit(const ErAttendArgs &p, uint32_t s, const Sequence &q, uint32_t h, uint32_t col0, uint32_t from,
                         uint32_t to, bool complete, uint32_t part, float *lds) {
     // what follows from the thread's index is formed for each unit: kept from one to the next, it takes registers
     // that head width 256 needs for its tile
@@ -611,26 +601,21 @@ ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, u
     const uint32_t lane = tid & 63u, wave = uniform(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t every = (uint32_t)q.n * p.group, cols = min(every - col0, 16u);
     const Spans w = spans_of(p, q, col0, col0 + cols - 1);
-    // The steps are those of all columns.  Places are tokens; under masks they
-    // are counted without the gap behind the sinks.
-    const Reach reach = A::MASKED ? reach_of(p, spans_of(p, q, 0, every - 1)) : Reach{};
-    const int base = A::MASKED ? 0 : column_of(p, q, h, 0).lo & ~63;
-    const int begin = base + 64 * (int)from, end = min(A::MASKED ? w.anyHi - reach.skip : w.anyHi, base + 64 * (int)to);
-    auto token_at = [&](int at) { return A::MASKED ? token_of(reach, at) : at; };
+    const int base = column_of(p, q, h, 0).lo & ~63;  // the steps are those of all columns
+    const int begin = base + 64 * (int)from, end = min(w.anyHi, base + 64 * (int)to);
     const Column c = column_of(p, q, h, col0 + min(n, cols - 1));
 
     // The tiles that all columns see whole go through a loop of their own, two
     // in registers at a time; the few others (ends, missing pages) follow one
     // by one.  A branch between the two around the sums would have them copied.
     auto whole = [&](const NarrowPages &k, int T) {
-        return k.page[0] >= 0 && k.page[1] >= 0 && within(p, token_at(T), token_at(T) + 32, w.allLo, w.allHi);
+        return k.page[0] >= 0 && k.page[1] >= 0 && T >= w.allLo && T + 32 <= w.allHi;
     };
-    auto pages_of = [&](int T) { return narrow_pages<P>(p, s, token_at(T), w.anyLo, A::MASKED ? w.anyHi : end); };
     NarrowPages pages;
     int rest = end;  // the first tile that is not whole
     auto next_whole = [&](int T) {  // the wave's next whole tile from T on, its pages in `pages`; `end` if there is none
         for (; T < end; T += 128) {
-            pages = pages_of(T);
+            pages = narrow_pages<P>(p, s, T, w.anyLo, end);
             if (whole(pages, T)) return T;
             rest = min(rest, T);
         }
@@ -639,7 +624,7 @@ ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, u
     NarrowTile<D> t0, t1;
     int T = next_whole(begin + 32 * (int)wave);
     const NarrowPages firstPages = pages;
-    if (D < 256 && T < end) load_narrow<D, P>(t0, firstPages, p, h, token_at(T), n, g);
+    if (D < 256 && T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
     int U = next_whole(T + 128);
     h8 qb[TERMS][D / 32];
     const float qf = load_query<D / 32, TERMS>(p.q + (size_t)c.row * p.qStride + (size_t)c.head * D, n < cols,
@@ -649,34 +634,31 @@ ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, u
     st.m = ER_NO_MAX;
     if constexpr (D < 256) {
         while (T < end) {
-            if (U < end) load_narrow<D, P>(t1, pages, p, h, token_at(U), n, g);
+            if (U < end) load_narrow<D, P>(t1, pages, p, h, U, n, g);
             T = next_whole(U + 128);
-            attend_narrow<D, TERMS, false, A>(st, t0, qb, qf, p, 0, c, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
             if (U >= end) break;
-            if (T < end) load_narrow<D, P>(t0, pages, p, h, token_at(T), n, g);
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
             U = next_whole(T + 128);
-            attend_narrow<D, TERMS, false, A>(st, t1, qb, qf, p, 0, c, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false>(st, t1, qb, qf, 0, 0, 0, w, g, vtop);
         }
     } else {
         // 16 KB a tile: one in registers, and twice the waves; the first waits
         // until the query's fp32 values have left theirs
-        if (T < end) load_narrow<D, P>(t0, firstPages, p, h, token_at(T), n, g);
+        if (T < end) load_narrow<D, P>(t0, firstPages, p, h, T, n, g);
         while (T < end) {
-            attend_narrow<D, TERMS, false, A>(st, t0, qb, qf, p, 0, c, 0, w, g, vtop);
+            attend_narrow<D, TERMS, false>(st, t0, qb, qf, 0, 0, 0, w, g, vtop);
             T = U;
-            if (T < end) load_narrow<D, P>(t0, pages, p, h, token_at(T), n, g);
+            if (T < end) load_narrow<D, P>(t0, pages, p, h, T, n, g);
             U = next_whole(T + 128);
         }
     }
     vtop = st.vref;  // it has only gone up
     bool second = false;  // of a tile whose halves' value scales lie far apart: a column may see the small one alone
     for (T = rest; T < end;) {
-        pages = pages_of(T);
+        pages = narrow_pages<P>(p, s, T, w.anyLo, end);
         if (!whole(pages, T) && (pages.page[0] >= 0 || pages.page[1] >= 0)) {
-            const int token = token_at(T);
-            uint32_t shown = 0;
-            if constexpr (A::MASKED) shown = (sees32(p, c, token) | drafts_at(p, q, c, token)) >> (4 * g);
-            load_narrow<D, P>(t0, pages, p, h, token, n, g);
+            load_narrow<D, P>(t0, pages, p, h, T, n, g);
             if constexpr (P < 32) {
                 ScaleRange r = {0u, ~0u};
                 r.add(__float_as_uint(uniform(t0.vs[0])));
@@ -687,12 +669,12 @@ ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, u
                     second = !second;
                 }
             }
-            attend_narrow<D, TERMS, true, A>(st, t0, qb, qf, p, token, c, shown, w, g, vtop);
+            attend_narrow<D, TERMS, true>(st, t0, qb, qf, T, c.lo, c.hi, w, g, vtop);
         }
         if (!second) T += 128;
     }
     // each wave marks its own sums, for the tokens of all four: the sums are joined, and NaN is NaN in any of them
-    if (__any(st.nans)) mark_nans<D>(st, p, s, q, h, reach, begin, end, c, g);
+    if (__any(st.nans)) mark_nans<D>(st, p, s, h, begin, end, c.lo, c.hi, g);
 
     // the waves' columns, [wave][column][D + 4], and their references and sums (-1: nothing seen)
     constexpr uint32_t PITCH = D + 4;
@@ -746,8 +728,8 @@ ER_DEV void narrow_unit(const A &p, uint32_t s, const Sequence &q, uint32_t h, u
     }
 }
 
-template <int D, int P, int TERMS, class A>
-ER_DEV void kv8_attend_narrow(const A &p, float *lds) {
+template <int D, int P, int TERMS>
+ER_DEV void kv8_attend_narrow(const ErAttendArgs &p, float *lds) {
     const uint32_t H = p.c.heads, lane = threadIdx.x & 63u;
     if (p.shares == 0) {
         const uint32_t block = blockIdx.x % p.tiles, h = blockIdx.x / p.tiles % H, s = blockIdx.x / p.tiles / H;
@@ -1320,8 +1302,8 @@ ER_DEV void join_parts(const ErAttendArgs &p, uint32_t parts, int row, uint32_t 
 // One row and query head after the wide kernel (a part a piece) or the narrow
 // one (a part a workgroup that had some of the unit's steps): 9 us for 64 users
 // of 32 heads, 7 for one of 64 parts, a launch and a chain of loads.
-template <int D, class A>
-ER_DEV void kv8_join(const A &p, float *lds) {
+template <int D>
+ER_DEV void kv8_join(const ErAttendArgs &p, float *lds) {
     const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
     const uint32_t lane = threadIdx.x & 63u;
     const LaneSequence first = lane_sequence(p, lane);
@@ -1393,28 +1375,28 @@ ER_DEV void kv8_join_row(const ErAttendArgs &p) {
 
 extern __shared__ __attribute__((aligned(16))) float er_kv8_lds[];
 
-// The same code under masks goes by other names, in a code object of its own.
+// One kernel for each head width, page size and output type.  WAVES: waves a
+// SIMD that the registers leave room for.  Under masks, in a code object of its
+// own, the wide kernel and its join go by other names.
 #ifdef ER_KV8_MASKED
 #define ER_KV8_NAME(NAME) er_kv8_masked_##NAME
 #define ER_KV8_ARGS ErMaskedArgs
 #define ER_KV8_DRAFTS __shared__ uint32_t drafts[128][ER_DRAFT_WORDS];
+#define ER_KV8_NARROW(D, P, TERMS, NAME, WAVES)
 #else
 #define ER_KV8_NAME(NAME) er_kv8_##NAME
 #define ER_KV8_ARGS ErAttendArgs
 #define ER_KV8_DRAFTS uint32_t(*drafts)[ER_DRAFT_WORDS] = nullptr;
-#endif
-
-// One kernel for each head width, page size and output type.  WAVES: waves a
-// SIMD that the registers leave room for.
 #define ER_KV8_NARROW(D, P, TERMS, NAME, WAVES)                                                                    \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        ER_KV8_NAME(attend_narrow_d##D##_p##P##_##NAME)(ER_KV8_ARGS p) {                                                \
+        er_kv8_attend_narrow_d##D##_p##P##_##NAME(ErAttendArgs p) {                                                \
         __shared__ __attribute__((aligned(16))) float sums[64 * (D + 4) + 128];                                    \
         kv8_attend_narrow<D, P, TERMS>(p, sums);                                                                   \
     }
+#endif
 #define ER_KV8_WIDE(D, P, TERMS, NAME, WAVES)                                                                      \
     extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS, WAVES)                                            \
-        ER_KV8_NAME(attend_wide_d##D##_p##P##_##NAME)(ER_KV8_ARGS p) {                                                  \
+        ER_KV8_NAME(attend_wide_d##D##_p##P##_##NAME)(ER_KV8_ARGS p) {                                             \
         __shared__ __attribute__((aligned(16))) WideLds<D> tiles[2];                                               \
         ER_KV8_DRAFTS                                                                                              \
         kv8_attend_wide<D, P, TERMS>(p, tiles, drafts);                                                            \
@@ -1434,10 +1416,10 @@ ER_KV8_PAGES(128, 16, 2, 2)
 ER_KV8_PAGES(256, 16, 1, 1)
 
 #define ER_KV8_JOIN(D)                                                                                             \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_d##D)(ER_KV8_ARGS p) {                \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_d##D)(ER_KV8_ARGS p) {           \
         kv8_join<D>(p, er_kv8_lds);                                                                                \
     }                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_row_d##D)(ER_KV8_ARGS p) {            \
+    extern "C" __global__ void __launch_bounds__(ER_KV8_THREADS) ER_KV8_NAME(join_row_d##D)(ER_KV8_ARGS p) {       \
         kv8_join_row<D>(p);                                                                                        \
     }
 ER_KV8_JOIN(64)

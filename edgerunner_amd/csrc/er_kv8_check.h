@@ -228,11 +228,23 @@ inline er_status check_group(const char *op, const er_kv8_cache *c, const er_kv8
     return ER_OK;
 }
 
+// How the parts of an attention call are joined.
+struct JoinLaunch {
+    hipFunction_t f;
+    uint64_t blocks;
+    uint32_t lds;
+};
+// After the wide kernel, a workgroup a row where the parts are few; else one a
+// row and head.
+inline JoinLaunch join_of(const AttendPlan &p, hipFunction_t join, hipFunction_t joinRow, uint32_t rows, uint32_t heads) {
+    if (!p.shares && p.splits <= ER_KV8_ROW_PARTS) return JoinLaunch{joinRow, rows, 0};
+    return JoinLaunch{join, (uint64_t)rows * heads, (4 * ER_KV8_THREADS + (p.shares ? p.shares : p.splits)) * 4};
+}
+
 // The launches of an attention call whose other arguments are in `a`.
 template <class ARGS>
-er_status launch_attend(const char *op, hipFunction_t attend, hipFunction_t join, hipFunction_t joinRow, ARGS &a,
-                        const AttendPlan &p, const er_kv8_batch *batch, uint32_t heads, uint32_t d, const er_buffer &workspace,
-                        er_stream stream) {
+er_status launch_attend(const char *op, hipFunction_t attend, const JoinLaunch &join, ARGS &a, const AttendPlan &p, uint32_t d,
+                        const er_buffer &workspace, er_stream stream) {
     const bool joined = p.splits > 1 || p.shares > 0;
     er_status st = ER_OK;
     if (joined) {
@@ -241,19 +253,15 @@ er_status launch_attend(const char *op, hipFunction_t attend, hipFunction_t join
         a.partO = (float *)workspace.data;
         a.partML = a.partO + p.parts * d;
     }
-    const uint64_t pairs = (uint64_t)batch->sequences * a.c.heads;
+    const uint64_t pairs = (uint64_t)a.b.sequences * a.c.heads;
     const uint64_t blocks = p.shares ? p.shares : pairs * p.splits * p.tiles;  // narrow: one split
-    const bool byRow = !p.shares && p.splits <= ER_KV8_ROW_PARTS;
-    const uint64_t joins = !joined ? 0 : byRow ? batch->rows : (uint64_t)batch->rows * heads;
     // both, before the first is queued
     st = check_blocks(op, blocks);
-    if (st == ER_OK) st = check_blocks(op, joins);
+    if (st == ER_OK && joined) st = check_blocks(op, join.blocks);
     if (st != ER_OK) return st;
     st = launch(attend, op, blocks, 0, stream, &a);
     if (st != ER_OK || !joined) return st;
-    if (byRow) return launch(joinRow, op, joins, 0, stream, &a);
-    const uint32_t most = p.shares ? p.shares : p.splits;
-    return launch(join, op, joins, (4 * ER_KV8_THREADS + most) * 4, stream, &a);
+    return launch(join.f, op, join.blocks, join.lds, stream, &a);
 }
 
 }  // namespace er_detail

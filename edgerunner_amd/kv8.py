@@ -139,11 +139,13 @@ class KV8AttentionKernel(_Kernel):
     entry = "er_hip_kv8_attention"
 
     def workspaceBytes(self, cache: KV8Cache, batch: KV8Batch, qHeads: int) -> int:
-        """Bytes of scratch that encode needs for such a batch, whatever its window and output type."""
-        n = C.c_uint64()
+        """Bytes of scratch that encode needs for such a batch, whatever its window, masks and output type."""
+        n, masked = C.c_uint64(), C.c_uint64()
         check(self.lib.er_hip_kv8_attention_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(n)),
               self.lib)
-        return int(n.value)
+        check(self.lib.er_hip_kv8_attention_masked_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(masked)),
+              self.lib)
+        return max(int(n.value), int(masked.value))
 
     def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, q: HeadRows, out: HeadRows,
                scale: float, window: int = 0, workspace: Optional[Buffer] = None, outBF16: bool = False, sinks: int = 0,

@@ -555,12 +555,15 @@ typedef struct er_drafts {
  * window, and of the rows those that `seen` says, whatever the window; reads
  * seen and, where window is not 0, position, which counts as no less than the
  * first row's token (kv_len - n) and no more than the last's.  A row that
- * nothing is visible to gets zeros.  Types, precision, workspace (of
- * er_hip_kv8_attention_workspace), limits and errors are er_hip_kv8_attention's. */
+ * nothing is visible to gets zeros.  Types, precision, limits and errors are
+ * er_hip_kv8_attention's, and so are the rules of workspace, whose bytes
+ * er_hip_kv8_attention_masked_workspace gives. */
 er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
                                       const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
                                       uint32_t out_type, float scale, uint32_t window, uint32_t sinks,
                                       const er_drafts *drafts, er_buffer workspace);
+er_status er_hip_kv8_attention_masked_workspace(er_hip_ctx *ctx, const er_kv8_cache *cache, const er_kv8_batch *batch,
+                                                uint32_t q_heads, uint64_t *bytes);
 
 /* Keeps of each sequence's rows those that were chosen: the first row (the
  * token that was known), then, as long as there is one, the lowest later row

@@ -178,6 +178,11 @@ def test_workspace_query():
     f = _ffi.load().er_hip_choose_logits_workspace
     assert f(None, 6, 0, C.byref(n)) == VEC and n.value == 0
     assert f(None, 6, 1000, C.byref(n)) == NO_CTX and f(None, 6, 1000, None) == ARG
+    n = C.c_uint64(7)
+    f = _ffi.load().er_hip_kv8_attention_masked_workspace
+    assert f(None, ref(cache()), ref(batch()), 3, C.byref(n)) == VEC and n.value == 0
+    assert f(None, ref(cache(d=96)), ref(batch()), 4, C.byref(n)) == VEC and f(None, ref(cache()), None, 4, C.byref(n)) == ARG
+    assert f(None, ref(cache()), ref(batch()), 4, C.byref(n)) == NO_CTX and f(None, ref(cache()), ref(batch()), 4, None) == ARG
 
 
 # ---------------------------------------------------------------- launches
@@ -189,7 +194,8 @@ def host(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", str(ROCM / "include"),
                     "-I", str(ROOT / "include"), "-I", str(CSRC), str(CSRC / "er_draft.cpp"), str(stub), "-o", str(out)], check=True)
     lib = C.CDLL(str(out))
-    for name in ("er_hip_kv8_attention_masked", "er_hip_kv8_accept", "er_hip_choose_logits", "er_hip_choose_logits_workspace"):
+    for name in ("er_hip_kv8_attention_masked", "er_hip_kv8_accept", "er_hip_choose_logits", "er_hip_choose_logits_workspace",
+                 "er_hip_kv8_attention_masked_workspace"):
         f = getattr(lib, name)
         f.restype, f.argtypes = _ffi.SIGNATURES[name]
     lib.stub_create.restype = C.c_void_p
@@ -209,7 +215,7 @@ def ctx(host):
 def launches(host):
     a = (C.c_uint * 4)()
     n = host.stub_launches(a)
-    return [(a[2 * i], a[2 * i + 1]) for i in range(n)]
+    return [(a[2 * i], a[2 * i + 1]) for i in range(min(n, 2))]
 
 
 def test_ordinary_calls_launch(host, ctx):
@@ -226,6 +232,26 @@ def test_ordinary_calls_launch(host, ctx):
         grids.append(launches(host)[0][0])
     assert grids[1] < grids[2] < grids[0]
     assert accept(**on) == 0 and [g for g, _ in launches(host)] == [2 * 2 * 2]
+
+
+def test_workspace_holds_the_parts_of_every_call(host, ctx):
+    """What the query says is enough for each window, sinks and masks of such a batch, and one byte less is refused
+    where the call that needs all of it is made."""
+    n = C.c_uint64()
+    f = host.er_hip_kv8_attention_masked_workspace
+    for heads, most, tokens, P, need in ((4, 4, 512, 16, False), (4, 4, 4000, 16, True), (64, 20, 40000, 64, True), (64, 4, 900, 32, True)):
+        c, b = cache(4000, 2, P), batch(3, 40, most, tokens, P)
+        assert f(ctx, ref(c), ref(b), heads, C.byref(n)) == 0 and (n.value > 0) == need
+        refused = 0
+        for short in (0, 1):
+            for window, sinks, d in ((0, 0, None), (700, 0, None), (700, 100, drafts(40)), (0, 0, drafts(40)), (1 << 31, 1 << 31, None)):
+                ws = buf(n.value - short, 7 << 50) if need else NULL
+                st = attend(c, b, rows(heads, 40, 5 << 50), rows(heads, 40, 6 << 50), window=window, sinks=sinks, d=d, ws=ws,
+                            lib=host, ctx=ctx, n=40)
+                assert st == (ENC if st and short and need else 0), (heads, window, sinks, host.stub_error())
+                refused += st != 0
+        assert (refused > 0) == need
+    launches(host)
 
 
 def test_small_calls_do_nothing(host, ctx):
