@@ -46,7 +46,7 @@ er_status draft_load(DraftKernels &k) {
         find(k.joinRow[d], "er_kv8_masked_join_row_d%d", dims[d]);
         find(k.accept[d], "er_kv8_accept_d%d", dims[d]);
     }
-    find(k.choose, "er_choose_slices");
+    for (int i = 0; i < 2; ++i) find(k.choose[i], "er_choose_s%d", 1 + i);
     find(k.chooseJoin, "er_choose_join");
     if (st != ER_OK) draft_unload(k);
     return st;
@@ -136,19 +136,17 @@ er_status check_no_overlap(const char *op, std::initializer_list<Range> outputs,
     return ER_OK;
 }
 
-// Tokens of a row that one workgroup takes.
+// Tokens of a row that one workgroup takes.  Few of them scan the context more often, many have room in LDS for fewer
+// workgroups at once: by 1024, 2048, 4096, us, one user 7.5, 7.5, 8.7, 64 users with 4096 tokens of context, biases and
+// masks 29.6, 23.9, 32.8, 172 nodes of trees 57, 42, 46.  A vocabulary below a slice takes half.
 struct ChoosePlan {
     uint32_t slices, slice;
 };
-ChoosePlan plan_choose(uint32_t rows, uint32_t vocab, int cu) {
-    ChoosePlan p{};
-    p.slice = 4096;
-    while (p.slice > 1024 && (uint64_t)rows * ((vocab + p.slice - 1) / p.slice) < 2ull * cu) p.slice /= 2;
-    p.slices = (vocab + p.slice - 1) / p.slice;
-    return p;
+ChoosePlan plan_choose(uint32_t vocab) {
+    const uint32_t slice = vocab < ER_CHOOSE_SLICE ? ER_CHOOSE_SLICE / 2 : ER_CHOOSE_SLICE;
+    return ChoosePlan{(vocab + slice - 1) / slice, slice};
 }
-// The smallest slices bound what the workspace holds, whatever the chip.
-uint64_t choose_workspace(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + 1023) / 1024) * 8; }
+uint64_t choose_workspace(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * plan_choose(vocab).slices * 8; }
 
 er_status check_logits(const char *op, uint32_t rows, uint32_t vocab) {
     if (rows > 0x3fffffffu || vocab == 0 || vocab > 0x3fffffffu)
@@ -361,14 +359,15 @@ er_status er_hip_choose_logits(er_hip_ctx *ctx, er_stream stream, er_buffer logi
                               {{logits.data, span, "logits"}});
     if (st == ER_OK) st = make_ready(op, ctx);
     if (st != ER_OK) return st;
-    const ChoosePlan plan = plan_choose(rows, vocab, cu_count_of(ctx));
-    a.slices = plan.slices, a.slice = plan.slice;
+    const ChoosePlan plan = plan_choose(vocab);
+    a.slices = plan.slices;
     a.partV = (float *)workspace.data;
     a.partI = (uint32_t *)workspace.data + (uint64_t)rows * plan.slices;
-    const uint32_t lds = ((a.penalty ? 1u : 0u) + (a.bias ? 1u : 0u)) * plan.slice * 4;
+    // counts, entries and the list
+    const uint32_t lds = a.penalty || a.bias ? plan.slice * (a.bias ? 10 : 6) : 0;
     const uint64_t blocks = (uint64_t)rows * plan.slices, joins = ((uint64_t)rows + 3) / 4;
     st = check_blocks(op, blocks);
-    if (st == ER_OK) st = launch(draft_of(ctx).choose, op, blocks, lds, stream, &a);
+    if (st == ER_OK) st = launch(draft_of(ctx).choose[plan.slice < ER_CHOOSE_SLICE ? 0 : 1], op, blocks, lds, stream, &a);
     if (st != ER_OK || !chosen.data || plan.slices == 1) return st;
     return launch(draft_of(ctx).chooseJoin, op, joins, 0, stream, &a);
 }

@@ -5,6 +5,7 @@
 #include "er_kv8.h"
 
 #define ER_CHOOSE_THREADS 256
+#define ER_CHOOSE_SLICE (8 * ER_CHOOSE_THREADS)  // tokens of a workgroup; half below a vocabulary of as many
 
 struct ErAcceptArgs {
     ErKv8Cache c;
@@ -30,5 +31,5 @@ struct ErChooseArgs {
     const int32_t *token;
     uint32_t rows, maxRows, sequences, vocab, stride;
     uint32_t historyStride, biasStride, allowedStride, words;
-    uint32_t slices, slice;   // workgroups of a row, tokens of each (a multiple of 1024)
+    uint32_t slices;          // workgroups of a row
 };

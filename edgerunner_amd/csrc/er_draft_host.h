@@ -12,7 +12,7 @@ struct DraftKernels {
     hipFunction_t few[2][kKv8Dims][kKv8Pages][2] = {}, wide[kKv8Dims][kKv8Pages][2] = {};
     hipFunction_t joinFew[2][kKv8Dims] = {}, joinColumn[2][kKv8Dims] = {}, join[kKv8Dims] = {}, joinRow[kKv8Dims] = {};
     hipFunction_t accept[kKv8Dims] = {};
-    hipFunction_t choose = nullptr, chooseJoin = nullptr;
+    hipFunction_t choose[2] = {}, chooseJoin = nullptr;  // half slices, slices
 };
 
 // Loads the code object on the current device and resolves its kernels; where
