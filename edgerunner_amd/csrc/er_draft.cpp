@@ -108,9 +108,6 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     p.tiles = (uint32_t)((cols + 16 * p.blocks - 1) / (16 * p.blocks));
     if (full > 512) {
         p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
-        // by 2, 3, 4, 6 steps, us: a user of 8000 tokens 18.3, 17.0, 14.0, 15.7; where 2 leave half the workgroups without
-        // work, one user's tree of 26 drafts 13.7, 13.7, 14.6, 15.0, a window of 1020 tokens 12.4, 12.9, 12.8, 13.5
-        p.least = 4;
         p.parts = 2ull * p.shares * 16 * p.blocks;
     }
     return p;
@@ -202,7 +199,7 @@ er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const e
         a.position = (const int32_t *)drafts->position.data;
     }
     const MaskedPlan p = plan_masked(cache, batch, a.group, a.window, cu_count_of(ctx), a.sinks, drafts != nullptr);
-    a.shares = p.shares, a.least = p.least;
+    a.shares = p.shares;
     a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
     const DraftKernels &kernels = draft_of(ctx);
     const int di = dim_index(d), nb = (int)p.blocks - 1;

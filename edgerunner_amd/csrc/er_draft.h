@@ -4,6 +4,7 @@
 
 #include "er_kv8.h"
 
+#define ER_FEW_LEAST 4u  // 64-token steps that a share of an attention call has at least; half where they fit half the workgroups
 #define ER_CHOOSE_THREADS 256
 #define ER_CHOOSE_SLICE (8 * ER_CHOOSE_THREADS)  // tokens of a workgroup; half below a vocabulary of as many
 

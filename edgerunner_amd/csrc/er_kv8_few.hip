@@ -16,31 +16,36 @@ ER_DEV uint32_t few_blocks(const ErAttendArgs &p, const Sequence &q) {
 ER_DEV uint32_t few_length(uint32_t steps, bool aligned, uint32_t quota) {
     return aligned ? (steps + quota - 1) / quota * quota : steps;
 }
-// Shares of p.least steps (half of it where half the workgroups do) and, as long
+// Shares of ER_FEW_LEAST steps (half of it where half the workgroups do) and, as long
 // as the units do not fit the workgroups so, half as many again: a workgroup that
-// takes two units starts and ends twice.  Past four times p.least that counts less
-// than an even share.  16 draft checks at head width 256, 64 units of up to 47
-// steps: 25 us by 6 steps, 31 by 4 across units.
+// takes two units starts and ends twice.  Past four times that it counts less than an
+// even share.  16 draft checks at head width 256, 64 units of up to 47 steps: 25 us by
+// 6 steps, 31 by 4 across units.  By 2, 3, 4, 6 steps, us: a user of 8000 tokens 18.3,
+// 17.0, 14.0, 15.7; where 2 leave half the workgroups without work, one user's tree of
+// 26 drafts 13.7, 13.7, 14.6, 15.0, a window of 1020 tokens 12.4, 12.9, 12.8, 13.5.
+constexpr uint32_t few_next(uint32_t quota) { return quota < ER_FEW_LEAST ? ER_FEW_LEAST : quota + quota / 2; }
+template <int NB, uint32_t QUOTA, class A>
+ER_DEV Shares few_shares_by(const A &p, const LaneSequence &first, uint32_t lane) {
+    Shares s;
+    s.aligned = QUOTA <= 4 * ER_FEW_LEAST;
+    s.quota = s.aligned ? QUOTA : 1;
+    uint32_t sum = 0;
+    for (uint32_t at = 0; at < p.b.sequences; at += 64) {
+        const LaneSequence l = at ? lane_sequence(p, at + lane) : first;
+        sum += few_length(l.steps, s.aligned, s.quota) * few_blocks<NB>(p, l.q);
+    }
+    s.total = wave_sum(sum) * p.c.heads;
+    if constexpr (QUOTA > 4 * ER_FEW_LEAST) {
+        s.quota = max(ER_FEW_LEAST, (s.total + p.shares - 1) / p.shares);
+        return s;
+    } else {
+        if (s.total <= p.shares * (QUOTA < ER_FEW_LEAST ? QUOTA / 2 : QUOTA)) return s;
+        return few_shares_by<NB, few_next(QUOTA)>(p, first, lane);
+    }
+}
 template <int NB, class A>
 ER_DEV Shares few_shares(const A &p, const LaneSequence &first, uint32_t lane) {
-    Shares s;
-    s.aligned = true;
-    for (s.quota = p.least / 2;; s.quota = s.quota < p.least ? p.least : s.quota + s.quota / 2) {
-        if (s.quota > 4 * p.least) {
-            s.aligned = false;
-            s.quota = 1;  // lengths as they are
-        }
-        uint32_t sum = 0;
-        for (uint32_t at = 0; at < p.b.sequences; at += 64) {
-            const LaneSequence l = at ? lane_sequence(p, at + lane) : first;
-            sum += few_length(l.steps, true, s.quota) * few_blocks<NB>(p, l.q);
-        }
-        s.total = wave_sum(sum) * p.c.heads;
-        if (!s.aligned) break;
-        if (s.total <= p.shares * (s.quota < p.least ? s.quota / 2 : s.quota)) return s;
-    }
-    s.quota = max(p.least, (s.total + p.shares - 1) / p.shares);
-    return s;
+    return few_shares_by<NB, ER_FEW_LEAST / 2>(p, first, lane);
 }
 // The sequence that place `at` of the line belongs to, and where it begins.
 template <int NB, class A>
@@ -529,8 +534,15 @@ struct FewParts {
 template <int NB, class A>
 ER_DEV bool few_line(const A &p, uint32_t row, uint32_t lane, LaneSequence &l, Shares &sh, uint32_t &before) {
     const LaneSequence first = lane_sequence(p, lane);
-    const uint32_t s = uniform(sequence_of_row(p.b, row, lane));
-    if (s >= p.b.sequences) return false;
+    uint32_t s;
+    if (p.b.sequences <= 64) {  // no second read of their starts
+        const uint64_t has = __ballot((int)row >= first.q.row0 && (int)row < first.q.row0 + first.q.n);
+        if (!has) return false;
+        s = (uint32_t)__ffsll((unsigned long long)has) - 1u;
+    } else {
+        s = uniform(sequence_of_row(p.b, row, lane));
+        if (s >= p.b.sequences) return false;
+    }
     l = lane_sequence_at(p, first, s);
     if ((int)row < l.q.row0 || (int)row >= l.q.row0 + l.q.n) return false;
     sh = few_shares<NB>(p, first, lane);
@@ -558,16 +570,56 @@ ER_DEV FewParts few_parts(const A &p, const LaneSequence &l, const Shares &sh, u
 }
 
 // One column (a row of a query head) a workgroup: many parts of few columns, one
-// user far into a document.
+// user far into a document.  Up to 64 parts, a lane's references and sums and the first
+// outputs are asked for at once.
 template <int D, int NB, class A>
 ER_DEV void few_join_column(const A &p, float *lds) {
+    constexpr uint32_t LANES = D / 4, AT_ONCE = ER_KV8_THREADS / LANES, EARLY = 64 / AT_ONCE < 4 ? 64 / AT_ONCE : 4;
     const uint32_t heads = p.group * p.c.heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
     LaneSequence l;
     Shares sh;
     uint32_t before;
-    if (!few_line<NB>(p, row, threadIdx.x & 63u, l, sh, before)) return;
+    if (!few_line<NB>(p, row, lane, l, sh, before)) return;
     const FewParts f = few_parts<NB>(p, l, sh, before, row, head);
-    if (f.parts) join_parts<D>(p, f.parts, (int)row, head, lds, [&](uint32_t i) { return f.index(i); });
+    if (f.parts == 0) return;
+    if (f.parts > 64) {
+        join_parts<D>(p, f.parts, (int)row, head, lds, [&](uint32_t i) { return f.index(i); });
+        return;
+    }
+    const uint32_t mine = tid / LANES, d = (tid % LANES) * 4;
+    const f32x2 ml = *(const f32x2 *)(p.partML + 2 * f.index(min(lane, f.parts - 1)));
+    f32x4 early[EARLY];
+#pragma unroll
+    for (uint32_t k = 0; k < EARLY; ++k)
+        early[k] = *(const f32x4 *)(p.partO + f.index(min(mine + k * AT_ONCE, f.parts - 1)) * D + d);
+    const bool some = lane < f.parts && !(ml.y < 0.0f);
+    const float top = wave_top(ml.x);
+    float weight = some ? ml.y * __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;
+    // every wave has the sum, of the same terms in the same order
+    const float total = group_sum<64>(weight);
+    const bool seen = __any(some);
+    weight = some ? share_of(weight, total) : -1.0f;
+    f32x4 o = {};
+#pragma unroll
+    for (uint32_t k = 0; k < EARLY; ++k) {
+        const uint32_t i = mine + k * AT_ONCE;
+        const float w = __shfl(weight, (int)(i & 63u));
+        if (i < f.parts && (w >= 0.0f || w != w)) o += early[k] * w;
+    }
+    for (uint32_t i0 = EARLY * AT_ONCE; i0 < f.parts; i0 += AT_ONCE) {
+        const uint32_t i = i0 + mine;
+        const float w = __shfl(weight, (int)(i & 63u));
+        if (i < f.parts && (w >= 0.0f || w != w)) o += *(const f32x4 *)(p.partO + f.index(i) * D + d) * w;
+    }
+    *(f32x4 *)(lds + 4 * tid) = o;
+    __syncthreads();
+    if (tid < LANES) {
+        f32x4 v = {};
+#pragma unroll
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v += *(const f32x4 *)(lds + 4 * (k * LANES + tid));
+        store4(p, (int)row, head, 4 * tid, D, joined(v, seen, total));
+    }
 }
 
 // D / 4 threads a column, whose parts, most often two or three, follow each
@@ -586,13 +638,37 @@ ER_DEV void few_join(const A &p) {
     if (f.parts == 0) return;
     float top = ER_NO_MAX, total = 0.0f;
     bool seen = false;
+    f32x4 o = {};
+    if (f.parts <= 4) {  // all that is read is asked for at once
+        f32x2 ml[4];
+        f32x4 part[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const size_t at = f.index(min(i, f.parts - 1));
+            ml[i] = *(const f32x2 *)(p.partML + 2 * at);
+            part[i] = *(const f32x4 *)(p.partO + at * D + d);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const bool some = i < f.parts && !(ml[i].y < 0.0f);
+            ml[i].x = some ? ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - top) : 0.0f;
+            seen |= some;
+            total += ml[i].x;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (i < f.parts && !(ml[i].y < 0.0f)) o += part[i] * share_of(ml[i].x, total);
+        store4(p, (int)row, head, d, D, joined(o, seen, total));
+        return;
+    }
     for (uint32_t i = 0; i < f.parts; ++i) top = fmaxf(top, p.partML[2 * f.index(i)]);
     for (uint32_t i = 0; i < f.parts; ++i) {
         const f32x2 ml = *(const f32x2 *)(p.partML + 2 * f.index(i));
         seen |= !(ml.y < 0.0f);
         total += ml.y < 0.0f ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
     }
-    f32x4 o = {};
     for (uint32_t i = 0; i < f.parts; ++i) {
         const size_t at = f.index(i);
         const f32x2 ml = *(const f32x2 *)(p.partML + 2 * at);
