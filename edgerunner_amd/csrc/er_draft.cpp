@@ -83,6 +83,8 @@ er_status check_drafts(const char *op, const er_drafts *d, uint32_t rows, uint32
 
 // How an attention call under masks is cut up: in shares as the narrow kernel's,
 // with 16 or 32 columns a wave, or as the wide kernel's.
+constexpr uint32_t kUnshared = 512;  // tokens of a sequence up to which a unit is not shared
+uint32_t few_columns(const er_kv8_cache *c) { return c->head_dim == 256 ? 256 : 128; }
 struct MaskedPlan : AttendPlan {
     uint32_t blocks;  // of 16 columns that a wave has; 0: the wide kernel
 };
@@ -93,7 +95,7 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     // Shares against the wide kernel, us: trees of 128 columns of 32 sequences of up to 6000 tokens 149 / 196, of 192
     // of 8 of 4000 58 / 60, of 256 (bf16) 62 / 58, of 512 of 2 of 20000 122 / 107; of 256 of width 256 of 16 of 4000
     // 117 / 176.
-    if (cols > (c->head_dim == 256 ? 256 : 128)) {
+    if (cols > few_columns(c)) {
         (AttendPlan &)p = plan_attend(c, b, group, window, cu, sinks, drafts);
         return p;
     }
@@ -106,11 +108,19 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     const uint64_t steps = (uint64_t)b->sequences * c->kv_heads * ((cols + 15) / 16) * ((full + 63) / 64);
     p.blocks = c->head_dim < 256 && cols > 16 && steps >= 64ull * 2 * (uint64_t)cu ? 2 : 1;
     p.tiles = (uint32_t)((cols + 16 * p.blocks - 1) / (16 * p.blocks));
-    if (full > 512) {
+    if (full > kUnshared) {
         p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
         p.parts = 2ull * p.shares * 16 * p.blocks;
     }
     return p;
+}
+
+// The line that shares are cut from, with what rounds a unit's length up (fewer than 16 steps), is counted in 32 bits.
+er_status check_line(const char *op, const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group) {
+    const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b), steps = (full + 63) / 64 + 16;
+    if (cols > few_columns(c) || full <= kUnshared || b->sequences * steps * c->kv_heads <= 0xffffffffull / ((cols + 15) / 16)) return ER_OK;
+    return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: %u sequences of up to %u tokens and %u rows: too many to count in 32 bits", op,
+                b->sequences, most_tokens(c, b), b->max_rows);
 }
 
 struct Range {
@@ -179,6 +189,7 @@ er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const e
     if (st != ER_OK) return st;
     if (q->heads != out->heads) return fail(ER_ERR_INVALID_VECTOR_SHAPE, "%s: q and out differ in heads", op);
     st = check_group(op, cache, batch, q->heads);
+    if (st == ER_OK) st = check_line(op, cache, batch, q->heads / cache->kv_heads);
     if (st == ER_OK) st = check_apart(op, "q and out", q, out, batch->rows, d, 4, outBytes, false);
     if (st == ER_OK && drafts) st = check_drafts(op, drafts, batch->rows, batch->max_rows, true);
     if (st == ER_OK && drafts && window) st = check_buffer(op, "position", drafts->position, (uint64_t)batch->rows * 4, 4);
@@ -223,6 +234,7 @@ er_status er_hip_kv8_attention_masked_workspace(er_hip_ctx *ctx, const er_kv8_ca
     er_status st = check_cache(op, cache);
     if (st == ER_OK) st = check_batch(op, batch);
     if (st == ER_OK) st = check_group(op, cache, batch, q_heads);
+    if (st == ER_OK) st = check_line(op, cache, batch, q_heads / cache->kv_heads);
     if (st == ER_OK) st = check_ctx(ctx);
     if (st != ER_OK) return st;
     if (batch->rows == 0 || batch->sequences == 0) return ER_OK;

@@ -137,6 +137,19 @@ def test_attention_refusals():
     assert reaches_the_context(attend(d=drafts(position=NULL)))
 
 
+def test_lines_of_steps_that_32_bits_do_not_count():
+    """Sequences of 513 tokens: 9 steps and 16 that rounding may add, of two heads, in 16 blocks of columns."""
+    fit, d, ws = ((1 << 32) - 1) // (25 * 2 * 16), 256, C.c_uint64()
+    f = _ffi.load().er_hip_kv8_attention_masked_workspace
+    # 257 columns are the wide kernel's, which does not count them, and 512 tokens no shares
+    for n, tokens, group, status in ((fit, 513, 256, NO_CTX), (fit + 1, 513, 256, VEC), (fit + 1, 513, 240, NO_CTX),
+                                     (fit + 1, 513, 257, NO_CTX), (fit + 1, 512, 256, NO_CTX)):
+        c, b = cache(100, 2, 64, d), batch(n, n, 1, tokens, 64)
+        q, o = (_ffi.er_head_rows(buf(n * 2 * group * d * 4, x << 50), 2 * group, 2 * group * d) for x in (5, 6))
+        assert attend(c, b, q, o, n=n) == status, (n, tokens, group)
+        assert f(None, ref(c), ref(b), 2 * group, C.byref(ws)) == status, (n, tokens, group)
+
+
 def test_accept_refusals():
     assert accept(d=None) == ARG and "null drafts" in last()
     assert accept(b=batch(n=1025, most=1025), d=drafts(1025), n=1025) == VEC and "1024" in last()
