@@ -215,6 +215,33 @@ def test_list_lengths_are_bounded(ctx):
     c.check()
 
 
+@pytest.mark.parametrize("vocab", [1, 2, 3, 4, 5, 2046, 2047, 2048, 2049, 2050, 2051, 2052, 4095])
+@pytest.mark.parametrize("past,bias", [(9001, 700), (4097, 300), (5, 3)])
+def test_lengths_of_lists(ctx, vocab, past, bias):
+    """Lists that end anywhere in a group of four, have more entries than a slice has threads, or fewer than four."""
+    c = Case(ctx, vocab + past, vocab, [1] * 12, past=past, bias=bias, allowed=vocab > 2047)
+    ends = [past - i for i in range(4)] + [0, 1, 2, 3, 4, 5, min(1024, past), min(4096, past)]
+    c.past_len[:] = [max(n, 0) for n in ends]
+    c.bias_len[:] = [bias - i % 3 for i in range(6)] + [0, 1, 2, 3, min(256, bias), min(257, bias)]
+    c.run()
+
+
+def test_logits_beyond_32_bits(ctx):
+    """Rows whose offsets pass 2^32 bytes, in place."""
+    vocab, stride, n = 5003, 1 << 26, 18
+    c = Case(ctx, 12, vocab, [1] * n, past=40, bias=9, allowed=True)
+    c.upload()
+    far = ctx.alloc(4 * ((n - 1) * stride + vocab))
+    for r in range(n):
+        far.upload(c.x[r], 4 * r * stride)
+    c.kern.encode(None, far, n, vocab, c.rules, out=far, chosen=c.cb, workspace=c.ws, rowStride=stride)
+    ctx.synchronize()
+    for r in range(n):
+        c.ob.upload(far.download(np.float32, vocab, 4 * r * stride), 4 * r * vocab)
+    c.check()
+    far.free()
+
+
 @pytest.mark.parametrize("tree", [False, True])
 def test_replayed_graph(ctx, tree):
     """A recorded call follows later histories, masks and logits, beside eager calls with a workspace of their own."""
