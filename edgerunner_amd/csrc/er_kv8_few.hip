@@ -5,6 +5,12 @@
 // tile's codes are converted once for all of them.  Like the narrow kernel's,
 // units (sequence, head, 16 NB columns) lie on one line that the resident
 // workgroups share evenly; a workgroup's four waves take its tiles in turn.
+//
+// Decode is bound by memory: 48 users of 32 over 8 heads of 128 read 777 MB in 140
+// us, 5.5 TB/s.  Trees are bound by issue: those of 32 users (639 rows of 32 heads over
+// 8 of 128, fp32) take 143 us with the join, of which vector instructions
+// are 59% of the SIMDs' cycles and products 32%; a tile costs a SIMD some 1325 cycles
+// with one block of columns.  One user's call is a chain of loads, 8 to 10 us.
 
 #define ER_DEV_MEMBER __device__ __forceinline__
 
