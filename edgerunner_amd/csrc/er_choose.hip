@@ -27,25 +27,47 @@ ER_DEV Candidate wave_best(Candidate a) {
     return dpp_better<ER_DPP_ROW_BCAST31, 0xc>(a);
 }
 
-// The sequence of a row, and the row's place in it; false: it belongs to none.
+// What the rules know of a row's sequence, and the row's place in it.
 struct LogitRow {
     uint32_t s;
     int row0, n;
+    float repetition, presence, frequency;
+    uint32_t known, entries;  // of the history and the biases
 };
+// Of sequence s, which may differ between lanes.  Nothing waits for anything else.
+ER_DEV LogitRow logit_sequence(const ErChooseArgs &p, uint32_t s) {
+    LogitRow r = {s, (int)s, 1, 1.0f, 0.0f, 0.0f, 0, 0};
+    if (p.start) {
+        const int rows = (int)p.rows;
+        r.row0 = min(max(p.start[s], 0), rows);
+        r.n = min(max(min(p.start[s + 1], rows) - r.row0, 0), (int)p.maxRows);
+    }
+    if (p.penalty) {
+        const float *w = p.penalty + 3 * (size_t)s;
+        r.repetition = w[0], r.presence = w[1], r.frequency = w[2];
+        if (p.history) r.known = min((uint32_t)max(p.historyLen[s], 0), p.historyStride);
+    }
+    if (p.bias) r.entries = min((uint32_t)max(p.biasLen[s], 0), p.biasStride);
+    return r;
+}
+// Lanes look at a sequence each; false: the row belongs to none.
 ER_DEV bool logit_row(const ErChooseArgs &p, uint32_t row, uint32_t lane, LogitRow &r) {
     if (!p.start) {
-        r = LogitRow{row, (int)row, 1};
-        return row < p.sequences;
+        if (row >= p.sequences) return false;
+        r = logit_sequence(p, row);
+        return true;
     }
-    ErKv8Batch b = {};
-    b.start = p.start;
-    b.sequences = p.sequences;
-    r.s = uniform(sequence_of_row(b, row, lane));
-    if (r.s >= p.sequences) return false;
-    const int rows = (int)p.rows;
-    r.row0 = min(max(load_shared(p.start + r.s), 0), rows);
-    r.n = min(max(min(load_shared(p.start + r.s + 1), rows) - r.row0, 0), (int)p.maxRows);
-    return (int)row >= r.row0 && (int)row < r.row0 + r.n;
+    for (uint32_t at = 0; at < p.sequences; at += 64) {
+        const LogitRow l = logit_sequence(p, min(at + lane, p.sequences - 1));
+        const uint64_t has = __ballot((int)row >= l.row0 && (int)row < l.row0 + l.n);
+        if (!has) continue;
+        const uint32_t i = (uint32_t)__ffsll((unsigned long long)has) - 1u;
+        r = LogitRow{lane_of(l.s, i), (int)lane_of((uint32_t)l.row0, i), (int)lane_of((uint32_t)l.n, i),
+                     scalar_of(l.repetition, i), scalar_of(l.presence, i), scalar_of(l.frequency, i),
+                     lane_of(l.known, i), lane_of(l.entries, i)};
+        return true;
+    }
+    return false;
 }
 
 // The largest of the wave's, none of which is NaN, in lane 63.
@@ -96,7 +118,7 @@ ER_DEV u32x4 four_of(u32x4 r, uint32_t i, uint32_t n) {
 //
 // Reads and writes the logits once, which bounds it: 172 nodes of 128256 logits, 4/32
 // bytes of masks each, 41.7 us with the join, 4.2 TB/s.  64 rows with 4096 tokens of
-// context and biases take 23.3 us, 2.9 TB/s, without them 14.9: the more of a workgroup's
+// context and biases take 22.7 us, 2.9 TB/s, without them 14.9: the more of a workgroup's
 // time passes between its reads and its writes, the fewer bytes are under way.  Counts
 // that answer (to list a token when it is first met) took 25.1, with a lane's dummy for
 // tokens of other slices, so that no branch lies between them, 26.5.  The rules in 64 bits
@@ -111,18 +133,9 @@ ER_DEV void choose_slice(const ErChooseArgs &p, uint32_t *lds) {
         if (p.chosen && p.slices > 1 && tid == 0) p.partI[blockIdx.x] = ER_NO_ROW;
         return;
     }
-    double repetition = 1.0, presence = 0.0, frequency = 0.0;
-    uint32_t known = 0, drafts = 0, entries = 0;
-    if (p.penalty) {
-        const float *w = p.penalty + 3 * (size_t)r.s;
-        const float a = load_shared(w), b = load_shared(w + 1), c = load_shared(w + 2);
-        repetition = a, presence = b, frequency = c;
-        if (!(a == 1.0f && b == 0.0f && c == 0.0f)) {
-            if (p.history) known = min((uint32_t)max(load_shared(p.historyLen + r.s), 0), p.historyStride);
-            if (p.seen) drafts = (uint32_t)r.n;
-        }
-    }
-    if (p.bias) entries = min((uint32_t)max(load_shared(p.biasLen + r.s), 0), p.biasStride);
+    const bool counts = !(r.repetition == 1.0f && r.presence == 0.0f && r.frequency == 0.0f);
+    const double repetition = r.repetition, presence = r.presence, frequency = r.frequency;
+    const uint32_t known = counts ? r.known : 0, drafts = counts && p.seen ? (uint32_t)r.n : 0, entries = r.entries;
     const int32_t *history = p.history + (size_t)r.s * p.historyStride;
     // Loads return in order: those that LDS waits for come first.
     uint32_t words[S];
