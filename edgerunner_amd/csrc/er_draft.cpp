@@ -83,7 +83,7 @@ er_status check_drafts(const char *op, const er_drafts *d, uint32_t rows, uint32
 
 // How an attention call under masks is cut up: in shares as the narrow kernel's,
 // with 16 or 32 columns a wave, or as the wide kernel's.
-constexpr uint32_t kUnshared = 512;  // tokens of a sequence up to which a unit is not shared
+constexpr uint32_t kUnshared = 512;  // tokens of a sequence up to which a unit is never shared
 uint32_t few_columns(const er_kv8_cache *c) { return c->head_dim == 256 ? 256 : 128; }
 struct MaskedPlan : AttendPlan {
     uint32_t blocks;  // of 16 columns that a wave has; 0: the wide kernel
@@ -108,7 +108,18 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     const uint64_t steps = (uint64_t)b->sequences * c->kv_heads * ((cols + 15) / 16) * ((full + 63) / 64);
     p.blocks = c->head_dim < 256 && cols > 16 && steps >= 64ull * 2 * (uint64_t)cu ? 2 : 1;
     p.tiles = (uint32_t)((cols + 16 * p.blocks - 1) / (16 * p.blocks));
-    if (full > kUnshared) {
+    // Where units are many and short, a workgroup has a unit each: shares cut some of them in two, whose sums a join then
+    // reads, and a workgroup that goes from unit to unit waits for each one's lengths.  Shared / not, us, of sequences of
+    // up to 1000 tokens (16 steps): 64 units 12.8 / 12.3, 96 15.2 / 12.5, 256 20.3 / 13.6 and 18.4 / 14.8, 512 34.2 / 20.0,
+    // 1600 98 / 59; of 2000: 64 15.4 / 17.9, 128 17.6 / 18.0 and 20.5 / 19.2, 256 28.2 / 20.3, 512 51.9 / 38.9 and 32.9 /
+    // 32.7; under a window of 2048: 512 64.2 / 54.1 and 46.0 / 36.1, 384 32.4 / 35.0; of 4000: 128 24.8 / 28.4, 256 44.9 /
+    // 38.8, but 512 44.5 / 56.2, as the longest unit then decides.  At width 256 64 of 1000 17.6 / 24.5, 512 44.1 / 46.6.
+    uint64_t span = full;
+    if (window)
+        span = std::min<uint64_t>(span, (uint64_t)window + b->max_rows + 127 + (((uint64_t)sinks + 63) & ~63ull));
+    const uint64_t most = (span + 63) / 64, units = (uint64_t)b->sequences * c->kv_heads * p.tiles;
+    const bool whole = c->head_dim < 256 && most <= 40 && units * 64 >= most * (uint64_t)cu;
+    if (span > kUnshared && !whole) {
         p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
         p.parts = 2ull * p.shares * 16 * p.blocks;
     }

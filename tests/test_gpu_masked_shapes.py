@@ -1,5 +1,7 @@
 """Attention under masks where the work is cut up otherwise (two blocks of columns a wave, shares across units), where values'
 scales lie far apart, and in a pool of more than 2^32 code bytes."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -34,6 +36,21 @@ def test_two_blocks_a_wave(ctx, d, P, hq, hkv, long, few, masks, window, sinks, 
 def test_shared_across_units(ctx, d, P, hq, hkv, lens, rows, masks):
     c = Case(ctx, d + P, lens, rows, P, d, hq, hkv, masks)
     c.check(c.run())
+
+
+@pytest.mark.parametrize("d,P,hq,hkv,most,masks,window,sinks", [
+    (64, 16, 8, 4, 1900, "tree", 0, 0), (128, 32, 8, 8, 1500, None, 700, 70), (64, 64, 16, 8, 2048, "any", 0, 0),
+    (128, 16, 8, 4, 1100, "tree", 200, 1), (128, 64, 4, 4, 5000, None, 900, 4), (64, 32, 24, 4, 2500, "tree", 0, 0)])
+def test_a_workgroup_a_unit(ctx, d, P, hq, hkv, most, masks, window, sinks):
+    """Many units of middling length, or of long caches under a window, each one workgroup's: no workspace where none is long."""
+    rng = np.random.default_rng(most)
+    lens = [most, 0, 1] + [int(x) for x in rng.integers(1, min(most, 1200), 37)]
+    rows = [min(m, int(x)) for m, x in zip(lens, rng.integers(0, 7, 40))]
+    c = Case(ctx, d + P, lens, rows, P, d, hq, hkv, masks)
+    c.check(c.run(window=window, sinks=sinks), window=window, sinks=sinks)
+    if most <= 2500:
+        assert c.kern.lib.er_hip_kv8_attention_masked_workspace(ctx.handle, c.cache.ref, c.b.upload(ctx).ref, hq,
+                                                                C.byref(n := C.c_uint64(1))) == 0 and n.value == 0
 
 
 @pytest.mark.parametrize("half", [False, True])
