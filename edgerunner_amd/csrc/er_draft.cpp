@@ -118,7 +118,7 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     if (window)
         span = std::min<uint64_t>(span, (uint64_t)window + b->max_rows + 127 + (((uint64_t)sinks + 63) & ~63ull));
     const uint64_t most = (span + 63) / 64, units = (uint64_t)b->sequences * c->kv_heads * p.tiles;
-    const bool whole = c->head_dim < 256 && most <= 40 && units * 64 >= most * (uint64_t)cu;
+    const bool whole = c->head_dim < 256 && most <= 40 && units * 64 >= most * (uint64_t)cu && units <= kMostBlocks;
     if (span > kUnshared && !whole) {
         p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
         p.parts = 2ull * p.shares * 16 * p.blocks;

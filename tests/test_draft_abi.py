@@ -247,6 +247,16 @@ def test_ordinary_calls_launch(host, ctx):
     assert accept(**on) == 0 and [g for g, _ in launches(host)] == [2 * 2 * 2]
 
 
+def test_more_units_than_workgroups_are_shared(host, ctx):
+    """Units of middling length are a workgroup's each as long as a launch counts them."""
+    on = {"lib": host, "ctx": ctx, "n": 600000}
+    for n, grid in ((500000, 500000 * 8 * 4), (600000, 512)):
+        c, b = cache(100, 8), batch(n, 600000, 16, 1000)
+        q, o = rows(64, 600000, 5 << 50), rows(64, 600000, 6 << 50)
+        assert attend(c, b, q, o, ws=buf(1 << 40, 7 << 50), **on) == 0, host.stub_error()
+        assert launches(host)[0][0] == grid
+
+
 def test_workspace_holds_the_parts_of_every_call(host, ctx):
     """What the query says is enough for each window, sinks and masks of such a batch, and one byte less is refused
     where the call that needs all of it is made."""
