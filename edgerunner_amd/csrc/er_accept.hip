@@ -59,10 +59,12 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
     float *scales = values ? p.c.vs : p.c.ks;
     const int lane = (int)(tid % LANES), at = (int)(tid / LANES);
     uint32_t turn = 0;
-    for (int begin = first & ~(P - 1); begin < last; begin += P, turn ^= 1u) {
+    for (int begin = first & ~(P - 1); begin < last; begin += P) {
         const int t0 = max(first, begin), t1 = min(last, begin + P);
         const int page = uniform(page_of(p.b, p.c, s, begin));
         if (page < 0) continue;
+        // Only a page that goes on to the barrier takes the other copy of the peaks: so one lies between two uses of a copy.
+        turn ^= 1u;
         uint32_t c[PASSES];
         float f[PASSES];  // -1: nothing to write
         float peak = 0.0f;
