@@ -39,6 +39,16 @@ ER_DEV Walk walk(const ErAcceptArgs &p, const Sequence &q, const int *parent, co
     }
 }
 
+// The scale that codes of magnitude m (finite, in codes' own units) under the scale f ask for by the append's rule.
+// The value m * f is not formed: 256 under 2^120, which an append leaves for values next to fp32's largest, is past
+// them.  A value that is not finite asks for the least.
+ER_DEV float scale_for(float m, float f) {
+    const uint32_t u = __float_as_uint(f);
+    if (m == 0.0f || finite_magnitude(f) == 0.0f) return exp2i(-100);
+    const int j = block_exponent(m * __uint_as_float((u & 0x7fffffu) | 0x3f800000u)) + (int)(u >> 23) - 127;
+    return exp2i(min(max(j, -100), 127));
+}
+
 // One workgroup takes the keys or values of one sequence and head; each walks
 // for itself, the first of a sequence also writes the path.  Kept tokens that
 // change their place are appended anew, page by page in ascending order, as
@@ -49,7 +59,7 @@ ER_DEV Walk walk(const ErAcceptArgs &p, const Sequence &q, const int *parent, co
 // most.
 template <int D, int P>
 ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, uint32_t head, bool values, const Walk &w,
-                         const int *path, float (*peaks)[4]) {
+                         const int *path, float (*needs)[4]) {
     constexpr int LANES = D / 4;                                                     // lanes a token
     constexpr int TOKENS = ER_KV8_THREADS / LANES < P ? ER_KV8_THREADS / LANES : P;  // tokens a pass
     constexpr int PASSES = P / TOKENS;
@@ -63,11 +73,11 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
         const int t0 = max(first, begin), t1 = min(last, begin + P);
         const int page = uniform(page_of(p.b, p.c, s, begin));
         if (page < 0) continue;
-        // Only a page that goes on to the barrier takes the other copy of the peaks: so one lies between two uses of a copy.
+        // Only a page that goes on to the barrier takes the other copy of the needs: so one lies between two uses of a copy.
         turn ^= 1u;
         uint32_t c[PASSES];
         float f[PASSES];  // -1: nothing to write
-        float peak = 0.0f;
+        float need = 0.0f;  // the largest scale that a token asks for; 0: none has come
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int t = begin + i * TOKENS + at;
@@ -88,17 +98,17 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
             const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
             const float m = fmaxf(fmaxf(finite_magnitude(lo.x), finite_magnitude(lo.y)),
                                   fmaxf(finite_magnitude(hi.x), finite_magnitude(hi.y)));
-            peak = fmaxf(peak, fmaxf(finite_magnitude(m * f[i]), 1.2e-38f));  // above 0 where a token comes
+            need = fmaxf(need, scale_for(m, f[i]));
         }
-        peak = wave_max(peak);
-        if ((tid & 63u) == 0) peaks[turn][tid >> 6] = peak;
+        need = wave_max(need);
+        if ((tid & 63u) == 0) needs[turn][tid >> 6] = need;
         const size_t block = (size_t)page * H + head;
         uint8_t *to = codes + block * (size_t)(P * D);
         const float old = t0 > begin ? scales[block] : 0.0f;
         __syncthreads();
-        peak = fmaxf(fmaxf(peaks[turn][0], peaks[turn][1]), fmaxf(peaks[turn][2], peaks[turn][3]));
-        if (peak == 0.0f) continue;  // none of the page's tokens has a page of its own
-        const float now = fmaxf(old, exp2i(block_exponent(peak)));
+        need = fmaxf(fmaxf(needs[turn][0], needs[turn][1]), fmaxf(needs[turn][2], needs[turn][3]));
+        if (need == 0.0f) continue;  // none of the page's tokens has a page of its own
+        const float now = fmaxf(old, need);
         if (now > old && t0 > begin) {
             const float g = old / now;
             for (uint32_t i = tid; i < (uint32_t)(t0 - begin) * (D / 4); i += ER_KV8_THREADS) {
@@ -106,13 +116,12 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
                 *x = recode4(*x, g);
             }
         }
-        const float over = 1.0f / now;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             if (f[i] < 0.0f) continue;
             const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
-            *((uint32_t *)(to + (i * TOKENS + at) * D) + lane) =
-                codes4(lo.x * f[i] * over, lo.y * f[i] * over, hi.x * f[i] * over, hi.y * f[i] * over);
+            const float g = f[i] / now;  // scales are powers of two
+            *((uint32_t *)(to + (i * TOKENS + at) * D) + lane) = codes4(lo.x * g, lo.y * g, hi.x * g, hi.y * g);
         }
         if (tid == 0) scales[block] = now;
     }
@@ -121,7 +130,7 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
 template <int D>
 ER_DEV void kv8_accept(const ErAcceptArgs &p) {
     __shared__ int parent[ER_MOST_DRAFTS], token[ER_MOST_DRAFTS], chosen[ER_MOST_DRAFTS], path[ER_MOST_DRAFTS];
-    __shared__ float peaks[2][4];
+    __shared__ float needs[2][4];
     __shared__ Walk walked;
     const uint32_t H = p.c.heads, tid = threadIdx.x;
     const uint32_t part = blockIdx.x % (2 * H), s = blockIdx.x / (2 * H), head = part >> 1;
@@ -157,11 +166,11 @@ ER_DEV void kv8_accept(const ErAcceptArgs &p) {
     }
     if (w.first == w.count) return;
     if (p.c.shift == 4)
-        accept_moves<D, 16>(p, q, s, head, values, w, path, peaks);
+        accept_moves<D, 16>(p, q, s, head, values, w, path, needs);
     else if (p.c.shift == 5)
-        accept_moves<D, 32>(p, q, s, head, values, w, path, peaks);
+        accept_moves<D, 32>(p, q, s, head, values, w, path, needs);
     else
-        accept_moves<D, 64>(p, q, s, head, values, w, path, peaks);
+        accept_moves<D, 64>(p, q, s, head, values, w, path, needs);
 }
 
 #define ER_KV8_ACCEPT(D)                                                                                           \

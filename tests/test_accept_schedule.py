@@ -60,3 +60,30 @@ def test_orders_over_missing_pages(lib, gaps):
         assert exp[1][1][0] == 109
         for order in ORDERS:
             c.check(accept(lib, c, order), exp)
+
+
+def near_the_largest(seed, P, d, scales, whole=False):
+    """Kept drafts whose codes, 208 to 448, stand for values past fp32's largest under some of the pages' scales."""
+    c = Case(None, seed, [3 * P + 5], [2 * P + 9], P, d, 1, 1.0)
+    n = c.b.rows[0]
+    for i in (0, 2):
+        big = c.rng.integers(0x75, 0x7f, c.before[i].shape).astype(np.uint8) | (c.rng.integers(0, 2, c.before[i].shape) << 7).astype(np.uint8)
+        c.before[i] = big if whole else np.where(c.rng.random(big.shape) < 0.1, big, c.before[i])
+        c.before[i + 1][:] = np.float32(2.0) ** c.rng.choice(scales, c.before[i + 1].shape).astype(np.float32)
+    c.parent[2:n] = np.arange(1, n - 1)
+    c.parent[1:3] = 0
+    c.chosen[:n - 1], c.token[1] = c.token[1:n], 2000
+    c.chosen[0] = c.token[2]
+    return c
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("scales", [[120], [118, 119, 120], [-100, 0, 120]])
+def test_values_past_fp32(lib, scales, whole):
+    """A finite code under a scale of up to 2^120 moves as what it stands for, although fp32 does not hold that."""
+    for seed, P in ((70, 16), (71, 32)):
+        c = near_the_largest(seed, P, 64, scales, whole)
+        exp = c.expect()
+        # the append's rule asks for no larger scale than the codes come from, so none of them is lost
+        assert max(float(exp[0][i].max()) for i in (1, 3)) <= 2.0 ** max(scales)
+        c.check(accept(lib, c, ORDERS[0]), exp)
