@@ -578,8 +578,9 @@ er_status er_hip_kv8_attention_masked_workspace(er_hip_ctx *ctx, const er_kv8_ca
  * path (int32 [rows]): the kept rows of each sequence, in the places of its
  * first rows, -1 in those of the others; count, next, kv_len (int32
  * [sequences]): how many they are, the token chosen at the last one (no row:
- * -1), and the tokens that the sequence now has.  Rows of no sequence are left
- * as they were.  Outputs overlap neither each other nor what the call reads
+ * -1), and the tokens that the sequence now has; these are written for each
+ * sequence of a batch without rows too, whose arrays of rows are not looked at.
+ * Rows of no sequence are left as they were.  Outputs overlap neither each other nor what the call reads
  * (kv_len is not the batch's own): INVALID_ARGUMENT.  Other errors as
  * er_hip_kv8_append's. */
 er_status er_hip_kv8_accept(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache, const er_kv8_batch *batch,

@@ -1,5 +1,6 @@
 """Acceptance of drafts at the ends of its range: values next to fp32's largest,
 and pages that are missing in front of ones that are there."""
+import numpy as np
 import pytest
 
 from test_accept_schedule import near_the_largest
@@ -32,3 +33,22 @@ def test_pages_around_gaps(ctx, d, P, heads):
         exp = c.expect()
         assert list(exp[1][1]) == [9 * P - 1, 5 * P - 1]
         c.check(c.run(), exp)
+
+
+@pytest.mark.parametrize("max_len", [None, 20])
+def test_idle_sequences(ctx, max_len):
+    """A batch without a single row: what an earlier step left in counts, tokens and lengths does not stay."""
+    c = Case(ctx, 3, [33, 0, 5], [0, 0, 0], 16, 64, 2, behind=4)
+    c.upload()
+    full = c.b.upload(ctx, max_len=max_len)
+    c.b.total = 0
+    idle = c.b.upload(ctx, max_rows=0, max_len=max_len)
+    for batch in (full, idle):
+        for x in c.out:
+            x.upload(np.full(x.length // 4, -77, np.int32))
+        c.encode(batch)
+        ctx.synchronize()
+        cache, (path, count, after, left) = c.state()
+        assert np.all(path == -77) and list(count) == [0, 0, 0] and list(after) == [-1, -1, -1]
+        assert list(left) == [min(33, max_len or 33), 0, 5]
+        assert all(np.array_equal(a, b) for a, b in zip(cache, c.before))
