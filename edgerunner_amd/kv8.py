@@ -138,14 +138,19 @@ class KV8AttentionKernel(_Kernel):
 
     entry = "er_hip_kv8_attention"
 
-    def workspaceBytes(self, cache: KV8Cache, batch: KV8Batch, qHeads: int) -> int:
-        """Bytes of scratch that encode needs for such a batch, whatever its window, masks and output type."""
-        n, masked = C.c_uint64(), C.c_uint64()
-        check(self.lib.er_hip_kv8_attention_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(n)),
-              self.lib)
-        check(self.lib.er_hip_kv8_attention_masked_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(masked)),
-              self.lib)
-        return max(int(n.value), int(masked.value))
+    def workspaceBytes(self, cache: KV8Cache, batch: KV8Batch, qHeads: int, masked: Optional[bool] = None) -> int:
+        """Bytes of scratch that encode needs for such a batch, whatever its window and output type: with masks (sinks or
+        drafts), without (False: often fewer), or for either (None; a batch that masked calls refuse, as it has
+        too many steps to count, has the other's)."""
+        n, m = C.c_uint64(), C.c_uint64()
+        if not masked:
+            check(self.lib.er_hip_kv8_attention_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(n)),
+                  self.lib)
+        if masked is not False:
+            status = self.lib.er_hip_kv8_attention_masked_workspace(self.ctx.handle, cache.ref, batch.ref, qHeads, C.byref(m))
+            if masked:
+                check(status, self.lib)
+        return max(int(n.value), int(m.value))
 
     def encode(self, stream: Optional[Stream], cache: KV8Cache, batch: KV8Batch, q: HeadRows, out: HeadRows,
                scale: float, window: int = 0, workspace: Optional[Buffer] = None, outBF16: bool = False, sinks: int = 0,
