@@ -89,7 +89,7 @@ struct MaskedPlan : AttendPlan {
     uint32_t blocks;  // of 16 columns that a wave has; 0: the wide kernel
 };
 MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t group, uint32_t window, int cu, uint32_t sinks,
-                       bool drafts) {
+                       bool drafts, bool half) {
     MaskedPlan p{};
     const uint64_t cols = (uint64_t)b->max_rows * group, full = most_tokens(c, b);
     // Shares against the wide kernel, us: trees of 128 columns of 32 sequences of up to 6000 tokens 149 / 196, of 192
@@ -120,8 +120,13 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     const uint64_t most = (span + 63) / 64, units = (uint64_t)b->sequences * c->kv_heads * p.tiles;
     const bool whole = c->head_dim < 256 && most <= 40 && units * 64 >= most * (uint64_t)cu && units <= kMostBlocks;
     if (span > kUnshared && !whole) {
-        p.shares = (uint32_t)cu * 2;  // two workgroups a CU are resident
-        p.parts = 2ull * p.shares * 16 * p.blocks;
+        // Two workgroups a CU are resident; of the kernel whose registers leave a SIMD one wave (wide heads, two pages a
+        // tile, two terms), one.  By one / two a CU, us: a user's 26 drafts behind 8000 tokens 25.3 / 33.6, 32 users' next
+        // tokens behind 8000 69 / 82, trees of 100 of 8 of 4000 74.6 / 83.4, of 5 of 64 of 1000 29.5 / 37.7, of 5 of 8
+        // of 2000 19.0 / 18.8.
+        const bool one = c->head_dim == 256 && c->page_tokens == 16 && !half;
+        p.shares = (uint32_t)cu * (one ? 1 : 2);
+        p.parts = 4ull * (uint32_t)cu * 16 * p.blocks;  // of either output type
     }
     return p;
 }
@@ -220,7 +225,7 @@ er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const e
         a.words = drafts->seen_words;
         a.position = (const int32_t *)drafts->position.data;
     }
-    const MaskedPlan p = plan_masked(cache, batch, a.group, a.window, cu_count_of(ctx), a.sinks, drafts != nullptr);
+    const MaskedPlan p = plan_masked(cache, batch, a.group, a.window, cu_count_of(ctx), a.sinks, drafts != nullptr, a.half);
     a.shares = p.shares;
     a.splits = p.splits, a.chunk = p.chunk, a.tiles = p.tiles;
     const DraftKernels &kernels = draft_of(ctx);
@@ -249,7 +254,7 @@ er_status er_hip_kv8_attention_masked_workspace(er_hip_ctx *ctx, const er_kv8_ca
     if (st == ER_OK) st = check_ctx(ctx);
     if (st != ER_OK) return st;
     if (batch->rows == 0 || batch->sequences == 0) return ER_OK;
-    const MaskedPlan p = plan_masked(cache, batch, q_heads / cache->kv_heads, 0, cu_count_of(ctx), 0, false);
+    const MaskedPlan p = plan_masked(cache, batch, q_heads / cache->kv_heads, 0, cu_count_of(ctx), 0, false, false);
     *bytes = p.parts * (cache->head_dim + 2) * 4;
     return ER_OK;
 }

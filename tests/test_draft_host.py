@@ -1,9 +1,11 @@
 """What the host of the operators on drafts and logits launches and refuses
 beyond test_draft_abi.py, whose calls and recorded runtime it shares: no GPU."""
+import ctypes as C
+
 import pytest
 
 from edgerunner_amd import _ffi
-from test_draft_abi import ENC, NULL, accept, batch, buf, drafts, launches
+from test_draft_abi import BF16, ENC, F32, NULL, accept, attend, batch, buf, cache, launches, ref, rows
 from test_draft_abi import ctx, host  # noqa: F401  (fixtures)
 
 
@@ -23,3 +25,14 @@ def test_acceptance_of_idle_sequences(host, ctx):  # noqa: F811
         assert accept(b=idle, **on, **{part: buf(8, 2 << 40)}) != 0, part  # the batch's lengths
     assert accept(b=batch(0, 0, 0), **on) == 0
     assert launches(host) == []
+
+
+@pytest.mark.parametrize("d,P,out,grid", [(256, 16, F32, 256), (256, 16, BF16, 512), (256, 32, F32, 512), (128, 16, F32, 512)])
+def test_shares_are_as_many_as_the_chip_holds(host, ctx, d, P, out, grid):  # noqa: F811
+    """One workgroup a CU of the kernel that leaves room for one, two of the others, in the workspace of either type."""
+    c, b, n = cache(4000, 2, P, d), batch(2, 6, 4, 4000, P), C.c_uint64()
+    assert host.er_hip_kv8_attention_masked_workspace(ctx, ref(c), ref(b), 4, C.byref(n)) == 0
+    assert n.value == 2 * 512 * 16 * (d + 2) * 4
+    q, o = rows(4, 6, 5 << 50, d), rows(4, 6, 6 << 50, d, 2 if out == BF16 else 4)
+    assert attend(c, b, q, o, ot=out, ws=buf(n.value, 7 << 50), lib=host, ctx=ctx) == 0, host.stub_error()
+    assert launches(host)[0][0] == grid
