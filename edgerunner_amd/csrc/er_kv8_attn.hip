@@ -15,16 +15,16 @@
 // the products formed twice; for bf16 output one term (11 bits, to bf16's 8)
 // does.  Sums, maxima and outputs are fp32 throughout.
 //
-// The running maximum is a reference that only moves when a score passes it
-// by more than 2 (in powers of two); weights are 2^(s - m + 13), so at most
-// 2^15, and the reference cancels in the quotient.  Most tiles rescale nothing.
-// fp16's smallest step, 2^-24, is then 2^-37 of the row's largest weight at the
+// Weights are 2^(s - m).  The reference m is set 13 (in powers of two) below the
+// running maximum and only moves when a score is more than 15 above it, so
+// weights are at most 2^15; it cancels in the quotient.  Most tiles rescale
+// nothing.  fp16's smallest step, 2^-24, is then 2^-37 of the row's largest weight at the
 // most: what the rounding of smaller weights leaves out of 2^18 tokens is 2^-20
-// of their values.  By 8 and + 7, which rescales less, it was 2^-14; a prompt of
+// of their values.  By 7 and 15, which rescales less, it was 2^-14; a prompt of
 // 4096 rows then took 183.4 us where it takes 185.3 so.
 
-#define ER_SLACK 2.0f
 #define ER_LIFT 13.0f
+#define ER_ROOM 15.0f
 #define ER_NO_MAX (-3.0e38f)  // reference of a column that has seen no score
 
 ER_DEV f32x4 mfma16(h8 a, h8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -342,7 +342,13 @@ ER_DEV Reach reach_of(const A &p, const Spans &w) {
 }
 ER_DEV int token_of(const Reach &r, int x) { return x < r.head ? x : x + r.skip; }
 
-// Moves a column's reference up to its scores' largest.
+// The reference below a column's largest score.  From 2^24 on fp32's steps may make 16 of the 13, by which weights
+// would leave fp16: there, and past them, scores are so far apart that the largest is the reference itself.
+ER_DEV float reference_of(float top) {
+    const float m = top - ER_LIFT;
+    return top - m > ER_LIFT + 1.0f ? top : m;
+}
+// Moves a column's reference up.
 template <int N, typename ACC>
 ER_DEV void raise_reference(float to, float &m, float &l, ACC (&o)[N]) {
     const float f = __builtin_amdgcn_exp2f(m - to);
@@ -429,7 +435,7 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
     const float f0 = score_factor(qf, ok0 ? t.ks[0] : t.ks[1]), f1 = score_factor(qf, ok1 ? t.ks[1] : t.ks[0]);
     const float top = fmaxf(fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[0].z, s[0].w)) * f0,
                             fmaxf(fmaxf(s[1].x, s[1].y), fmaxf(s[1].z, s[1].w)) * f1);
-    if (__any(top > st.m + ER_SLACK)) raise_reference(fmaxf(st.m, column_max4(top)), st.m, st.l, st.o);
+    if (__any(top - st.m > ER_ROOM)) raise_reference(fmaxf(st.m, reference_of(column_max4(top))), st.m, st.l, st.o);
     const float vs0 = ok0 ? t.vs[0] : t.vs[1], vs1 = ok1 ? t.vs[1] : t.vs[0];
     if constexpr (MASKED) {
         ScaleRange r = {0u, ~0u};
@@ -439,10 +445,10 @@ ER_DEV void attend_narrow(NarrowState<D> &st, NarrowTile<D> &t, const h8 (&qb)[T
     } else if (fmaxf(vs0, vs1) > st.vref) {
         raise_scale(fmaxf(vs0, vs1), st.vref, st.vinv, st.o);
     }
-    const float v0 = vs0 * st.vinv, v1 = vs1 * st.vinv, base = st.m - ER_LIFT;
+    const float v0 = vs0 * st.vinv, v1 = vs1 * st.vinv;
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(s[i / 4][i & 3] * (i < 4 ? f0 : f1) - base);
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(s[i / 4][i & 3] * (i < 4 ? f0 : f1) - st.m);
     st.l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     h8 b[TERMS];
     weight_terms<TERMS>(x, b);
@@ -1178,14 +1184,13 @@ ER_DEV void kv8_attend_wide(const A &p, WideLds<D> *lds, uint32_t (*drafts)[ER_D
                     for (int j = 1; j < 8; ++j) peak = fmaxf(peak, sc[8 * i + j]);
                     top = fmaxf(top, peak * f[i]);
                 }
-                if (__any(top > m + ER_SLACK)) raise_reference(fmaxf(m, column_max2(top)), m, l, o);
-                const float base = m - ER_LIFT;
+                if (__any(top - m > ER_ROOM)) raise_reference(fmaxf(m, reference_of(column_max2(top))), m, l, o);
                 h8 wb[2][TERMS];
 #pragma unroll
                 for (int sl = 0; sl < 2; ++sl) {
                     float e[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(sc[8 * sl + i] * f[sl] - base);
+                    for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(sc[8 * sl + i] * f[sl] - m);
                     l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
                     weight_terms<TERMS>(e, wb[sl]);
                 }

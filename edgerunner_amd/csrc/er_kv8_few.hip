@@ -128,12 +128,12 @@ ER_DEV void attend_few(FewState<D, NB> &st, NarrowTile<D> &t, const h8 (&qb)[NB]
         f1[b] = score_factor(qf[b], ks1);
         top[b] = fmaxf(fmaxf(fmaxf(s[b][0].x, s[b][0].y), fmaxf(s[b][0].z, s[b][0].w)) * f0[b],
                        fmaxf(fmaxf(s[b][1].x, s[b][1].y), fmaxf(s[b][1].z, s[b][1].w)) * f1[b]);
-        above |= top[b] > st.m[b] + ER_SLACK;
+        above |= top[b] - st.m[b] > ER_ROOM;
     }
     if (__any(above)) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float to = fmaxf(st.m[b], column_max4(top[b])), f = __builtin_amdgcn_exp2f(st.m[b] - to);
+            const float to = fmaxf(st.m[b], reference_of(column_max4(top[b]))), f = __builtin_amdgcn_exp2f(st.m[b] - to);
             st.m[b] = to;
             st.l[b] *= f;
 #pragma unroll
@@ -148,10 +148,9 @@ ER_DEV void attend_few(FewState<D, NB> &st, NarrowTile<D> &t, const h8 (&qb)[NB]
     h8 weights[NB][TERMS];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const float base = st.m[b] - ER_LIFT;
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(s[b][i / 4][i & 3] * (i < 4 ? f0[b] : f1[b]) - base);
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(s[b][i / 4][i & 3] * (i < 4 ? f0[b] : f1[b]) - st.m[b]);
         st.l[b] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         weight_terms<TERMS>(x, weights[b]);
     }

@@ -511,7 +511,8 @@ er_status er_hip_kv8_append(er_hip_ctx *ctx, er_stream stream, const er_kv8_cach
  * (q->heads / kv_heads), w = softmax(scale * q . k_t).  q fp32; out of
  * out_type ER_TYPE_F32 (products of fp32 accuracy) or ER_TYPE_BF16 (queries
  * and weights rounded to fp16 for the products); either holds a weight to
- * 2^-38 of its row's largest.  A row that no token is
+ * 2^-38 of its row's largest (2^-25 where scores pass 2^25, between which fp32
+ * has steps of 4 and more).  A row that no token is
  * visible to gets zeros.  out does not overlap q.
  * workspace: scratch of er_hip_kv8_attention_workspace bytes (which depend on
  * the batch's and cache's sizes and q_heads alone), 16-byte aligned; calls and
