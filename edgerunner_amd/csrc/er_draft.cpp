@@ -114,6 +114,8 @@ MaskedPlan plan_masked(const er_kv8_cache *c, const er_kv8_batch *b, uint32_t gr
     // 1600 98 / 59; of 2000: 64 15.4 / 17.9, 128 17.6 / 18.0 and 20.5 / 19.2, 256 28.2 / 20.3, 512 51.9 / 38.9 and 32.9 /
     // 32.7; under a window of 2048: 512 64.2 / 54.1 and 46.0 / 36.1, 384 32.4 / 35.0; of 4000: 128 24.8 / 28.4, 256 44.9 /
     // 38.8, but 512 44.5 / 56.2, as the longest unit then decides.  At width 256 64 of 1000 17.6 / 24.5, 512 44.1 / 46.6.
+    // The longest unit and their number do not tell all of these apart: the rule is wrong for 384 under the window (by 8%)
+    // and for 256 of 4000 (by 16%).
     uint64_t span = full;
     if (window)
         span = std::min<uint64_t>(span, (uint64_t)window + b->max_rows + 127 + (((uint64_t)sinks + 63) & ~63ull));

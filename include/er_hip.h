@@ -556,9 +556,13 @@ typedef struct er_drafts {
  * window, and of the rows those that `seen` says, whatever the window; reads
  * seen and, where window is not 0, position, which counts as no less than the
  * first row's token (kv_len - n) and no more than the last's.  A row that
- * nothing is visible to gets zeros.  Types, precision, limits and errors are
- * er_hip_kv8_attention's, and so are the rules of workspace, whose bytes
- * er_hip_kv8_attention_masked_workspace gives. */
+ * nothing is visible to gets zeros.  out_type F32: products of fp32 accuracy;
+ * BF16: queries and softmax weights are rounded to fp16 for the products, as
+ * er_hip_kv8_attention's, whose other statements on precision, limits and errors hold too, and so do the rules of
+ * workspace, whose bytes er_hip_kv8_attention_masked_workspace gives.  Batches
+ * whose 64-token steps (16 more a sequence) times heads and blocks of 16 columns pass
+ * 2^32 - 1 -> INVALID_VECTOR_SHAPE, where a head has at most 128 columns (rows times
+ * query heads; 256 of width 256) and sequences more than 512 tokens. */
 er_status er_hip_kv8_attention_masked(er_hip_ctx *ctx, er_stream stream, const er_kv8_cache *cache,
                                       const er_kv8_batch *batch, const er_head_rows *q, const er_head_rows *out,
                                       uint32_t out_type, float scale, uint32_t window, uint32_t sinks,
