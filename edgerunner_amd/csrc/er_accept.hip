@@ -73,7 +73,7 @@ ER_DEV void accept_moves(const ErAcceptArgs &p, const Sequence &q, uint32_t s, u
         const int t0 = max(first, begin), t1 = min(last, begin + P);
         const int page = uniform(page_of(p.b, p.c, s, begin));
         if (page < 0) continue;
-        // Only a page that goes on to the barrier takes the other copy of the needs: so one lies between two uses of a copy.
+        // Only a page that goes on to the barrier takes the other copy of the needs: two uses of a copy have a barrier between.
         turn ^= 1u;
         uint32_t c[PASSES];
         float f[PASSES];  // -1: nothing to write
